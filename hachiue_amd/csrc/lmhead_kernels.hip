@@ -238,6 +238,7 @@ hipError_t prepare_gemv() {
       e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize,
                               (int)gemv_tern_lds_bytes(kGemvMaxK));
   if (e == hipSuccess) e = prepare_gemv_batch();
+  if (e == hipSuccess) e = prepare_verify();
   return e;
 }
 

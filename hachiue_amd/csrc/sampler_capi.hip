@@ -122,6 +122,29 @@ struct DevBuf {
   }
 };
 
+// Grow-only device buffer whose memory stays where it is, however it grows:
+// a captured graph keeps the addresses of its call.  (It doubles at least, so
+// what it left behind is less than what it holds.)
+struct KeptBuf {
+  DevBuf b;
+  std::vector<void *> left;
+  hipError_t ensure(size_t need) {
+    if (need <= b.bytes) return hipSuccess;
+    DevBuf n;
+    left.reserve(left.size() + 1);   // (before anything is allocated)
+    const hipError_t e = n.ensure(need > 2 * b.bytes ? need : 2 * b.bytes);
+    if (e != hipSuccess) return e;
+    if (b.p) left.push_back(b.p);
+    b = n;
+    return hipSuccess;
+  }
+  void release() {
+    for (void *p : left) (void)hipFree(p);
+    left.clear();
+    b.release();
+  }
+};
+
 // Grow-only pinned host buffer (hipHostMalloc: the device reads and writes it
 // directly, and copies from it are truly asynchronous).
 struct PinBuf {
@@ -157,6 +180,12 @@ constexpr size_t kPinLogitsMax = size_t(64) << 20;
 // memory and none back.
 constexpr size_t kZeroCopyMax = size_t(4) << 20;
 constexpr size_t pin_align(size_t b) { return (b + 255) / 256 * 256; }
+
+// Workspaces that a context has from its creation on: of 64 sequences with 8
+// drafts over 262144 logits, and of 4096 rows with adapters of rank 64.
+constexpr size_t kVerifyWorkBytes = size_t(1) << 20;
+constexpr size_t kVerifyCountBytes = size_t(16) << 10;
+constexpr size_t kLoraWorkBytes = size_t(1) << 20;
 
 // Routing of rows to kernels, uploaded next to the plans.
 struct Routing {
@@ -199,6 +228,8 @@ struct hs_context {
   // vector-unit weights (F32, Q4_0, Q4_1).  (Calls whose GEMV reads the
   // weights once for several rows, gemv_batched: two launches always.)
   int fuse = 1;
+  KeptBuf verify_ws, verify_cnt;   // verification of drafts (verify_cnt: zero between calls)
+  KeptBuf lora_t;               // x A^T of the adapters' rows
   DevBuf minp_cand, minp_meta;  // split min-p rows' hand-over (counted in by split_cnt)
   DevBuf large_retry;           // two-pass large-k rows handed back
   DevBuf large_replay;          // slot-history replays asked for by the large-k kernel
@@ -245,6 +276,11 @@ struct hs_context {
                                            //   whether a large row has k > kReplayMaxK
   uint64_t na_gen = 0;
 };
+
+// Every entry point that uses a context holds its mutex for the whole call.
+#define HS_LOCK(ctx)                                                   \
+  if (!(ctx)) return fail(HS_ERR_INVALID_ARGUMENT, "null context");    \
+  std::lock_guard<std::mutex> hs_lock_((ctx)->mu)
 
 namespace {
 
@@ -811,6 +847,14 @@ int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const 
   return HS_OK;
 }
 
+// Whether `s` is being captured.  Such a call neither waits for the context's
+// earlier calls nor leaves an event behind (neither may cross a capture's
+// border) and takes no timing events.
+bool is_capturing(hipStream_t s) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(s, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+}
+
 // Start/end events of timing slot `slot` for the call's one kernel, when
 // timing is on (null otherwise).
 int timed_slot(hs_context *ctx, int slot, hipEvent_t **ev) {
@@ -832,25 +876,48 @@ int timed_slot(hs_context *ctx, int slot, hipEvent_t **ev) {
   return HS_OK;
 }
 
+// The same for a call's two kernels (one timed call).
+int timed_pair(hs_context *ctx, int first, int second, hipEvent_t **ev1, hipEvent_t **ev2) {
+  *ev1 = *ev2 = nullptr;
+  if (!ctx->timing) return HS_OK;
+  hs_context::TimedCall tc{};
+  tc.mask = 1u << first | 1u << second;
+  for (int slot : {first, second})
+    for (int i = 0; i < 2; ++i) {
+      if (ctx->ev_free.empty()) {
+        hipEvent_t x;
+        HS_HIP(hipEventCreate(&x));
+        ctx->ev_free.push_back(x);
+      }
+      tc.ev[2 * slot + i] = ctx->ev_free.back();
+      ctx->ev_free.pop_back();
+    }
+  ctx->timed.push_back(tc);
+  *ev1 = ctx->timed.back().ev + 2 * first;
+  *ev2 = ctx->timed.back().ev + 2 * second;
+  return HS_OK;
+}
+
 int gemv_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *wt,
                 float *d_y, int64_t ldy, hipStream_t stream) {
   if (!ctx) return fail(HS_ERR_INVALID_ARGUMENT, "null context");
   DeviceGuard guard(ctx->device);
-  int rc = enter_stream(ctx, stream);
+  const bool cap = is_capturing(stream);
+  int rc = cap ? HS_OK : enter_stream(ctx, stream);
   if (rc) return rc;
   hs::GemvArgs g;
   bool skip = false;
   rc = gemv_setup(ctx, d_x, M, ldx, wt, d_y, ldy, stream, g, &skip);
   if (rc || skip) return rc;   // nothing was enqueued
   hipEvent_t *ev = nullptr;
-  rc = timed_slot(ctx, hs::kGemvTimedSlot, &ev);
+  if (!cap) rc = timed_slot(ctx, hs::kGemvTimedSlot, &ev);
   if (rc) return rc;
-  const hipError_t e = hs::launch_gemv(g, stream, ev, ctx->done_ev);
+  const hipError_t e = hs::launch_gemv(g, stream, ev, cap ? nullptr : ctx->done_ev);
   if (e != hipSuccess) {
-    (void)leave_stream(ctx, stream, false);
+    if (!cap) (void)leave_stream(ctx, stream, false);
     return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
   }
-  return leave_stream(ctx, stream, ev == nullptr);
+  return cap ? HS_OK : leave_stream(ctx, stream, ev == nullptr);
 }
 
 // Plans and routing lists written into fixed arrays (no allocation): the
@@ -1095,12 +1162,344 @@ int sample_host_zero_copy(hs_context *ctx, float *logits, size_t lbytes, int32_t
   return HS_OK;
 }
 
-}  // namespace
 
-// Every entry point that uses a context holds its mutex for the whole call.
-#define HS_LOCK(ctx)                                                   \
-  if (!(ctx)) return fail(HS_ERR_INVALID_ARGUMENT, "null context");    \
-  std::lock_guard<std::mutex> hs_lock_((ctx)->mu)
+// ---- verification of drafted tokens, low-rank adapters
+
+int kept_room(KeptBuf &b, size_t need, bool cap) {
+  if (need <= b.b.bytes) return HS_OK;
+  if (cap)
+    return fail(HS_ERR_UNSUPPORTED,
+                "a captured call of this size needs one outside of the capture first");
+  try {
+    HS_HIP(b.ensure(need));
+  } catch (const std::bad_alloc &) {
+    return fail(HS_ERR_OUT_OF_MEMORY, "host allocation failed");
+  }
+  return HS_OK;
+}
+
+// The calls below check their arguments before they take the context.
+
+// The checks that both forms of the verification share; *skip: nothing to do.
+int draft_args(const hs_draft_batch *b, const hs_decode_state *st, hs::DraftArgs &d, bool *skip) {
+  if (!b) return fail(HS_ERR_INVALID_ARGUMENT, "null draft batch");
+  if (b->seqs < 0) return fail(HS_ERR_INVALID_ARGUMENT, "seqs must be >= 0 (got %d)", b->seqs);
+  if (b->max_drafts < 0 || b->max_drafts > hs::kVerifyMaxDrafts)
+    return fail(HS_ERR_INVALID_ARGUMENT, "max_drafts must be in [0, %d] (got %d)",
+                hs::kVerifyMaxDrafts, b->max_drafts);
+  if (b->n_drafts < 0 || b->n_drafts > (int64_t)b->seqs * b->max_drafts)
+    return fail(HS_ERR_INVALID_ARGUMENT, "n_drafts must be in [0, seqs * max_drafts] (got %lld)",
+                (long long)b->n_drafts);
+  if (!b->offsets && b->n_drafts != (int64_t)b->seqs * b->max_drafts)
+    return fail(HS_ERR_INVALID_ARGUMENT, "without offsets n_drafts must be seqs * max_drafts");
+  *skip = b->seqs == 0;
+  if (*skip) return HS_OK;
+  if (b->seqs > 65535) return fail(HS_ERR_UNSUPPORTED, "seqs %d above 65535", b->seqs);
+  if (!b->uniforms || !b->tokens || !b->counts)
+    return fail(HS_ERR_INVALID_ARGUMENT, "uniforms, tokens and counts must not be null");
+  if (b->n_drafts > 0 && !b->drafts)
+    return fail(HS_ERR_INVALID_ARGUMENT, "drafts must not be null");
+  memset(&d, 0, sizeof d);
+  d.seqs = b->seqs;
+  d.max_drafts = b->max_drafts;
+  d.n_drafts = b->n_drafts;
+  d.off = b->offsets;
+  d.drafts = b->drafts;
+  d.uniforms = b->uniforms;
+  d.tokens = b->tokens;
+  d.counts = b->counts;
+  d.accept = b->accept;
+  if (!st) return HS_OK;
+  if (!st->ring || !st->len || !st->done)
+    return fail(HS_ERR_INVALID_ARGUMENT, "ring, len and done must not be null");
+  if (st->ring_cap < 128 || st->ring_cap > (int64_t(1) << 29))
+    return fail(HS_ERR_INVALID_ARGUMENT, "ring_cap must be in [128, 2^29] (got %lld)",
+                (long long)st->ring_cap);
+  if (st->n_stop < 0 || st->n_stop > hs::kMaxStopIds)
+    return fail(HS_ERR_INVALID_ARGUMENT, "n_stop must be in [0, %d] (got %d)", hs::kMaxStopIds,
+                st->n_stop);
+  if (st->n_stop > 0 && !st->stop_ids)
+    return fail(HS_ERR_INVALID_ARGUMENT, "stop ids must not be null");
+  d.ring = st->ring;
+  d.cap = st->ring_cap;
+  d.len = st->len;
+  d.done = st->done;
+  d.stop = st->stop_ids;
+  d.nstop = st->n_stop;
+  return HS_OK;
+}
+
+int verify_side(const hs_distribution *x, const char *what, int32_t vocab, hs::VerifyArgs &a, int side) {
+  if (x->kind != HS_DIST_LOGITS && x->kind != HS_DIST_PROBS)
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s distribution of unknown kind %d", what, x->kind);
+  if (x->row_stride < vocab)
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s row stride %lld below the vocabulary", what,
+                (long long)x->row_stride);
+  if (!x->data || (reinterpret_cast<uintptr_t>(x->data) & 3u))
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s rows must be given, 4-byte aligned", what);
+  a.rows[side] = x->data;
+  a.stride[side] = x->row_stride;
+  a.kind[side] = x->kind;
+  a.temps[side] = x->kind == HS_DIST_LOGITS ? x->temperatures : nullptr;
+  return HS_OK;
+}
+
+int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distribution *draft,
+                  int32_t vocab, const hs_draft_batch *batch, const hs_decode_state *state,
+                  hipStream_t stream) {
+  hs::VerifyArgs a;
+  memset(&a, 0, sizeof a);
+  bool skip = false;
+  int rc = draft_args(batch, state, a.d, &skip);
+  if (rc) return rc;
+  if (!target) return fail(HS_ERR_INVALID_ARGUMENT, "null target distribution");
+  if (vocab < 1 || vocab > hs::kVerifyMaxVocab)
+    return fail(HS_ERR_INVALID_ARGUMENT, "vocab must be in [1, %d] (got %d)", hs::kVerifyMaxVocab,
+                vocab);
+  if (skip) return HS_OK;
+  rc = verify_side(target, "target", vocab, a, 0);
+  if (rc) return rc;
+  a.kind[1] = hs::kDistNone;
+  if (draft) {   // (without drafts there is no row to ask for)
+    if (batch->n_drafts > 0) rc = verify_side(draft, "draft", vocab, a, 1);
+    else a.kind[1] = hs::kDistProbs;
+    if (rc) return rc;
+  }
+  a.vocab = vocab;
+  a.chunks = (vocab + hs::kVerifyChunk - 1) / hs::kVerifyChunk;
+  const size_t rows[2] = {(size_t)a.d.n_drafts + (size_t)a.d.seqs, (size_t)a.d.n_drafts};
+  const size_t judged = (size_t)a.d.seqs * (size_t)(a.d.max_drafts + 1);
+  size_t need = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = need;
+    need += pin_align(bytes);
+    return at;
+  };
+  size_t part[2] = {0, 0}, stat[2] = {0, 0};
+  for (int i = 0; i < 2; ++i)
+    if (a.kind[i] == hs::kDistLogits) {
+      part[i] = take(rows[i] * (size_t)a.chunks * sizeof(hs::VerifyPart));
+      stat[i] = take(rows[i] * sizeof(hs::VerifyStat));
+    }
+  const size_t verdict = take(judged * sizeof(hs::Verdict));
+  const size_t mass = take((size_t)a.d.seqs * (size_t)a.chunks * sizeof(double));
+  const size_t counts = judged + 2 * (size_t)a.d.seqs;
+  HS_LOCK(ctx);
+  DeviceGuard guard(ctx->device);
+  const bool cap = is_capturing(stream);
+  rc = kept_room(ctx->verify_ws, need, cap);
+  if (rc) return rc;
+  if (!cap) rc = enter_stream(ctx, stream);
+  if (rc) return rc;
+  if (counts * sizeof(uint32_t) > ctx->verify_cnt.b.bytes) {
+    rc = kept_room(ctx->verify_cnt, counts * sizeof(uint32_t), cap);
+    if (rc) return rc;
+    const hipError_t e = inject_failure()
+                             ? hipErrorOutOfMemory
+                             : hs::launch_fill_u32(static_cast<uint32_t *>(ctx->verify_cnt.b.p),
+                                                   (int64_t)(ctx->verify_cnt.b.bytes / 4), 0u, stream);
+    if (e != hipSuccess) {
+      ctx->verify_cnt.b.release();
+      return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
+    }
+  }
+  char *ws = static_cast<char *>(ctx->verify_ws.b.p);
+  for (int i = 0; i < 2; ++i)
+    if (a.kind[i] == hs::kDistLogits) {
+      a.part[i] = reinterpret_cast<hs::VerifyPart *>(ws + part[i]);
+      a.stat[i] = reinterpret_cast<hs::VerifyStat *>(ws + stat[i]);
+    }
+  a.verdict = reinterpret_cast<hs::Verdict *>(ws + verdict);
+  a.mass = reinterpret_cast<double *>(ws + mass);
+  a.arrived = static_cast<uint32_t *>(ctx->verify_cnt.b.p);
+  a.rejected = a.arrived + judged;
+  a.arrived_final = a.rejected + a.d.seqs;
+  hipEvent_t *ev1 = nullptr, *ev2 = nullptr;
+  if (!cap) {
+    if (a.kind[0] == hs::kDistLogits || a.kind[1] == hs::kDistLogits) {
+      rc = timed_pair(ctx, hs::kStatsTimedSlot, hs::kResolveTimedSlot, &ev1, &ev2);
+    } else {
+      rc = timed_slot(ctx, hs::kResolveTimedSlot, &ev2);
+    }
+    if (rc) return rc;
+  }
+  const hipError_t e = hs::launch_verify(a, stream, ev1, ev2, cap ? nullptr : ctx->done_ev);
+  if (e != hipSuccess) {
+    // the first launch may have left its counts behind
+    if (!cap) {
+      (void)hs::launch_fill_u32(a.arrived, (int64_t)counts, 0u, stream);
+      (void)leave_stream(ctx, stream, false);
+    }
+    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
+  }
+  return cap ? HS_OK : leave_stream(ctx, stream, ev2 == nullptr);
+}
+
+int list_side(const hs_candidates *x, const char *what, hs::ListArgs &a, int side) {
+  if (x->stride < 1 || x->stride > hs::kVerifyMaxList)
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s candidate stride must be in [1, %d] (got %d)", what,
+                hs::kVerifyMaxList, x->stride);
+  if (!x->ids || !x->probs || !x->kept)
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s candidate ids, probabilities and lengths must be given",
+                what);
+  a.ids[side] = x->ids;
+  a.probs[side] = x->probs;
+  a.kept[side] = x->kept;
+  a.tokens[side] = x->tokens;
+  a.stride[side] = x->stride;
+  return HS_OK;
+}
+
+int verify_candidates(hs_context *ctx, const hs_candidates *target, const hs_candidates *draft,
+                      const hs_draft_batch *batch, const hs_decode_state *state,
+                      hipStream_t stream) {
+  hs::ListArgs a;
+  memset(&a, 0, sizeof a);
+  bool skip = false;
+  int rc = draft_args(batch, state, a.d, &skip);
+  if (rc) return rc;
+  if (!target) return fail(HS_ERR_INVALID_ARGUMENT, "null target candidates");
+  if (skip) return HS_OK;
+  rc = list_side(target, "target", a, 0);
+  if (rc) return rc;
+  a.certain = !draft || batch->n_drafts == 0;
+  if (!a.certain) rc = list_side(draft, "draft", a, 1);
+  if (rc) return rc;
+  HS_LOCK(ctx);
+  DeviceGuard guard(ctx->device);
+  const bool cap = is_capturing(stream);
+  // (the histories may be another call's)
+  if (!cap) rc = enter_stream(ctx, stream);
+  if (rc) return rc;
+  hipEvent_t *ev = nullptr;
+  if (!cap) rc = timed_slot(ctx, hs::kListsTimedSlot, &ev);
+  if (rc) return rc;
+  const hipError_t e = hs::launch_verify_lists(a, stream, ev, cap ? nullptr : ctx->done_ev);
+  if (e != hipSuccess) {
+    if (!cap) (void)leave_stream(ctx, stream, false);
+    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
+  }
+  return cap ? HS_OK : leave_stream(ctx, stream, ev == nullptr);
+}
+
+// The checks of an adapter call; *skip: nothing to do.
+int lora_args(const float *d_x, int32_t M, int64_t ldx, const hs_adapters *ad, const int32_t *d_slots,
+              const float *d_base, int64_t ldb, float *d_y, int64_t ldy, hs::LoraArgs &g, bool *skip) {
+  if (!ad) return fail(HS_ERR_INVALID_ARGUMENT, "null adapters");
+  if (ad->type != hs::kA_F32 && ad->type != hs::kA_F16 && ad->type != hs::kA_BF16)
+    return fail(HS_ERR_UNSUPPORTED, "adapter type %d is not supported", ad->type);
+  if (ad->count < 0 || ad->cols < 1 || ad->rows < 0 || ad->rank < 1)
+    return fail(HS_ERR_INVALID_ARGUMENT, "adapters of count %d, rank %d, %d x %d", ad->count, ad->rank,
+                ad->rows, ad->cols);
+  if (ad->rank > hs::kLoraMaxRank)
+    return fail(HS_ERR_UNSUPPORTED, "adapter rank %d above %d", ad->rank, hs::kLoraMaxRank);
+  if (M < 0) return fail(HS_ERR_INVALID_ARGUMENT, "M must be >= 0 (got %d)", M);
+  if (M > 65535) return fail(HS_ERR_UNSUPPORTED, "M %d above 65535", M);
+  *skip = M == 0 || ad->rows == 0;
+  if (*skip) return HS_OK;
+  if (!d_x || !d_slots || !d_y || (ad->count > 0 && (!ad->a || !ad->b)))
+    return fail(HS_ERR_INVALID_ARGUMENT, "x, the adapters, slots and y must not be null");
+  if (ldx < ad->cols || ldy < ad->rows || (d_base && ldb < ad->rows))
+    return fail(HS_ERR_INVALID_ARGUMENT, "row strides %lld, %lld, %lld below the adapters' %d x %d",
+                (long long)ldx, (long long)ldb, (long long)ldy, ad->rows, ad->cols);
+  const uintptr_t al = ad->type == hs::kA_F32 ? 3u : 1u;
+  if (((reinterpret_cast<uintptr_t>(d_x) | reinterpret_cast<uintptr_t>(d_y) |
+        reinterpret_cast<uintptr_t>(d_base)) & 3u) ||
+      ((reinterpret_cast<uintptr_t>(ad->a) | reinterpret_cast<uintptr_t>(ad->b)) & al))
+    return fail(HS_ERR_INVALID_ARGUMENT, "x, base, y and the adapters must be aligned to their elements");
+  if (d_base == d_y && ldb != ldy)
+    return fail(HS_ERR_INVALID_ARGUMENT, "base in place of y needs y's row stride");
+  if (d_base && d_base != d_y) {
+    const uintptr_t b0 = reinterpret_cast<uintptr_t>(d_base), y0 = reinterpret_cast<uintptr_t>(d_y);
+    const uintptr_t b1 = b0 + 4 * ((uintptr_t)(M - 1) * (uintptr_t)ldb + (uintptr_t)ad->rows);
+    const uintptr_t y1 = y0 + 4 * ((uintptr_t)(M - 1) * (uintptr_t)ldy + (uintptr_t)ad->rows);
+    if (b0 < y1 && y0 < b1) return fail(HS_ERR_INVALID_ARGUMENT, "base overlaps y");
+  }
+  memset(&g, 0, sizeof g);
+  g.x = d_x;
+  g.ldx = ldx;
+  g.a = ad->a;
+  g.b = ad->b;
+  g.scales = ad->scales;
+  g.ranks = ad->ranks;
+  g.slots = d_slots;
+  g.base = d_base;
+  g.ldb = ldb;
+  g.y = d_y;
+  g.ldy = ldy;
+  g.M = M;
+  g.K = ad->cols;
+  g.N = ad->rows;
+  g.rank = ad->rank;
+  g.rank_pad = 16;
+  while (g.rank_pad < g.rank) g.rank_pad *= 2;
+  g.count = ad->count;
+  g.type = ad->type;
+  return HS_OK;
+}
+
+// (the context's lock is held)
+int lora_run(hs_context *ctx, hs::LoraArgs &g, hipStream_t stream) {
+  DeviceGuard guard(ctx->device);
+  const bool cap = is_capturing(stream);
+  int rc = kept_room(ctx->lora_t, (size_t)g.M * (size_t)g.rank_pad * sizeof(float), cap);
+  if (rc) return rc;
+  g.t = static_cast<float *>(ctx->lora_t.b.p);
+  if (!cap) rc = enter_stream(ctx, stream);
+  if (rc) return rc;
+  hipEvent_t *ev1 = nullptr, *ev2 = nullptr;
+  if (!cap && g.count > 0) rc = timed_pair(ctx, hs::kShrinkTimedSlot, hs::kExpandTimedSlot, &ev1, &ev2);
+  else if (!cap) rc = timed_slot(ctx, hs::kExpandTimedSlot, &ev2);
+  if (rc) return rc;
+  hipError_t e = hipSuccess;
+  if (g.count > 0) e = hs::launch_lora_shrink(g, stream, ev1);
+  if (e == hipSuccess) e = hs::launch_lora_expand(g, stream, ev2, cap ? nullptr : ctx->done_ev);
+  if (e != hipSuccess) {
+    if (!cap) (void)leave_stream(ctx, stream, false);
+    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
+  }
+  return cap ? HS_OK : leave_stream(ctx, stream, ev2 == nullptr);
+}
+
+int lora_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_adapters *ad,
+                const int32_t *d_slots, const float *d_base, int64_t ldb, float *d_y, int64_t ldy,
+                hipStream_t stream) {
+  hs::LoraArgs g;
+  bool skip = false;
+  const int rc = lora_args(d_x, M, ldx, ad, d_slots, d_base, ldb, d_y, ldy, g, &skip);
+  if (rc || skip) return rc;
+  HS_LOCK(ctx);
+  return lora_run(ctx, g, stream);
+}
+
+// The projection's and the adapters' arguments, for the calls with both.
+int gemv_lora_args(const float *d_x, int32_t M, int64_t ldx, const hs_weights *w,
+                   const hs_adapters *ad, const int32_t *d_slots, float *d_y, int64_t ldy,
+                   hs::LoraArgs &g, bool *skip) {
+  if (!w) return fail(HS_ERR_INVALID_ARGUMENT, "null weights");
+  const int rc = lora_args(d_x, M, ldx, ad, d_slots, d_y, ldy, d_y, ldy, g, skip);
+  if (rc) return rc;
+  if (ad->cols != w->cols || ad->rows != w->rows)
+    return fail(HS_ERR_INVALID_ARGUMENT, "adapters of %d x %d beside weights of %d x %d", ad->rows,
+                ad->cols, w->rows, w->cols);
+  return HS_OK;
+}
+
+// The projection, then the adapters on its result.  The adapters' workspace
+// comes first: a call that is refused for it enqueues nothing.
+int gemv_lora(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *w,
+              float *d_y, int64_t ldy, hs::LoraArgs &g, bool skip, hipStream_t stream) {
+  if (!skip) {
+    DeviceGuard guard(ctx->device);
+    const int rc = kept_room(ctx->lora_t, (size_t)g.M * (size_t)g.rank_pad * sizeof(float),
+                             is_capturing(stream));
+    if (rc) return rc;
+  }
+  const int rc = gemv_device(ctx, d_x, M, ldx, w, d_y, ldy, stream);
+  return rc || skip ? rc : lora_run(ctx, g, stream);
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -1164,6 +1563,14 @@ int hs_context_create(int device, hs_context **out) {
   }
   if (e == hipSuccess) e = ctx->gemv_tab.ensure(hs::kBatchWorkBytes);
   if (e == hipSuccess) e = hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking);
+  // (a first call may be captured: up to these sizes it needs no allocation)
+  if (e == hipSuccess) e = ctx->verify_ws.ensure(kVerifyWorkBytes);
+  if (e == hipSuccess) e = ctx->verify_cnt.ensure(kVerifyCountBytes);
+  if (e == hipSuccess) e = ctx->lora_t.ensure(kLoraWorkBytes);
+  if (e == hipSuccess)
+    e = hs::launch_fill_u32(static_cast<uint32_t *>(ctx->verify_cnt.b.p),
+                            (int64_t)(ctx->verify_cnt.b.bytes / sizeof(uint32_t)), 0u, ctx->stream);
+  if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
   if (e != hipSuccess) {
     hs_context_destroy(ctx);
     return fail(HS_ERR_HIP, "context setup failed: %s", hipGetErrorString(e));
@@ -1223,6 +1630,9 @@ int hs_context_destroy(hs_context *ctx) {
     ctx->gemv_cnt.release();
     ctx->gemv_rot.release();
     ctx->gemv_tab.release();
+    ctx->verify_ws.release();
+    ctx->verify_cnt.release();
+    ctx->lora_t.release();
     ctx->minp_cand.release();
     ctx->minp_meta.release();
     ctx->large_retry.release();
@@ -1435,6 +1845,60 @@ int hs_lm_head_sample_device_ex(hs_context *ctx, const float *d_x, int32_t M, in
   HS_LOCK(ctx);
   return lm_head_sample(ctx, d_x, M, ldx, w, d_logits, ldl, d_hist_ids, d_hist_offsets, configs,
                         d_uniforms, d_tokens, static_cast<hipStream_t>(stream));
+}
+
+int hs_verify_drafts_device(hs_context *ctx, const hs_distribution *target,
+                            const hs_distribution *draft, int32_t vocab,
+                            const hs_draft_batch *batch, const hs_decode_state *state,
+                            void *stream) {
+  return verify_drafts(ctx, target, draft, vocab, batch, state, static_cast<hipStream_t>(stream));
+}
+
+int hs_verify_candidates_device(hs_context *ctx, const hs_candidates *target,
+                                const hs_candidates *draft, const hs_draft_batch *batch,
+                                const hs_decode_state *state, void *stream) {
+  return verify_candidates(ctx, target, draft, batch, state, static_cast<hipStream_t>(stream));
+}
+
+int hs_lora_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
+                   const hs_adapters *adapters, const int32_t *d_slots, const float *d_base,
+                   int64_t ldb, float *d_y, int64_t ldy, void *stream) {
+  return lora_device(ctx, d_x, M, ldx, adapters, d_slots, d_base, ldb, d_y, ldy,
+                     static_cast<hipStream_t>(stream));
+}
+
+int hs_gemv_lora_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
+                        const hs_weights *w, const hs_adapters *adapters,
+                        const int32_t *d_slots, float *d_y, int64_t ldy, void *stream) {
+  hs::LoraArgs g;
+  bool skip = false;
+  const int rc = gemv_lora_args(d_x, M, ldx, w, adapters, d_slots, d_y, ldy, g, &skip);
+  if (rc) return rc;
+  HS_LOCK(ctx);
+  return gemv_lora(ctx, d_x, M, ldx, w, d_y, ldy, g, skip, static_cast<hipStream_t>(stream));
+}
+
+int hs_lm_head_lora_sample_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
+                                  const hs_weights *w, const hs_adapters *adapters,
+                                  const int32_t *d_slots, float *d_logits, int64_t ldl,
+                                  const int32_t *d_hist_ids, const int64_t *d_hist_offsets,
+                                  const hs_sample_config *configs, const double *d_uniforms,
+                                  int32_t *d_tokens, void *stream) {
+  hs::LoraArgs g;
+  bool skip = false;
+  int rc = gemv_lora_args(d_x, M, ldx, w, adapters, d_slots, d_logits, ldl, g, &skip);
+  if (rc) return rc;
+  // (what the sampler would refuse, before the projection is enqueued)
+  if (M > 0 && (!configs || !d_uniforms || !d_tokens))
+    return fail(HS_ERR_INVALID_ARGUMENT, "configs, uniforms and tokens must not be null");
+  if ((d_hist_ids == nullptr) != (d_hist_offsets == nullptr))
+    return fail(HS_ERR_INVALID_ARGUMENT, "history ids and offsets must both be given or both null");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  HS_LOCK(ctx);
+  rc = gemv_lora(ctx, d_x, M, ldx, w, d_logits, ldl, g, skip, st);
+  if (rc) return rc;
+  return sample_device(ctx, d_logits, M, ldl, w->rows, d_hist_ids, d_hist_offsets, configs,
+                       d_uniforms, d_tokens, 0, nullptr, nullptr, nullptr, nullptr, nullptr, st);
 }
 
 // src/engine.ts:80-175 (createBlockSplitter): GGUF blocks of Q1_0 ([d][16 B

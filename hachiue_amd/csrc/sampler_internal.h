@@ -205,10 +205,11 @@ struct LaunchArgs {
 // (0 penalty pre-pass, 1 row kernel, 2 chunk kernel, 3 finalize, 4 large-k
 // kernel, 5 mid kernel, 6 GPU greedy-route argmax, 8 two-pass large-k kernel,
 // 9 the large-k slot replay, 10 the device-memory slot replay, 11 min-p kernel;
-// 7 is the lm_head GEMV, launched apart), for the kernels that launch only:
+// 7 is the lm_head GEMV, 12 to 16 the serving operators below, launched
+// apart), for the kernels that launch only:
 // launched_kernels() says which.  The large-k kernel launches whenever a row
 // has k > 1024: it also takes the rows the two-pass kernel hands back.
-constexpr int kTimedKernels = 12;
+constexpr int kTimedKernels = 17;
 inline unsigned launched_kernels(const LaunchArgs &a) {
   return (a.n_pf > 0 ? 1u : 0u) | (a.n_row > 0 ? 2u : 0u) | (a.n_chunk > 0 ? 12u : 0u) |
          (a.n_large + a.n_lfast > 0 ? 16u : 0u) | (a.n_mid > 0 ? 32u : 0u) |
@@ -399,5 +400,105 @@ int fuse_waves_per_block(int type);
 hipError_t launch_kq_sample(const GemvArgs &g, const FuseArgs &f, hipStream_t stream,
                             hipEvent_t *ev, hipEvent_t done);
 int kq_sample_grid(const GemvArgs &g);
+
+// ---- verification of drafted tokens (verify_kernels.hip)
+constexpr int kVerifyMaxDrafts = 63;     // a sequence's tokens fit one wave
+constexpr int kVerifyThreads = 256;
+constexpr int kVerifyPer = 32;           // values of a row a thread holds
+constexpr int kVerifyChunk = kVerifyThreads * kVerifyPer;
+constexpr int kVerifyMaxVocab = 1 << 28;
+constexpr int kVerifyMaxList = 4096;     // candidates of a list
+constexpr int kStatsTimedSlot = 12, kResolveTimedSlot = 13, kListsTimedSlot = 14;
+enum DistKind : int32_t { kDistNone = -1, kDistLogits = 0, kDistProbs = 1 };
+
+// One chunk of a row of logits: its largest logit, that logit's lowest id
+// (greedy rows) and the sum of exp((v - m) / T).
+struct VerifyPart {
+  double s;
+  float m;
+  int32_t arg;
+};
+static_assert(sizeof(VerifyPart) == 16, "VerifyPart layout");
+// A whole row's.
+using VerifyStat = VerifyPart;
+// A drafted position's outcome.
+struct Verdict {
+  float ratio;               // min(1, p / q)
+  int32_t ok;                // accepted
+};
+
+// The drafts of all sequences, their uniforms and where the outcome goes:
+// what both forms of the verification share.
+struct DraftArgs {
+  int32_t seqs, max_drafts;
+  int64_t n_drafts;
+  const int64_t *off;        // [seqs + 1] or null: max_drafts each
+  const int32_t *drafts;
+  const double *uniforms;
+  int32_t *tokens, *counts;
+  float *accept;             // or null
+  // histories of a decode loop, or null (as in LaunchArgs)
+  int32_t *ring;
+  int64_t cap;
+  int64_t *len;
+  int32_t *done;
+  const int32_t *stop;
+  int32_t nstop;
+};
+
+struct VerifyArgs {
+  DraftArgs d;
+  const float *rows[2];      // target and draft rows
+  int64_t stride[2];
+  const double *temps[2];    // [seqs] or null: 1
+  int32_t kind[2];           // DistKind
+  int32_t vocab, chunks;
+  VerifyPart *part[2];       // [rows][chunks] of the sides that are logits
+  VerifyStat *stat[2];       // [rows]
+  Verdict *verdict;          // [seqs][max_drafts + 1]
+  double *mass;              // [seqs][chunks]
+  // zero between calls: chunks counted in per position, the first rejection
+  // found so far (64 - position), chunks of the final row counted in
+  uint32_t *arrived;         // [seqs][max_drafts + 1]
+  uint32_t *rejected;        // [seqs]
+  uint32_t *arrived_final;   // [seqs]
+};
+hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream, hipEvent_t *ev_stats,
+                         hipEvent_t *ev_resolve, hipEvent_t done);
+
+struct ListArgs {
+  DraftArgs d;
+  const int32_t *ids[2];     // candidate lists of the target's and the draft's rows
+  const float *probs[2];
+  const int32_t *kept[2];
+  const int32_t *tokens[2];  // ids of rows with an empty list, or null
+  int32_t stride[2];
+  int32_t certain;           // no draft lists: a draft's own probability is 1
+};
+hipError_t launch_verify_lists(const ListArgs &a, hipStream_t stream, hipEvent_t *ev,
+                               hipEvent_t done);
+hipError_t prepare_verify();    // per device, once (called by prepare_gemv)
+
+// ---- low-rank adapters (lora_kernels.hip)
+constexpr int kA_F32 = 0, kA_F16 = 1, kA_BF16 = 30;   // GGML type ids
+constexpr int kLoraMaxRank = 256;
+constexpr int kShrinkTimedSlot = 15, kExpandTimedSlot = 16;
+struct LoraArgs {
+  const float *x;            // [M][ldx]
+  int64_t ldx;
+  const void *a;             // [count][rank][K]
+  const void *b;             // [count][N][rank]
+  const float *scales;       // [count] or null: 1
+  const int32_t *ranks;      // [count] or null: rank
+  const int32_t *slots;      // [M]; outside [0, count): no adapter
+  float *t;                  // [M][rank_pad] scale * x A^T
+  const float *base;         // [M][ldb] or null: 0
+  int64_t ldb;
+  float *y;                  // [M][ldy]
+  int64_t ldy;
+  int32_t M, K, N, rank, rank_pad, count, type;
+};
+hipError_t launch_lora_shrink(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev);
+hipError_t launch_lora_expand(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev, hipEvent_t done);
 
 }  // namespace hs

@@ -17,7 +17,7 @@ import ctypes
 import numpy as np
 
 from . import hip
-from .sampler import Sampler, _configs
+from .sampler import DecodeStateC, Sampler, _configs, decode_state
 
 
 class DecodeState:
@@ -56,6 +56,27 @@ class DecodeState:
                                         self.ring_cap, self.len.addr, self.done.addr,
                                         self.stop.addr if self.n_stop else None, self.n_stop, cfgs,
                                         d_uniforms, d_tokens, stream)
+
+    def descriptor(self) -> DecodeStateC:
+        """The rings as the verification calls take them (hs_decode_state)."""
+        return decode_state(self.ring.addr, self.ring_cap, self.len.addr, self.done.addr,
+                            self.stop.addr if self.n_stop else None, self.n_stop)
+
+    def verify_drafts(self, target, draft, vocab: int, batch, stream=None) -> None:
+        """Enqueue one speculative step: the drafts of `batch` (one sequence
+        per row) verified against whole rows, and the tokens that stand
+        appended to the histories (Sampler.verify_drafts_device)."""
+        self._check(batch)
+        self.sampler.verify_drafts_device(target, draft, vocab, batch, self.descriptor(), stream)
+
+    def verify_candidates(self, target, draft, batch, stream=None) -> None:
+        """The same against candidate lists (Sampler.verify_candidates_device)."""
+        self._check(batch)
+        self.sampler.verify_candidates_device(target, draft, batch, self.descriptor(), stream)
+
+    def _check(self, batch) -> None:
+        if batch.seqs != self.rows:
+            raise ValueError(f"{batch.seqs} sequences of drafts for {self.rows} rows of state")
 
     def lengths(self) -> np.ndarray:
         hip.synchronize()

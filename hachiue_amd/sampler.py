@@ -38,6 +38,8 @@ EXPORTS = ("hs_abi_version", "hs_last_error", "hs_config_default", "hs_context_c
            "hs_sample_batch_device_noalloc", "hs_argmax_device",
            "hs_argmax", "hs_gemv_device", "hs_gemv_device_ex", "hs_split_blocks",
            "hs_lm_head_sample_device", "hs_lm_head_sample_device_ex", "hs_decode_step_device",
+           "hs_verify_drafts_device", "hs_verify_candidates_device", "hs_lora_device",
+           "hs_gemv_lora_device", "hs_lm_head_lora_sample_device",
            "hs_context_set_timing", "hs_context_kernel_times")
 
 
@@ -78,6 +80,83 @@ def weights(wtype: int, N: int, K: int, d_data: int, d_scales16: int | None = No
             hadamard: bool = False, d_signs: int | None = None) -> WeightsC:
     return WeightsC(int(wtype), int(N), int(K), 1 if hadamard else 0, d_data, d_scales16 or None,
                     d_signs or None)
+
+
+DIST_LOGITS, DIST_PROBS = 0, 1
+
+
+class DistributionC(ctypes.Structure):
+    """hs_distribution: one model's rows of logits or probabilities."""
+    _fields_ = [("kind", ctypes.c_int32), ("row_stride", ctypes.c_int64),
+                ("data", ctypes.c_void_p), ("temperatures", ctypes.c_void_p)]
+
+
+def distribution(kind: int, d_data: int, row_stride: int,
+                 d_temperatures: int | None = None) -> DistributionC:
+    """Rows for Sampler.verify_drafts_device: DIST_LOGITS (with float64
+    temperatures per sequence, None: 1) or DIST_PROBS."""
+    return DistributionC(int(kind), int(row_stride), d_data or None, d_temperatures or None)
+
+
+class DraftBatchC(ctypes.Structure):
+    """hs_draft_batch: the drafts of all sequences, their uniforms and where
+    the outcome goes."""
+    _fields_ = [("seqs", ctypes.c_int32), ("max_drafts", ctypes.c_int32),
+                ("n_drafts", ctypes.c_int64), ("offsets", ctypes.c_void_p),
+                ("drafts", ctypes.c_void_p), ("uniforms", ctypes.c_void_p),
+                ("tokens", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+                ("accept", ctypes.c_void_p)]
+
+
+def draft_batch(seqs: int, max_drafts: int, n_drafts: int, d_offsets: int | None, d_drafts: int,
+                d_uniforms: int, d_tokens: int, d_counts: int,
+                d_accept: int | None = None) -> DraftBatchC:
+    return DraftBatchC(int(seqs), int(max_drafts), int(n_drafts), d_offsets or None,
+                       d_drafts or None, d_uniforms or None, d_tokens or None, d_counts or None,
+                       d_accept or None)
+
+
+class DecodeStateC(ctypes.Structure):
+    """hs_decode_state: the history rings of a decode loop."""
+    _fields_ = [("ring", ctypes.c_void_p), ("ring_cap", ctypes.c_int64),
+                ("len", ctypes.c_void_p), ("done", ctypes.c_void_p),
+                ("stop_ids", ctypes.c_void_p), ("n_stop", ctypes.c_int32)]
+
+
+def decode_state(d_ring: int, ring_cap: int, d_len: int, d_done: int,
+                 d_stop_ids: int | None = None, n_stop: int = 0) -> DecodeStateC:
+    return DecodeStateC(d_ring or None, int(ring_cap), d_len or None, d_done or None,
+                        d_stop_ids or None, int(n_stop))
+
+
+class CandidatesC(ctypes.Structure):
+    """hs_candidates: the candidate lists that sample_device leaves."""
+    _fields_ = [("stride", ctypes.c_int32), ("ids", ctypes.c_void_p),
+                ("probs", ctypes.c_void_p), ("kept", ctypes.c_void_p),
+                ("tokens", ctypes.c_void_p)]
+
+
+def candidates(stride: int, d_ids: int, d_probs: int, d_kept: int,
+               d_tokens: int | None = None) -> CandidatesC:
+    """Lists for Sampler.verify_candidates_device: the d_cand_ids, d_cand_probs,
+    d_cutoff and d_tokens of a sample_device call with cand_stride `stride`."""
+    return CandidatesC(int(stride), d_ids or None, d_probs or None, d_kept or None,
+                       d_tokens or None)
+
+
+class AdaptersC(ctypes.Structure):
+    """hs_adapters: low-rank adapters of one projection, stacked."""
+    _fields_ = [("type", ctypes.c_int32), ("count", ctypes.c_int32), ("rank", ctypes.c_int32),
+                ("cols", ctypes.c_int32), ("rows", ctypes.c_int32), ("a", ctypes.c_void_p),
+                ("b", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("ranks", ctypes.c_void_p)]
+
+
+def adapters(atype: int, count: int, rank: int, K: int, N: int, d_a: int, d_b: int,
+             d_scales: int | None = None, d_ranks: int | None = None) -> AdaptersC:
+    """A [count][rank][K] and B [count][N][rank] of GGML type 0 (F32), 1 (F16)
+    or 30 (BF16), with a float32 scale and an int32 rank per adapter."""
+    return AdaptersC(int(atype), int(count), int(rank), int(K), int(N), d_a or None, d_b or None,
+                     d_scales or None, d_ranks or None)
 
 
 class SampleConfigC(ctypes.Structure):
@@ -152,6 +231,14 @@ def _load() -> ctypes.CDLL:
     L.hs_split_blocks.argtypes = [i32, vp, i64, vp, vp]
     L.hs_decode_step_device.argtypes = [vp, vp, i32, i64, i32, vp, i64, vp, vp, vp, i32,
                                         P(SampleConfigC), vp, vp, vp]
+    L.hs_verify_drafts_device.argtypes = [vp, P(DistributionC), P(DistributionC), i32,
+                                          P(DraftBatchC), P(DecodeStateC), vp]
+    L.hs_verify_candidates_device.argtypes = [vp, P(CandidatesC), P(CandidatesC), P(DraftBatchC),
+                                              P(DecodeStateC), vp]
+    L.hs_lora_device.argtypes = [vp, vp, i32, i64, P(AdaptersC), vp, vp, i64, vp, i64, vp]
+    L.hs_gemv_lora_device.argtypes = [vp, vp, i32, i64, P(WeightsC), P(AdaptersC), vp, vp, i64, vp]
+    L.hs_lm_head_lora_sample_device.argtypes = [vp, vp, i32, i64, P(WeightsC), P(AdaptersC), vp,
+                                                vp, i64, vp, vp, P(SampleConfigC), vp, vp, vp]
     L.hs_context_set_timing.argtypes = [vp, ctypes.c_int]
     L.hs_context_kernel_times.argtypes = [vp, P(dbl), i32, P(i64)]
     return L
@@ -241,7 +328,9 @@ class Sampler:
 
     KERNELS = ("pen_kernel", "row_kernel", "chunk_kernel", "finalize_kernel", "large_kernel",
                "mid_kernel", "argmax_kernel", "gemv_kernel", "large_fast_kernel",
-               "large_replay_kernel", "large_replay_dev_kernel", "minp_kernel")
+               "large_replay_kernel", "large_replay_dev_kernel", "minp_kernel",
+               "verify_stats_kernel", "verify_resolve_kernel", "verify_lists_kernel",
+               "lora_shrink_kernel", "lora_expand_kernel")
 
     def kernel_times(self):
         """({kernel: total device ms}, calls) since the last query."""
@@ -411,6 +500,46 @@ class Sampler:
             self._ctx, vp(d_logits), int(rows), int(row_stride), int(vocab), vp(d_ring),
             int(ring_cap), vp(d_len), vp(d_done), vp(d_stop_ids or 0), int(n_stop), cfgs,
             vp(d_uniforms), vp(d_tokens), st))
+
+    # ---- drafted tokens -------------------------------------------------------
+    def verify_drafts_device(self, target: DistributionC, draft: DistributionC | None, vocab: int,
+                             batch: DraftBatchC, state: DecodeStateC | None = None,
+                             stream=None) -> None:
+        """Enqueue the verification of drafted tokens against whole rows
+        (hs_verify_drafts_device); draft None: certain drafts."""
+        st = stream.handle if isinstance(stream, hip.Stream) else stream
+        _check(lib().hs_verify_drafts_device(self._ctx, target, draft, vocab, batch, state, st))
+
+    def verify_candidates_device(self, target: CandidatesC, draft: CandidatesC | None,
+                                 batch: DraftBatchC, state: DecodeStateC | None = None,
+                                 stream=None) -> None:
+        """The same against the candidate lists that sample_device leaves
+        (hs_verify_candidates_device)."""
+        st = stream.handle if isinstance(stream, hip.Stream) else stream
+        _check(lib().hs_verify_candidates_device(self._ctx, target, draft, batch, state, st))
+
+    # ---- low-rank adapters -------------------------------------------------------
+    def lora_device(self, d_x: int, M: int, ldx: int, ad: AdaptersC, d_slots: int,
+                    d_base: int | None, ldb: int, d_y: int, ldy: int, stream=None) -> None:
+        """y = base + scale (x A^T) B^T with each row's adapter (hs_lora_device)."""
+        st = stream.handle if isinstance(stream, hip.Stream) else stream
+        _check(lib().hs_lora_device(self._ctx, d_x, M, ldx, ad, d_slots, d_base, ldb, d_y, ldy, st))
+
+    def gemv_lora_device(self, d_x: int, M: int, ldx: int, w: WeightsC, ad: AdaptersC,
+                         d_slots: int, d_y: int, ldy: int, stream=None) -> None:
+        """gemv_device_ex with the rows' adapters on its result."""
+        st = stream.handle if isinstance(stream, hip.Stream) else stream
+        _check(lib().hs_gemv_lora_device(self._ctx, d_x, M, ldx, w, ad, d_slots, d_y, ldy, st))
+
+    def lm_head_lora_sample_device(self, d_x: int, M: int, ldx: int, w: WeightsC, ad: AdaptersC,
+                                   d_slots: int, d_logits: int, ldl: int, d_hist_ids, d_hist_off,
+                                   configs, d_uniforms: int, d_tokens: int, stream=None) -> None:
+        """gemv_lora_device into d_logits, then sampling of its M rows."""
+        cfgs = configs if isinstance(configs, ctypes.Array) else _configs(configs, M)
+        st = stream.handle if isinstance(stream, hip.Stream) else stream
+        _check(lib().hs_lm_head_lora_sample_device(
+            self._ctx, d_x, M, ldx, w, ad, d_slots, d_logits, ldl, d_hist_ids or None,
+            d_hist_off or None, cfgs, d_uniforms, d_tokens, st))
 
     # ---- device-resident batch ----------------------------------------------
     def sample_device(self, d_logits: int, rows: int, row_stride: int, vocab: int,

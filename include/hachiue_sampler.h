@@ -308,6 +308,155 @@ int hs_decode_step_device(hs_context *ctx, float *d_logits, int32_t rows,
                           const double *d_uniforms, int32_t *d_tokens,
                           void *stream);
 
+/* ---- Several tokens per step: verification of drafted tokens.  No
+ * counterpart in the reference, whose decode loop (src/engine.ts:1626-1644)
+ * takes one token per forward pass.
+ *
+ * A draft model (or a lookup in the prompt) proposes tokens x_0 .. x_(n-1) for
+ * each sequence; one forward pass gives the target's distributions p_0 .. p_n
+ * at all of their positions (p_i after the first i drafts).  With uniforms
+ * u_0 .. u_n in [0, 1) and the distributions q_i that the drafts were drawn
+ * from, draft i is accepted iff u_i * q_i(x_i) < p_i(x_i), in order up to the
+ * first rejection a (a = n: none).  One more token follows: the first id v
+ * whose running sum of r(0) .. r(v) is above u_n times the sum of r, with
+ * r = max(p_a - q_a, 0) after a rejection (p_a where that is 0 everywhere) and
+ * r = p_n without one.  All in binary64.  The tokens are distributed as the
+ * target's own draws.  Without draft distributions (a lookup) each draft is
+ * taken as certain: q_i is 1 at x_i. */
+
+/* The distributions of one model, a row of `vocab` floats per position:
+ *   HS_DIST_LOGITS: exp((l - max) / T) normalised, T = temperatures[b] of the
+ *     row's sequence (1 where temperatures is NULL); T <= 0 or NaN: all on the
+ *     first maximum.  A logit of -infinity or NaN weighs 0; among logits of
+ *     +infinity the weight is shared.
+ *   HS_DIST_PROBS: probabilities as given (they need not sum to 1 exactly); one
+ *     that is negative, NaN or infinite counts as 0. */
+#define HS_DIST_LOGITS 0
+#define HS_DIST_PROBS 1
+typedef struct hs_distribution {
+  int32_t kind;
+  int64_t row_stride;          /* floats, at least vocab */
+  const float *data;           /* device */
+  const double *temperatures;  /* device [seqs] or NULL; logits only */
+} hs_distribution;
+
+/* The drafts of `seqs` sequences, one after another.  Sequence b has
+ * n_b = offsets[b + 1] - offsets[b] of them (at most max_drafts, and max_drafts
+ * each where offsets is NULL; then n_drafts is seqs * max_drafts) at
+ * drafts[offsets[b]] ...; its n_b + 1 target rows, uniforms and output tokens
+ * start at index offsets[b] + b, its draft rows and acceptance probabilities at
+ * offsets[b].  n_drafts is the arrays' size: offsets up to it are followed, and
+ * what lies behind the last sequence is neither read nor written.
+ *   tokens [n_drafts + seqs]: the accepted drafts, the one more token, then -1
+ *   counts [seqs]: tokens of each sequence (accepted drafts + 1)
+ *   accept [n_drafts] or NULL: min(1, p_i(x_i) / q_i(x_i)) up to the first
+ *     rejection, 0 behind it
+ * A row without any candidate rejects its draft and gives token 0, as the
+ * sampler does. */
+typedef struct hs_draft_batch {
+  int32_t seqs;
+  int32_t max_drafts;          /* 0 .. 63 */
+  int64_t n_drafts;
+  const int64_t *offsets;      /* device [seqs + 1] or NULL */
+  const int32_t *drafts;       /* device */
+  const double *uniforms;      /* device */
+  int32_t *tokens;             /* device */
+  int32_t *counts;             /* device */
+  float *accept;               /* device or NULL */
+} hs_draft_batch;
+
+/* The histories of hs_decode_step_device, or NULL in the calls below: a
+ * sequence's tokens join its ring up to a stop id, which sets done[b], is
+ * reported and ends its tokens (those behind it are -1 and not counted).  A
+ * sequence that was done before the call gets count 0. */
+typedef struct hs_decode_state {
+  int32_t *ring;               /* device [seqs][ring_cap] */
+  int64_t ring_cap;            /* 128 .. 2^29 */
+  int64_t *len;                /* device [seqs] */
+  int32_t *done;               /* device [seqs] */
+  const int32_t *stop_ids;     /* device [n_stop] */
+  int32_t n_stop;              /* 0 .. 1024 */
+} hs_decode_state;
+
+/* Verification against whole rows; draft may be NULL (certain drafts).
+ * Asynchronous on `stream`.  The call may be captured into a HIP graph: the
+ * workspace is the context's, of a size that the context has from its creation
+ * (or from a larger earlier call; a captured call that needs more returns
+ * HS_ERR_UNSUPPORTED), and it stays where it is until hs_context_destroy.
+ * Graphs captured on one context share that workspace: replay them, and call
+ * the context, one after the other, or capture on contexts of their own. */
+int hs_verify_drafts_device(hs_context *ctx, const hs_distribution *target,
+                            const hs_distribution *draft, int32_t vocab,
+                            const hs_draft_batch *batch, const hs_decode_state *state,
+                            void *stream);
+
+/* Rows as the sampler leaves them: the candidate lists, their normalised
+ * probabilities and the kept-prefix lengths (d_cand_ids, d_cand_probs,
+ * d_cutoff with cand_stride = stride of hs_sample_batch_device_ex), that is
+ * distributions truncated by top-k, min-p and top-p with the penalties
+ * applied.  A row's p is its kept probabilities over their sum.  A row with
+ * kept 0 (a greedy one, or one without candidates) is all on tokens[row], the
+ * token the sampler gave it (0 where tokens is NULL).  A list's ids are
+ * distinct. */
+typedef struct hs_candidates {
+  int32_t stride;              /* entries of a row, 1 .. 4096 */
+  const int32_t *ids;          /* device [rows][stride] */
+  const float *probs;          /* device [rows][stride] */
+  const int32_t *kept;         /* device [rows] */
+  const int32_t *tokens;       /* device [rows] or NULL */
+} hs_candidates;
+
+/* Verification against candidate lists; draft may be NULL (certain drafts).
+ * The one more token is drawn in the target list's order, as the sampler draws.
+ * A sequence that meets a list kept only in part (kept > stride) or a row that
+ * the sampler left unresolved (token -1) gets count -1 and no tokens.
+ * Asynchronous on `stream`, no workspace; may be captured. */
+int hs_verify_candidates_device(hs_context *ctx, const hs_candidates *target,
+                                const hs_candidates *draft, const hs_draft_batch *batch,
+                                const hs_decode_state *state, void *stream);
+
+/* ---- Low-rank adapters beside a projection, a different one per row (no
+ * counterpart in the reference, which holds one model's weights): for row m
+ * with adapter s = slots[m],
+ *   y[m] = base[m] + scales[s] * (x[m] A_s^T) B_s^T,
+ * and y[m] = base[m] for a slot outside [0, count).  A [count][rank][cols] and
+ * B [count][rows][rank] are stacked device arrays of F32 (0), F16 (1) or BF16
+ * (30) elements, aligned as such; adapter s uses the first ranks[s] ranks of its stack
+ * (rank where ranks is NULL), and nothing behind them matters.  x, base and y
+ * are binary32; the products are summed in binary32. */
+typedef struct hs_adapters {
+  int32_t type;                /* GGML type id: 0, 1 or 30 */
+  int32_t count;
+  int32_t rank;                /* 1 .. 256 */
+  int32_t cols;                /* K: inputs of the projection */
+  int32_t rows;                /* N: its outputs */
+  const void *a;
+  const void *b;
+  const float *scales;         /* device [count] or NULL: 1 */
+  const int32_t *ranks;        /* device [count] or NULL */
+} hs_adapters;
+
+/* The adapters' share alone: base [M][ldb] (NULL: 0) may be y itself (ldb ==
+ * ldy), and else must not overlap it.  M up to 65535.  Captured calls and the
+ * workspace as in hs_verify_drafts_device. */
+int hs_lora_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
+                   const hs_adapters *adapters, const int32_t *d_slots, const float *d_base,
+                   int64_t ldb, float *d_y, int64_t ldy, void *stream);
+
+/* hs_gemv_device_ex and the adapters on its result; the adapters' cols and rows
+ * are the weights'.  (A Hadamard-folded weight's adapters see x as given.) */
+int hs_gemv_lora_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
+                        const hs_weights *w, const hs_adapters *adapters,
+                        const int32_t *d_slots, float *d_y, int64_t ldy, void *stream);
+
+/* hs_lm_head_sample_device_ex with the adapters between its two steps. */
+int hs_lm_head_lora_sample_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
+                                  const hs_weights *w, const hs_adapters *adapters,
+                                  const int32_t *d_slots, float *d_logits, int64_t ldl,
+                                  const int32_t *d_hist_ids, const int64_t *d_hist_offsets,
+                                  const hs_sample_config *configs, const double *d_uniforms,
+                                  int32_t *d_tokens, void *stream);
+
 /* Diagnostics (no counterpart in the reference, which has no GPU sampler):
  * while enabled, every sampling call records HIP events on its stream around
  * each of its kernel launches.  hs_context_kernel_times() waits for the
@@ -316,7 +465,9 @@ int hs_decode_step_device(hs_context *ctx, float *d_logits, int32_t rows,
  * ms[3] finalize, ms[4] large-k kernel, ms[5] mid-k kernel, ms[6] greedy-route
  * argmax, ms[7] lm_head GEMV, ms[8] two-pass large-k kernel, ms[9] large-k
  * slot replay in LDS, ms[10] large-k slot replay in device memory, ms[11]
- * min-p kernel; a kernel a call did not launch adds 0)
+ * min-p kernel, ms[12] the drafted rows' sums, ms[13] their outcome, ms[14]
+ * verification against candidate lists, ms[15] and ms[16] the adapters' two
+ * products; a kernel a call did not launch adds 0)
  * and the number of
  * timed calls, and resets the totals. */
 int hs_context_set_timing(hs_context *ctx, int enable);
