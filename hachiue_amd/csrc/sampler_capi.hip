@@ -183,7 +183,7 @@ constexpr size_t pin_align(size_t b) { return (b + 255) / 256 * 256; }
 
 // Workspaces that a context has from its creation on: of 64 sequences with 8
 // drafts over 262144 logits, and of 4096 rows with adapters of rank 64.
-constexpr size_t kVerifyWorkBytes = size_t(1) << 20;
+constexpr size_t kVerifyWorkBytes = size_t(5) << 19;
 constexpr size_t kVerifyCountBytes = size_t(16) << 10;
 constexpr size_t kLoraWorkBytes = size_t(1) << 20;
 
@@ -1266,7 +1266,8 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
     if (rc) return rc;
   }
   a.vocab = vocab;
-  a.chunks = (vocab + hs::kVerifyChunk - 1) / hs::kVerifyChunk;
+  a.parts = (vocab + hs::kVerifyPart - 1) / hs::kVerifyPart;
+  a.blocks = (vocab + hs::kVerifyBlock - 1) / hs::kVerifyBlock;
   const size_t rows[2] = {(size_t)a.d.n_drafts + (size_t)a.d.seqs, (size_t)a.d.n_drafts};
   const size_t judged = (size_t)a.d.seqs * (size_t)(a.d.max_drafts + 1);
   size_t need = 0;
@@ -1278,11 +1279,12 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
   size_t part[2] = {0, 0}, stat[2] = {0, 0};
   for (int i = 0; i < 2; ++i)
     if (a.kind[i] == hs::kDistLogits) {
-      part[i] = take(rows[i] * (size_t)a.chunks * sizeof(hs::VerifyPart));
+      part[i] = take(rows[i] * (size_t)a.parts * sizeof(hs::VerifyPart));
       stat[i] = take(rows[i] * sizeof(hs::VerifyStat));
     }
   const size_t verdict = take(judged * sizeof(hs::Verdict));
-  const size_t mass = take((size_t)a.d.seqs * (size_t)a.chunks * sizeof(double));
+  const size_t mass = take((size_t)a.d.seqs * (size_t)a.parts * sizeof(double));
+  const size_t open = take((size_t)a.d.seqs * sizeof(int32_t));
   const size_t counts = judged + 2 * (size_t)a.d.seqs;
   HS_LOCK(ctx);
   DeviceGuard guard(ctx->device);
@@ -1313,14 +1315,14 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
   a.mass = reinterpret_cast<double *>(ws + mass);
   a.arrived = static_cast<uint32_t *>(ctx->verify_cnt.b.p);
   a.rejected = a.arrived + judged;
-  a.arrived_final = a.rejected + a.d.seqs;
+  a.left = a.rejected + a.d.seqs;
+  a.open = reinterpret_cast<int32_t *>(ws + open);
   hipEvent_t *ev1 = nullptr, *ev2 = nullptr;
   if (!cap) {
-    if (a.kind[0] == hs::kDistLogits || a.kind[1] == hs::kDistLogits) {
-      rc = timed_pair(ctx, hs::kStatsTimedSlot, hs::kResolveTimedSlot, &ev1, &ev2);
-    } else {
-      rc = timed_slot(ctx, hs::kResolveTimedSlot, &ev2);
-    }
+    const unsigned launches = hs::verify_launches(a);
+    if (launches == 3u) rc = timed_pair(ctx, hs::kStatsTimedSlot, hs::kResolveTimedSlot, &ev1, &ev2);
+    else if (launches == 1u) rc = timed_slot(ctx, hs::kStatsTimedSlot, &ev1);
+    else rc = timed_slot(ctx, hs::kResolveTimedSlot, &ev2);
     if (rc) return rc;
   }
   const hipError_t e = hs::launch_verify(a, stream, ev1, ev2, cap ? nullptr : ctx->done_ev);
@@ -1332,7 +1334,7 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
     }
     return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
   }
-  return cap ? HS_OK : leave_stream(ctx, stream, ev2 == nullptr);
+  return cap ? HS_OK : leave_stream(ctx, stream, !ev1 && !ev2);
 }
 
 int list_side(const hs_candidates *x, const char *what, hs::ListArgs &a, int side) {

@@ -405,13 +405,14 @@ int kq_sample_grid(const GemvArgs &g);
 constexpr int kVerifyMaxDrafts = 63;     // a sequence's tokens fit one wave
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyPer = 32;           // values of a row a thread holds
-constexpr int kVerifyChunk = kVerifyThreads * kVerifyPer;
+constexpr int kVerifyPart = 64 * kVerifyPer;   // a wave's, the unit of the sums
+constexpr int kVerifyBlock = kVerifyThreads * kVerifyPer;
 constexpr int kVerifyMaxVocab = 1 << 28;
 constexpr int kVerifyMaxList = 4096;     // candidates of a list
 constexpr int kStatsTimedSlot = 12, kResolveTimedSlot = 13, kListsTimedSlot = 14;
 enum DistKind : int32_t { kDistNone = -1, kDistLogits = 0, kDistProbs = 1 };
 
-// One chunk of a row of logits: its largest logit, that logit's lowest id
+// One part of a row of logits: its largest logit, that logit's lowest id
 // (greedy rows) and the sum of exp((v - m) / T).
 struct VerifyPart {
   double s;
@@ -452,17 +453,24 @@ struct VerifyArgs {
   int64_t stride[2];
   const double *temps[2];    // [seqs] or null: 1
   int32_t kind[2];           // DistKind
-  int32_t vocab, chunks;
-  VerifyPart *part[2];       // [rows][chunks] of the sides that are logits
+  int32_t vocab, parts, blocks;   // parts of a row, workgroups of a row
+  VerifyPart *part[2];       // [rows][parts] of the sides that are logits
   VerifyStat *stat[2];       // [rows]
   Verdict *verdict;          // [seqs][max_drafts + 1]
-  double *mass;              // [seqs][chunks]
-  // zero between calls: chunks counted in per position, the first rejection
-  // found so far (64 - position), chunks of the final row counted in
+  double *mass;              // [seqs][parts]
+  int32_t *open;             // [seqs] the rejected position, -1: the outcome is written
+  // zero between calls: workgroups counted in per position, and out per
+  // sequence, the first rejection found so far (64 - position)
   uint32_t *arrived;         // [seqs][max_drafts + 1]
   uint32_t *rejected;        // [seqs]
-  uint32_t *arrived_final;   // [seqs]
+  uint32_t *left;            // [seqs]
 };
+// The kernels of a call: bit 0 the rows' sums (logits on a side), bit 1 the
+// rows that a rejection leaves open (draft rows, or probabilities alone).
+inline unsigned verify_launches(const VerifyArgs &a) {
+  const bool sums = a.kind[0] == kDistLogits || a.kind[1] == kDistLogits;
+  return (sums ? 1u : 0u) | (!sums || a.kind[0] != kDistLogits || a.kind[1] != kDistNone ? 2u : 0u);
+}
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream, hipEvent_t *ev_stats,
                          hipEvent_t *ev_resolve, hipEvent_t done);
 

@@ -99,8 +99,11 @@ __device__ __forceinline__ bool greedy_temp(double T) { return !(T > 0.0); }
 // exp((l - m) / T) of a logit under a maximum m (NaN where the row has no
 // candidate, which makes every weight 0).  The maximum weighs 1, also where it
 // is +infinity; a NaN or -infinity weighs 0.
+__device__ __forceinline__ double weight_below(float l, float m, double c) {   // (m finite or NaN)
+  return exp2_neg(((double)l - (double)m) * c);
+}
 __device__ __forceinline__ double weight(float l, float m, double c) {
-  const double e = exp2_neg(((double)l - (double)m) * c);
+  const double e = weight_below(l, m, c);
   return l == m ? 1.0 : e;
 }
 __device__ __forceinline__ float max_or_nan(float m) {
@@ -196,12 +199,12 @@ __device__ __forceinline__ Verdict judge(double p, double q, double u) {
 
 // ---- whole rows
 
-// Four consecutive values of a row from id i on; past the vocabulary: NaN,
-// which weighs 0 in both kinds of row.  Rows need only their floats' own
+// Four consecutive values of a row.  Rows need only their floats' own
 // alignment.
 struct __attribute__((packed, aligned(4))) Float4 {
   float v[4];
 };
+// From id i on; past the vocabulary NaN, which weighs 0 in both kinds of row.
 __device__ __forceinline__ Float4 load4(const float *row, int i, int vocab) {
   if (i + 4 <= vocab) return *reinterpret_cast<const Float4 *>(row + i);
   Float4 f;
@@ -209,19 +212,30 @@ __device__ __forceinline__ Float4 load4(const float *row, int i, int vocab) {
   for (int e = 0; e < 4; ++e) f.v[e] = i + e < vocab ? row[i + e] : __builtin_nanf("");
   return f;
 }
-// The first id of a thread's j-th float4 of a chunk, a workgroup's width apart.
-__device__ __forceinline__ int chunk_id(int chunk, int j) {
-  return chunk * kVerifyChunk + (j * kVerifyThreads + (int)threadIdx.x) * 4;
+// A wave's part of a row: float4 j of lane l is ids 256 j + 4 l of the part.
+// (One test per part, so that its loads are all on their way together.)
+__device__ __forceinline__ int part_id(int part, int j) {
+  return part * kVerifyPart + j * 256 + (int)(threadIdx.x & 63) * 4;
+}
+template <int n>
+__device__ __forceinline__ void load_part_of(const float *row, int part, int j0, int vocab,
+                                             Float4 (&v)[n]) {
+  if ((part + 1) * kVerifyPart <= vocab) {
+#pragma unroll
+    for (int j = 0; j < n; ++j) v[j] = *reinterpret_cast<const Float4 *>(row + part_id(part, j0 + j));
+  } else {
+#pragma unroll
+    for (int j = 0; j < n; ++j) v[j] = load4(row, part_id(part, j0 + j), vocab);
+  }
 }
 
 struct VerifySmem {
-  float fmax[kWavesV];
-  int imin[kWavesV], imax[kWavesV];
   double sum[kWavesV];
+  int imin[kWavesV], imax[kWavesV];
   int32_t last;
   VerifyStat stat[2];
-  int acc, chunk;
-  double at;                 // the draw, within the chunk
+  int acc, pick;
+  double at;                 // the draw, within the part
 };
 
 // One side's distribution at a position: what a row's elements are turned
@@ -256,31 +270,40 @@ __device__ __forceinline__ double prob_at(const Row &r, int id, int vocab) {
   return id >= 0 && id < vocab ? prob(r, r.p[id], id) : 0.0;
 }
 
-__device__ Verdict judge_at(const VerifyArgs &a, int b, const Range &r, int i,
-                            const VerifyStat &st, const VerifyStat &sq) {
+__device__ __forceinline__ Verdict judge_at(const VerifyArgs &a, int b, const Range &r, int i,
+                                            const VerifyStat &st, const VerifyStat &sq) {
   const int x = a.d.drafts[r.start + i];
   const double p = prob_at(row_of(a, 0, b, r.start + b + i, st), x, a.vocab);
   const double q = a.kind[1] == kDistNone ? 1.0 : prob_at(row_of(a, 1, b, r.start + i, sq), x, a.vocab);
   return judge(p, q, a.d.uniforms[r.start + b + i]);
 }
 
-// A row's summary from its chunks', by one wave.
-__device__ VerifyStat combine(const VerifyPart *part, int chunks, double T) {
+// A row's summary from its parts', by one wave.
+__device__ __forceinline__ VerifyStat combine(const VerifyPart *part, int parts, double T) {
   const int lane = threadIdx.x & 63;
   const double c = log2_scale(T);
   const bool greedy = greedy_temp(T);
   VerifyStat r;
-  float m = -__builtin_inff();
-  for (int i = lane; i < chunks; i += 64) m = fmaxf(m, load_part(part + i).m);
+  // (most rows have at most two parts a lane: those stay in registers)
+  VerifyPart own[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    own[i] = {0.0, -__builtin_inff(), 0x7FFFFFFF};
+    if (lane + 64 * i < parts) own[i] = load_part(part + lane + 64 * i);
+  }
+  float m = fmaxf(own[0].m, own[1].m);
+  for (int i = lane + 128; i < parts; i += 64) m = fmaxf(m, load_part(part + i).m);
   r.m = wave_max(m);
   const float mm = max_or_nan(r.m);
   double s = 0.0;
   int arg = 0x7FFFFFFF;
-  for (int i = lane; i < chunks; i += 64) {
-    const VerifyPart p = load_part(part + i);
+  auto add = [&](const VerifyPart &p) {
     s += p.s * weight(p.m, mm, c);
     if (p.m == mm) arg = min(arg, p.arg);
-  }
+  };
+  add(own[0]);
+  add(own[1]);
+  for (int i = lane + 128; i < parts; i += 64) add(load_part(part + i));
   r.s = greedy ? 1.0 : wave_sum(s);
   r.arg = greedy ? wave_min(arg) : -1;
   if (r.m == -__builtin_inff()) {
@@ -288,90 +311,6 @@ __device__ VerifyStat combine(const VerifyPart *part, int chunks, double T) {
     r.arg = -1;
   }
   return r;
-}
-
-// One workgroup per chunk of a row of logits: its maximum and the sum of its
-// weights.  The rows of every sequence's first position come first in the
-// grid, then the second's and so on; the workgroup that completes a position
-// judges its draft, and a workgroup of a position behind a rejection found by
-// then ends at once: nothing of its rows is asked for.  (Whether it is found
-// in time changes what is read, never the outcome.)
-__global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs a) {
-  __shared__ VerifySmem sm;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const bool both = a.kind[0] == kDistLogits && a.kind[1] == kDistLogits;
-  const int pos = both ? blockIdx.z >> 1 : blockIdx.z;
-  const int side = both ? blockIdx.z & 1 : a.kind[0] != kDistLogits;
-  const int b = blockIdx.y;
-  const Range r = drafts_of(a.d, b);
-  if (pos > r.n || (side == 1 && pos == r.n) || (a.d.done && a.d.done[b])) return;
-  const uint32_t rej = load_agent32(a.rejected + b);
-  if (rej && 64 - (int)rej < pos) return;
-  const double T = a.temps[side] ? a.temps[side][b] : 1.0;
-  const bool greedy = greedy_temp(T);
-  const int64_t row = side ? r.start + pos : r.start + b + pos;
-  const int chunk = blockIdx.x;
-  const float *rowp = a.rows[side] + row * a.stride[side];
-  Float4 v[kVerifyPer / 4];
-#pragma unroll
-  for (int j = 0; j < kVerifyPer / 4; ++j) v[j] = load4(rowp, chunk_id(chunk, j), a.vocab);
-  float m = -__builtin_inff();
-#pragma unroll
-  for (int i = 0; i < kVerifyPer; ++i) m = fmaxf(m, v[i / 4].v[i % 4]);
-  m = wave_max(m);
-  if (lane == 0) sm.fmax[wave] = m;
-  __syncthreads();
-  m = sm.fmax[0];
-#pragma unroll
-  for (int w = 1; w < kWavesV; ++w) m = fmaxf(m, sm.fmax[w]);
-  VerifyPart part;
-  part.m = m;
-  part.s = 0.0;
-  part.arg = -1;
-  const float mm = max_or_nan(m);
-  if (greedy) {
-    int arg = 0x7FFFFFFF;
-#pragma unroll
-    for (int i = 0; i < kVerifyPer; ++i)
-      if (v[i / 4].v[i % 4] == mm) arg = min(arg, chunk_id(chunk, i / 4) + i % 4);
-    arg = wave_min(arg);
-    if (lane == 0) sm.imin[wave] = arg;
-    __syncthreads();
-    if (tid == 0)
-      for (int w = 0; w < kWavesV; ++w) part.arg = w ? min(part.arg, sm.imin[w]) : sm.imin[0];
-  } else {
-    const double c = log2_scale(T);
-    double s = 0.0;
-#pragma unroll
-    for (int i = 0; i < kVerifyPer; ++i) s += weight(v[i / 4].v[i % 4], mm, c);
-    s = wave_sum(s);
-    if (lane == 0) sm.sum[wave] = s;
-    __syncthreads();
-    if (tid == 0)
-      for (int w = 0; w < kWavesV; ++w) part.s += sm.sum[w];
-  }
-  if (tid == 0) store_part(a.part[side] + row * a.chunks + chunk, part);
-  const bool two = both && pos < r.n;
-  const int slot = b * (a.d.max_drafts + 1) + pos;
-  if (!arrive(a.arrived + slot, (uint32_t)a.chunks * (two ? 2u : 1u), &sm.last)) return;
-  // both rows of the position are done
-  if (wave < 2) {
-    const int64_t wr = wave ? r.start + pos : r.start + b + pos;
-    if (a.kind[wave] == kDistLogits && (wave == 0 || pos < r.n)) {
-      const VerifyStat st = combine(a.part[wave] + wr * a.chunks, a.chunks,
-                                    a.temps[wave] ? a.temps[wave][b] : 1.0);
-      if (lane == 0) {
-        sm.stat[wave] = st;
-        a.stat[wave][wr] = st;
-      }
-    }
-  }
-  __syncthreads();
-  if (tid == 0 && pos < r.n) {
-    const Verdict vd = judge_at(a, b, r, pos, sm.stat[0], sm.stat[1]);
-    a.verdict[slot] = vd;
-    if (!vd.ok) atomicMax(a.rejected + b, (uint32_t)(64 - pos));
-  }
 }
 
 // What the final token is drawn from, per element of the row.
@@ -388,213 +327,347 @@ __device__ __forceinline__ double final_weight(const Final &f, float vp, float v
   return fmax(p - prob(f.q, vq, id), 0.0);
 }
 
-__device__ double chunk_mass(const VerifyArgs &a, const Final &f, int chunk, VerifySmem &sm) {
-  const int tid = threadIdx.x;
+// The mass of a part, by one wave.
+__device__ __forceinline__ double part_mass(const VerifyArgs &a, const Final &f, int part) {
   double s = 0.0;
 #pragma unroll 1
-  for (int j0 = 0; j0 < kVerifyPer / 4; j0 += 4) {
+  for (int h = 0; h < kVerifyPer / 4; h += 4) {
     Float4 vp[4], vq[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) vp[j] = load4(f.p.p, chunk_id(chunk, j0 + j), a.vocab);
-    if (f.pair) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) vq[j] = load4(f.q.p, chunk_id(chunk, j0 + j), a.vocab);
-    }
+    load_part_of(f.p.p, part, h, a.vocab, vp);
+    if (f.pair) load_part_of(f.q.p, part, h, a.vocab, vq);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       s += final_weight(f, vp[i / 4].v[i % 4], f.pair ? vq[i / 4].v[i % 4] : 0.0f,
-                        chunk_id(chunk, j0 + i / 4) + i % 4);
+                        part_id(part, h + i / 4) + i % 4);
   }
-  s = wave_sum(s);
-  __syncthreads();
-  if ((tid & 63) == 0) sm.sum[tid >> 6] = s;
-  __syncthreads();
-  s = 0.0;
-  for (int w = 0; w < kWavesV; ++w) s += sm.sum[w];
-  return s;
+  return wave_sum(s);
 }
 
-// The first id whose running sum is above u times the whole, from the chunks'
-// masses; -1 where the whole is 0.  Every thread of the workgroup.
-__device__ int draw_id(const VerifyArgs &a, const Final &f, const double *mass, double u,
-                       VerifySmem &sm) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (wave == 0) {
-    double total = 0.0;
-    int live = -1;           // the last chunk with any mass
-    for (int c0 = 0; c0 < a.chunks; c0 += 64) {
-      const double v = c0 + lane < a.chunks
-                           ? __longlong_as_double((long long)load_agent64(mass + c0 + lane)) : 0.0;
-      live = max(live, v > 0.0 ? c0 + lane : -1);
-      total += __shfl(wave_scan(v), 63);
-    }
-    live = wave_max(live);
-    const double at = u * total;
-    int chunk = live;
-    double before = 0.0, within = __builtin_inf();   // (past the end: the last id with mass)
-    for (int c0 = 0; c0 < a.chunks; c0 += 64) {
-      const double v = c0 + lane < a.chunks
-                           ? __longlong_as_double((long long)load_agent64(mass + c0 + lane)) : 0.0;
-      const double s = wave_scan(v);
-      const unsigned long long hit = __ballot(v > 0.0 && before + s > at);
-      if (hit) {
-        const int l = __ffsll(hit) - 1;
-        chunk = c0 + l;
-        const double up = __shfl(s, max(l - 1, 0));
-        within = at - (before + (l ? up : 0.0));
-        break;
-      }
-      before += __shfl(s, 63);
-    }
-    if (lane == 0) {
-      sm.chunk = total > 0.0 ? chunk : -1;
-      sm.at = within;
-    }
-  }
-  __syncthreads();
-  const int chunk = sm.chunk, base = chunk * kVerifyChunk;
-  const double at = sm.at;
-  __syncthreads();   // (both are written again below)
-  if (chunk < 0) return -1;
-  // kVerifyPer consecutive ids a thread: the thread that the draw falls to,
-  // then its ids one a lane
-  const int id0 = base + tid * kVerifyPer;
-  double own = 0.0;
-#pragma unroll 1
-  for (int j0 = 0; j0 < kVerifyPer; j0 += 8) {
-    Float4 vp[2], vq[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) vp[j] = load4(f.p.p, id0 + j0 + 4 * j, a.vocab);
-    if (f.pair) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) vq[j] = load4(f.q.p, id0 + j0 + 4 * j, a.vocab);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      own += final_weight(f, vp[i / 4].v[i % 4], f.pair ? vq[i / 4].v[i % 4] : 0.0f, id0 + j0 + i);
-  }
+// The running sums of a value per thread over the workgroup: this thread's
+// (before it, and with it) and the whole.
+struct Scan {
+  double before, end, total;
+};
+__device__ __forceinline__ Scan block_scan(double own, VerifySmem &sm) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const double incl = wave_scan(own);
+  __syncthreads();
   if (lane == 63) sm.sum[wave] = incl;
   __syncthreads();
-  double start = 0.0;
-  for (int i = 0; i < wave; ++i) start += sm.sum[i];
+  double start = 0.0, total = 0.0;
+  for (int i = 0; i < kWavesV; ++i) {
+    if (i < wave) start += sm.sum[i];
+    total += sm.sum[i];
+  }
   const double up = __shfl_up(incl, 1);
-  const double before = start + (lane ? up : 0.0);
-  const unsigned long long hit = __ballot(own > 0.0 && start + incl > at);
-  const unsigned long long any = __ballot(own > 0.0);
+  return {start + (lane ? up : 0.0), start + incl, total};
+}
+// The first thread with `hit`, else the last with `any`, else -1.
+__device__ __forceinline__ int block_first(bool hit, bool any, bool *past, VerifySmem &sm) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned long long h = __ballot(hit), n = __ballot(any);
   if (lane == 0) {
-    sm.imin[wave] = hit ? tid + __ffsll(hit) - 1 : kVerifyThreads;
-    sm.imax[wave] = any ? tid + 63 - __clzll(any) : -1;
+    sm.imin[wave] = h ? wave * 64 + __ffsll(h) - 1 : kVerifyThreads;
+    sm.imax[wave] = n ? wave * 64 + 63 - __clzll(n) : -1;
   }
   __syncthreads();
-  int owner = kVerifyThreads, live = -1;
+  int first = kVerifyThreads, live = -1;
   for (int i = 0; i < kWavesV; ++i) {
-    owner = min(owner, sm.imin[i]);
+    first = min(first, sm.imin[i]);
     live = max(live, sm.imax[i]);
   }
-  const bool past = owner == kVerifyThreads;   // (rounding: the last id with mass)
-  if (past) owner = live;
-  if (tid == owner) sm.at = past ? __builtin_inf() : at - before;
-  __syncthreads();
-  if (wave == 0) {
-    const int id = base + owner * kVerifyPer + lane;
-    const bool in = lane < kVerifyPer && owner >= 0 && id < a.vocab;
-    const double w = in ? final_weight(f, f.p.p[id], f.pair ? f.q.p[id] : 0.0f, id) : 0.0;
-    const double s = wave_scan(w);
-    const unsigned long long h = __ballot(w > 0.0 && s > sm.at), n = __ballot(w > 0.0);
-    const int l = h ? __ffsll(h) - 1 : n ? 63 - __clzll(n) : -1;
-    if (lane == 0) sm.chunk = l >= 0 ? base + owner * kVerifyPer + l : -1;
-  }
-  __syncthreads();
-  return sm.chunk;
+  *past = first == kVerifyThreads;
+  return *past ? live : first;
 }
 
-// One workgroup per chunk of a sequence's final row: the mass of what the
-// final token is drawn from (taken from the first kernel where the chunk's sum
-// is that already); the one that completes the row draws and writes the
-// sequence's outcome.
-__global__ __launch_bounds__(kVerifyThreads) void verify_resolve_kernel(VerifyArgs a) {
+// The first id whose running sum is above u times the whole, from the parts'
+// masses (mass(part)); -1 where the whole is 0.  Every thread of the workgroup:
+// each takes consecutive parts, the one the draw falls to finds its part, then
+// each takes eight consecutive ids of that part.
+template <typename Mass>
+__device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, double u, Mass mass,
+                                       VerifySmem &sm) {
+  const int tid = threadIdx.x;
+  const int per = (a.parts + kVerifyThreads - 1) / kVerifyThreads;
+  const int c0 = min(tid * per, a.parts), c1 = min(c0 + per, a.parts);
+  const double one = c0 < c1 ? mass(c0) : 0.0;
+  double own = one;
+  for (int c = c0 + 1; c < c1; ++c) own += mass(c);
+  const Scan all = block_scan(own, sm);
+  const double at = u * all.total;
+  bool past;
+  int who = block_first(own > 0.0 && all.end > at, own > 0.0, &past, sm);
+  if (who < 0) return -1;
+  if (tid == who) {
+    double run = all.before, m = one;
+    int c = c0, live = c0;
+    double before = run;
+    for (;; m = mass(c)) {
+      if (m > 0.0) {
+        live = c;
+        before = run;
+        if (!past && run + m > at) break;
+      }
+      run += m;
+      if (++c >= c1) break;
+    }
+    sm.pick = live;
+    // (past the end by rounding: the last id with mass)
+    sm.at = past || c >= c1 ? __builtin_inf() : at - before;
+  }
+  __syncthreads();
+  const int part = sm.pick;
+  const double in = sm.at;
+  const int id0 = part * kVerifyPart + tid * 8;
+  Float4 vp[2], vq[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    vp[j] = load4(f.p.p, id0 + 4 * j, a.vocab);
+    if (f.pair) vq[j] = load4(f.q.p, id0 + 4 * j, a.vocab);
+  }
+  double w[8];
+  own = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = final_weight(f, vp[i / 4].v[i % 4], f.pair ? vq[i / 4].v[i % 4] : 0.0f, id0 + i);
+    own += w[i];
+  }
+  const Scan ids = block_scan(own, sm);
+  who = block_first(own > 0.0 && ids.end > in, own > 0.0, &past, sm);
+  if (tid == who) {
+    double run = ids.before;
+    int first = -1, live = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      run += w[i];
+      if (w[i] > 0.0) {
+        live = id0 + i;
+        if (first < 0 && run > in) first = live;
+      }
+    }
+    sm.pick = !past && first >= 0 ? first : live;
+  }
+  __syncthreads();
+  return who < 0 ? -1 : sm.pick;
+}
+
+// The outcome of a sequence whose final row's masses are the parts' sums that
+// the rows' workgroups published (no draft rows to take off), by the workgroup
+// that left last.
+__device__ __forceinline__ int draw_from_parts(const VerifyArgs &a, Final f, int64_t row, double u,
+                                               VerifySmem &sm) {
+  const VerifyPart *part = a.part[0] + row * a.parts;
+  // a certain draft's own id is taken out of its part
+  const int xp = f.residual && f.x >= 0 && f.x < a.vocab ? f.x / kVerifyPart : -1;
+  for (;;) {
+    double without = 0.0;
+    if (f.residual && xp >= 0) {   // (each wave for itself: the same sum)
+      without = part_mass(a, f, xp);
+    }
+    const bool out = f.residual && xp >= 0;
+    const int id = draw_id(a, f, u, [&](int c) {
+      if (out && c == xp) return without;
+      const VerifyPart p = load_part(part + c);
+      return p.s * weight(p.m, f.p.m, f.p.c) * f.p.inv;
+    }, sm);
+    if (id >= 0 || !f.residual) return max(id, 0);
+    f.residual = false;   // all of p is x: from p itself
+    __syncthreads();
+  }
+}
+
+// One workgroup per kVerifyBlock logits of a row, a wave for each part: its
+// maximum and the sum of its weights.  The rows of every sequence's first
+// position come first in the grid, then the second's and so on; the workgroup
+// that completes a position judges its draft, and a workgroup of a position
+// behind a rejection found by then ends at once: nothing of its rows is asked
+// for.  (Whether it is found in time changes what is read, never the outcome.)
+// The workgroup that leaves a sequence last writes its outcome, unless a
+// rejection leaves p - q to be summed (verify_open_kernel).
+__global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = blockIdx.y, chunk = blockIdx.x;
+  const bool both = a.kind[0] == kDistLogits && a.kind[1] == kDistLogits;
+  const int pos = both ? blockIdx.z >> 1 : blockIdx.z;
+  const int side = both ? blockIdx.z & 1 : a.kind[0] != kDistLogits;
+  const int b = blockIdx.y;
   const Range r = drafts_of(a.d, b);
+  // (rows of draft logits beside target probabilities: none at position n)
+  if (pos > r.n || (side == 1 && pos == r.n && (both || pos > 0))) return;
   if (a.d.done && a.d.done[b]) {   // done before this call
-    if (chunk == 0 && wave == 0) emit(a.d, b, r, -1, -1, 0.0f, 0);
+    if (blockIdx.x == 0 && blockIdx.z == 0 && wave == 0) {
+      emit(a.d, b, r, -1, -1, 0.0f, 0);
+      if (lane == 0) a.open[b] = -1;
+    }
     return;
   }
-  const bool judged = a.kind[0] == kDistLogits || a.kind[1] == kDistLogits;
-  const int slot = b * (a.d.max_drafts + 1);
+  const int slot = b * (a.d.max_drafts + 1) + pos;
+  // (read once for the whole workgroup: the waves must agree on it, and it may
+  // change between two reads)
+  if (tid == 0) sm.acc = (int)load_agent32(a.rejected + b);
+  __syncthreads();
+  const int rej = sm.acc;
+  const int64_t row = side ? r.start + pos : r.start + b + pos;
+  const bool there = !(side == 1 && pos == r.n);   // (a sequence without drafts still leaves)
+  if (there && !(rej && 64 - rej < pos)) {
+    const double T = a.temps[side] ? a.temps[side][b] : 1.0;
+    const int part = (int)blockIdx.x * kWavesV + wave;
+    if (part < a.parts) {
+      Float4 v[kVerifyPer / 4];
+      load_part_of(a.rows[side] + row * a.stride[side], part, 0, a.vocab, v);
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < kVerifyPer; ++i) m = fmaxf(m, v[i / 4].v[i % 4]);
+      VerifyPart out;
+      out.m = wave_max(m);
+      out.s = 0.0;
+      out.arg = -1;
+      const float mm = max_or_nan(out.m);
+      if (greedy_temp(T)) {
+        int arg = 0x7FFFFFFF;
+#pragma unroll
+        for (int i = 0; i < kVerifyPer; ++i)
+          if (v[i / 4].v[i % 4] == mm) arg = min(arg, part_id(part, i / 4) + i % 4);
+        out.arg = wave_min(arg);
+      } else {
+        if (mm == __builtin_inff()) {
+#pragma unroll
+          for (int i = 0; i < kVerifyPer; ++i) out.s += v[i / 4].v[i % 4] == mm ? 1.0 : 0.0;
+        } else {
+          const double c = log2_scale(T);
+#pragma unroll
+          for (int i = 0; i < kVerifyPer; ++i) out.s += weight_below(v[i / 4].v[i % 4], mm, c);
+        }
+        out.s = wave_sum(out.s);
+      }
+      if (lane == 0) store_part(a.part[side] + row * a.parts + part, out);
+    }
+    const bool two = both && pos < r.n;
+    if (arrive(a.arrived + slot, (uint32_t)a.blocks * (two ? 2u : 1u), &sm.last)) {
+      // both rows of the position are done
+      if (wave < 2) {
+        const int64_t wr = wave ? r.start + pos : r.start + b + pos;
+        if (a.kind[wave] == kDistLogits && (wave == 0 || pos < r.n)) {
+          const VerifyStat st = combine(a.part[wave] + wr * a.parts, a.parts,
+                                        a.temps[wave] ? a.temps[wave][b] : 1.0);
+          if (lane == 0) {
+            sm.stat[wave] = st;
+            store_part(a.stat[wave] + wr, st);
+          }
+        }
+      }
+      __syncthreads();
+      if (tid == 0 && pos < r.n) {
+        const Verdict vd = judge_at(a, b, r, pos, sm.stat[0], sm.stat[1]);
+        const unsigned long long w =
+            (unsigned long long)__float_as_uint(vd.ratio) | ((unsigned long long)(uint32_t)vd.ok << 32);
+        __hip_atomic_store(reinterpret_cast<unsigned long long *>(a.verdict + slot), w,
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (!vd.ok) atomicMax(a.rejected + b, (uint32_t)(64 - pos));
+      }
+    }
+  }
+  // out of the sequence
+  const int rows = both ? 2 * r.n + 1 : side ? max(r.n, 1) : r.n + 1;
+  if (!arrive(a.left + b, (uint32_t)(a.blocks * rows), &sm.last)) return;
   float ratio = 0.0f;
   if (wave == 0) {
-    Verdict v = {0.0f, 0};
-    if (lane < r.n) {
-      const VerifyStat none = {};
-      v = judged ? a.verdict[slot + lane] : judge_at(a, b, r, lane, none, none);
-    }
-    const int acc = first_rejected(v.ok != 0, r.n);
-    ratio = v.ratio;
+    unsigned long long w = 0;
+    if (lane < r.n) w = load_agent64(a.verdict + slot - pos + lane);
+    ratio = __uint_as_float((uint32_t)w);
+    const int acc = first_rejected((w >> 32) != 0, r.n);
     if (lane == 0) sm.acc = acc;
+  }
+  // zero for the next call
+  for (int i = tid; i <= a.d.max_drafts; i += kVerifyThreads)
+    store_agent(a.arrived + (int64_t)b * (a.d.max_drafts + 1) + i, 0u);
+  if (tid == 0) {
+    store_agent(a.rejected + b, 0u);
+    store_agent(a.left + b, 0u);
   }
   __syncthreads();
   const int acc = sm.acc;
-  const bool last_row = acc == r.n;
-  const int64_t row = r.start + b + acc;
-  const VerifyStat none = {};
+  // p - q, or a row of probabilities, is still to be summed
+  const bool open = a.kind[0] != kDistLogits || (acc < r.n && a.kind[1] != kDistNone);
   Final f;
-  f.p = row_of(a, 0, b, row, a.kind[0] == kDistLogits ? a.stat[0][row] : none);
-  f.residual = !last_row;
-  f.pair = f.residual && a.kind[1] != kDistNone;
-  f.x = f.residual ? a.d.drafts[r.start + acc] : -1;
-  if (f.pair)
-    f.q = row_of(a, 1, b, r.start + acc, a.kind[1] == kDistLogits ? a.stat[1][r.start + acc] : none);
-  int token = 0;
-  const bool logits = f.p.kind == kDistLogits;
+  const int64_t fr = r.start + b + acc;
+  if (a.kind[0] == kDistLogits) f.p = row_of(a, 0, b, fr, load_part(a.stat[0] + fr));
   // greedy: its one id.  No candidate at all: 0, as the sampler's
-  const bool known = logits && (f.p.greedy || !(f.p.inv > 0.0));
+  const bool known = a.kind[0] == kDistLogits && (f.p.greedy || !(f.p.inv > 0.0));
+  if (tid == 0 && a.open) a.open[b] = open && !known ? acc : -1;
+  if (open && !known) return;
+  int token;
   if (known) {
-    if (chunk != 0) return;
     token = max(f.p.arg, 0);
   } else {
-    const VerifyPart *part = logits ? a.part[0] + row * a.chunks : nullptr;
-    double *mass = a.mass + (int64_t)b * a.chunks;
-    const double u = a.d.uniforms[r.start + b + r.n];
-    // this chunk; then, where nothing is left beyond q (or x), all of p by the
-    // workgroup that found it so
-    int c0 = chunk, c1 = chunk + 1;
-    for (int again = 0;; ++again) {
-      for (int c = c0; c < c1; ++c) {
-        double s;
-        if (logits && !f.pair && !(f.residual && f.x >= 0 && f.x / kVerifyChunk == c)) {
-          const VerifyPart p = load_part(part + c);
-          s = p.s * weight(p.m, f.p.m, f.p.c) * f.p.inv;
-        } else {
-          s = chunk_mass(a, f, c, sm);
-        }
-        if (tid == 0) store_agent(mass + c, s);
-      }
-      if (!again) {
-        if (!arrive(a.arrived_final + b, (uint32_t)a.chunks, &sm.last)) return;
-      } else {
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-      }
-      token = draw_id(a, f, mass, u, sm);
-      if (token >= 0 || again) break;
-      f.residual = f.pair = false;
-      c0 = 0;
-      c1 = a.chunks;
-      __syncthreads();
-    }
-    token = max(token, 0);
+    f.residual = acc < r.n;
+    f.pair = false;
+    f.x = f.residual ? a.d.drafts[r.start + acc] : -1;
+    token = draw_from_parts(a, f, fr, a.d.uniforms[r.start + b + r.n], sm);
   }
   if (wave == 0) emit(a.d, b, r, acc, token, ratio, 0);
-  // zero for the next call
-  if (judged)
-    for (int i = tid; i <= a.d.max_drafts; i += kVerifyThreads) store_agent(a.arrived + slot + i, 0u);
-  if (tid == 0) {
-    store_agent(a.rejected + b, 0u);
-    store_agent(a.arrived_final + b, 0u);
+}
+
+// The sequences that a rejection left open, and every one where no side has
+// logits: one workgroup per kVerifyBlock ids of the final row sums what the
+// final token is drawn from, and the one that completes the row draws.
+__global__ __launch_bounds__(kVerifyThreads, 4) void verify_open_kernel(VerifyArgs a) {
+  __shared__ VerifySmem sm;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.y;
+  const Range r = drafts_of(a.d, b);
+  const bool judged = a.kind[0] == kDistLogits || a.kind[1] == kDistLogits;
+  const int slot = b * (a.d.max_drafts + 1);
+  Verdict v = {0.0f, 0};
+  int acc;
+  if (judged) {
+    acc = a.open[b];
+    if (acc < 0) return;
+    if (lane < r.n) v = a.verdict[slot + lane];
+  } else {
+    if (a.d.done && a.d.done[b]) {   // done before this call
+      if (blockIdx.x == 0 && wave == 0) emit(a.d, b, r, -1, -1, 0.0f, 0);
+      return;
+    }
+    const VerifyStat none = {};
+    if (lane < r.n) v = judge_at(a, b, r, lane, none, none);
+    acc = first_rejected(v.ok != 0, r.n);   // (each wave the same)
   }
+  const VerifyStat none = {};
+  const int64_t row = r.start + b + acc, drow = r.start + acc;
+  Final f;
+  f.p = row_of(a, 0, b, row, a.kind[0] == kDistLogits ? a.stat[0][row] : none);
+  f.residual = acc < r.n;
+  f.pair = f.residual && a.kind[1] != kDistNone;
+  f.x = f.residual ? a.d.drafts[drow] : -1;
+  if (f.pair) f.q = row_of(a, 1, b, drow, a.kind[1] == kDistLogits ? a.stat[1][drow] : none);
+  double *mass = a.mass + (int64_t)b * a.parts;
+  const double u = a.d.uniforms[r.start + b + r.n];
+  // this workgroup's parts; then, where nothing is left beyond q (or x), all
+  // of p's by the workgroup that found it so
+  int p0 = (int)blockIdx.x * kWavesV, p1 = min(p0 + kWavesV, a.parts), token;
+  for (int again = 0;; ++again) {
+    for (int p = p0 + wave; p < p1; p += kWavesV) {
+      const double s = part_mass(a, f, p);
+      if (lane == 0) store_agent(mass + p, s);
+    }
+    if (!again) {
+      if (!arrive(a.left + b, (uint32_t)a.blocks, &sm.last)) return;
+    } else {
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    }
+    token = draw_id(a, f, u, [&](int c) {
+      return __longlong_as_double((long long)load_agent64(mass + c));
+    }, sm);
+    if (token >= 0 || again) break;
+    f.residual = f.pair = false;
+    p0 = 0;
+    p1 = a.parts;
+    __syncthreads();
+  }
+  if (wave == 0) emit(a.d, b, r, acc, max(token, 0), v.ratio, 0);
+  if (tid == 0) store_agent(a.left + b, 0u);   // for the next call
 }
 
 // ---- candidate lists
@@ -807,16 +880,20 @@ hipError_t launch_v(K kernel, dim3 grid, size_t lds, hipStream_t stream, hipEven
 }  // namespace
 
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream, hipEvent_t *ev_stats,
-                         hipEvent_t *ev_resolve, hipEvent_t done) {
-  const int sides = (a.kind[0] == kDistLogits) + (a.kind[1] == kDistLogits);
-  if (sides > 0) {
-    const dim3 grid((unsigned)a.chunks, (unsigned)a.d.seqs,
-                    (unsigned)((a.d.max_drafts + 1) * (sides == 2 ? 2 : 1)));
-    const hipError_t e = launch_v(verify_stats_kernel, grid, 0, stream, ev_stats, nullptr, a);
+                         hipEvent_t *ev_open, hipEvent_t done) {
+  const unsigned launches = verify_launches(a);
+  if (launches & 1u) {
+    const bool both = a.kind[0] == kDistLogits && a.kind[1] == kDistLogits;
+    const dim3 grid((unsigned)a.blocks, (unsigned)a.d.seqs,
+                    (unsigned)((a.d.max_drafts + 1) * (both ? 2 : 1)));
+    const hipError_t e = launch_v(verify_stats_kernel, grid, 0, stream, ev_stats,
+                                  launches & 2u ? nullptr : done, a);
     if (e != hipSuccess) return e;
   }
-  return launch_v(verify_resolve_kernel, dim3((unsigned)a.chunks, (unsigned)a.d.seqs), 0, stream,
-                  ev_resolve, done, a);
+  if (launches & 2u)
+    return launch_v(verify_open_kernel, dim3((unsigned)a.blocks, (unsigned)a.d.seqs), 0, stream,
+                    ev_open, done, a);
+  return hipSuccess;
 }
 
 // (the longest lists' table and the kernel's own LDS pass 64 KB)
