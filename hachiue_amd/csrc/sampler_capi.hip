@@ -1268,6 +1268,7 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
   a.vocab = vocab;
   a.parts = (vocab + hs::kVerifyPart - 1) / hs::kVerifyPart;
   a.blocks = (vocab + hs::kVerifyBlock - 1) / hs::kVerifyBlock;
+  hs::verify_split(a);
   const size_t rows[2] = {(size_t)a.d.n_drafts + (size_t)a.d.seqs, (size_t)a.d.n_drafts};
   const size_t judged = (size_t)a.d.seqs * (size_t)(a.d.max_drafts + 1);
   size_t need = 0;

@@ -424,6 +424,7 @@ static_assert(sizeof(VerifyPart) == 16, "VerifyPart layout");
 using VerifyStat = VerifyPart;
 // A drafted position's outcome.
 struct Verdict {
+  double p;                  // the draft's, of the target
   float ratio;               // min(1, p / q)
   int32_t ok;                // accepted
 };
@@ -453,13 +454,17 @@ struct VerifyArgs {
   int64_t stride[2];
   const double *temps[2];    // [seqs] or null: 1
   int32_t kind[2];           // DistKind
-  int32_t vocab, parts, blocks;   // parts of a row, workgroups of a row
+  int32_t vocab, parts;      // parts of a row
+  int32_t split;             // workgroups of a row: the rows' sums,
+  int32_t blocks;            //   and the rows that are left open
+  int32_t look;              // more workgroups than start at once: the later ones
+                             //   look for a rejection before they read
   VerifyPart *part[2];       // [rows][parts] of the sides that are logits
   VerifyStat *stat[2];       // [rows]
   Verdict *verdict;          // [seqs][max_drafts + 1]
   double *mass;              // [seqs][parts]
   int32_t *open;             // [seqs] the rejected position, -1: the outcome is written
-  // zero between calls: workgroups counted in per position, and out per
+  // zero between calls: workgroups done with a position, positions done of a
   // sequence, the first rejection found so far (64 - position)
   uint32_t *arrived;         // [seqs][max_drafts + 1]
   uint32_t *rejected;        // [seqs]
@@ -470,6 +475,18 @@ struct VerifyArgs {
 inline unsigned verify_launches(const VerifyArgs &a) {
   const bool sums = a.kind[0] == kDistLogits || a.kind[1] == kDistLogits;
   return (sums ? 1u : 0u) | (!sums || a.kind[0] != kDistLogits || a.kind[1] != kDistNone ? 2u : 0u);
+}
+// Workgroups of a row whose logits are summed: enough that all rows together
+// give each compute unit four, but each has up to kVerifyDeep blocks of
+// kVerifyBlock logits to itself.
+constexpr int kVerifyDeep = 4;
+inline void verify_split(VerifyArgs &a) {
+  const int64_t rows = (a.kind[0] == kDistLogits ? a.d.n_drafts + a.d.seqs : 0) +
+                       (a.kind[1] == kDistLogits ? a.d.n_drafts : 0);
+  const int64_t want = rows > 0 ? 4 * kSplitCUs / rows : 1;
+  const int64_t least = (a.blocks + kVerifyDeep - 1) / kVerifyDeep;
+  a.split = (int32_t)(want < least ? least : want > a.blocks ? a.blocks : want);
+  a.look = rows * a.split > 4 * kSplitCUs;
 }
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream, hipEvent_t *ev_stats,
                          hipEvent_t *ev_resolve, hipEvent_t done);

@@ -70,23 +70,23 @@ __device__ __forceinline__ bool arrive(uint32_t *cnt, uint32_t of, int32_t *last
   return *last != 0;
 }
 
-// 2^d for d <= 0 (NaN: 0), to 1e-15: n = round(d), 2^(d - n) by a polynomial
-// 1 + f g(f), g the Chebyshev interpolant of (2^f - 1) / f of degree 9 on
-// [-1/2, 1/2].  Exact at whole d.
+// 2^d for d <= 0 (NaN: 0), to 4e-14.  n = round(d), 2^(d - n) by a polynomial 1 + f g(f),
+// g the Chebyshev interpolant of (2^f - 1) / f of degree 8 on [-1/2, 1/2].
+// Exact at whole d.  (Rounding, scaling and conversions take no longer than a
+// multiplication here.)
 __device__ __forceinline__ double exp2_neg(double d) {
   d = fmax(d, -1100.0);   // (below 2^-1074; a NaN takes the other operand)
   const double n = rint(d);
   const double f = d - n;
-  double g = 0x1.e5e9f548e5726p-28;
-  g = __builtin_fma(g, f, 0x1.b6571de2f2351p-24);
-  g = __builtin_fma(g, f, 0x1.62bfe46117445p-20);
-  g = __builtin_fma(g, f, 0x1.ffcb76789860fp-17);
-  g = __builtin_fma(g, f, 0x1.4309130378460p-13);
-  g = __builtin_fma(g, f, 0x1.5d87fe908f88ap-10);
-  g = __builtin_fma(g, f, 0x1.3b2ab6fba385fp-7);
-  g = __builtin_fma(g, f, 0x1.c6b08d7044119p-5);
-  g = __builtin_fma(g, f, 0x1.ebfbdff82c590p-3);
-  g = __builtin_fma(g, f, 0x1.62e42fefa39f7p-1);
+  double g = 0x1.b63880a30e9ffp-24;
+  g = __builtin_fma(g, f, 0x1.63d136366db24p-20);
+  g = __builtin_fma(g, f, 0x1.ffcb9515a8016p-17);
+  g = __builtin_fma(g, f, 0x1.4308ac85aa947p-13);
+  g = __builtin_fma(g, f, 0x1.5d87fe86fe88ep-10);
+  g = __builtin_fma(g, f, 0x1.3b2ab7181b755p-7);
+  g = __builtin_fma(g, f, 0x1.c6b08d7047e52p-5);
+  g = __builtin_fma(g, f, 0x1.ebfbdff823cedp-3);
+  g = __builtin_fma(g, f, 0x1.62e42fefa39efp-1);
   return __builtin_amdgcn_ldexp(__builtin_fma(g, f, 1.0), (int)n);
 }
 
@@ -112,30 +112,59 @@ __device__ __forceinline__ float max_or_nan(float m) {
 // A given probability; what is none counts as 0.
 __device__ __forceinline__ double given(float p) { return p > 0.0f && p <= FLT_MAX ? (double)p : 0.0; }
 
-__device__ __forceinline__ float wave_max(float x) {
-  for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-  return x;
+// Reductions and running sums over a wave by data-parallel moves (no LDS):
+// rows of 16 by shifts within the row, then the rows' last lanes broadcast.
+template <int ctrl, int rows>
+__device__ __forceinline__ double dpp0(double x) {   // (0 from no lane)
+  const long long b = __double_as_longlong(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, ctrl, rows, 0xF, rows == 0xF);
+  const uint32_t hi =
+      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)((unsigned long long)b >> 32), ctrl, rows, 0xF, rows == 0xF);
+  return __longlong_as_double((long long)((unsigned long long)hi << 32 | lo));
 }
-__device__ __forceinline__ int wave_min(int x) {
-  for (int d = 32; d; d >>= 1) x = min(x, __shfl_xor(x, d));
-  return x;
-}
-__device__ __forceinline__ int wave_max(int x) {
-  for (int d = 32; d; d >>= 1) x = max(x, __shfl_xor(x, d));
-  return x;
-}
-__device__ __forceinline__ double wave_sum(double x) {
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  return x;
+__device__ __forceinline__ double lane_of(double x, int lane) {   // (lane uniform)
+  const long long b = __double_as_longlong(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((unsigned long long)b >> 32), lane);
+  return __longlong_as_double((long long)((unsigned long long)hi << 32 | lo));
 }
 // Inclusive running sum over the wave's lanes.
 __device__ __forceinline__ double wave_scan(double x) {
-  const int lane = threadIdx.x & 63;
-  for (int d = 1; d < 64; d <<= 1) {
-    const double y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+  x += dpp0<0x111, 0xF>(x);
+  x += dpp0<0x112, 0xF>(x);
+  x += dpp0<0x114, 0xF>(x);
+  x += dpp0<0x118, 0xF>(x);
+  x += dpp0<0x142, 0xA>(x);
+  x += dpp0<0x143, 0xC>(x);
   return x;
+}
+__device__ __forceinline__ double wave_sum(double x) { return lane_of(wave_scan(x), 63); }
+// The lane below's value (0 in lane 0).
+__device__ __forceinline__ double lane_below(double x) { return dpp0<0x138, 0xF>(x); }
+template <int ctrl, int rows>
+__device__ __forceinline__ int dpp_own(int x) {      // (its own from no lane)
+  return __builtin_amdgcn_update_dpp(x, x, ctrl, rows, 0xF, false);
+}
+template <typename F>
+__device__ __forceinline__ int wave_fold(int x, F f) {
+  x = f(x, dpp_own<0x111, 0xF>(x));
+  x = f(x, dpp_own<0x112, 0xF>(x));
+  x = f(x, dpp_own<0x114, 0xF>(x));
+  x = f(x, dpp_own<0x118, 0xF>(x));
+  x = f(x, dpp_own<0x142, 0xA>(x));
+  x = f(x, dpp_own<0x143, 0xC>(x));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return __int_as_float(wave_fold(__float_as_int(x), [](int a, int b) {
+    return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
+  }));
+}
+__device__ __forceinline__ int wave_min(int x) {
+  return wave_fold(x, [](int a, int b) { return min(a, b); });
+}
+__device__ __forceinline__ int wave_max(int x) {
+  return wave_fold(x, [](int a, int b) { return max(a, b); });
 }
 
 // A sequence's drafts: first index and count, kept inside the arrays whatever
@@ -192,6 +221,7 @@ __device__ __forceinline__ int first_rejected(bool ok, int n) {
 // Tests a draft whose probabilities are p and q.
 __device__ __forceinline__ Verdict judge(double p, double q, double u) {
   Verdict v;
+  v.p = p;
   v.ok = u * q < p;
   v.ratio = p >= q ? (p > 0.0 ? 1.0f : 0.0f) : (float)(p / q);
   return v;
@@ -266,16 +296,35 @@ __device__ __forceinline__ double prob(const Row &r, float v, int id) {
   if (r.greedy) return id == r.arg ? 1.0 : 0.0;
   return weight(v, r.m, r.c) * r.inv;
 }
-__device__ __forceinline__ double prob_at(const Row &r, int id, int vocab) {
-  return id >= 0 && id < vocab ? prob(r, r.p[id], id) : 0.0;
-}
 
+// A draft's test, with what does not wait for its rows' sums: its id, its
+// uniform and the rows' values at its id.
+struct Test {
+  int x;
+  double u;
+  float v[2];
+};
+__device__ __forceinline__ Test test_of(const VerifyArgs &a, int b, const Range &r, int i) {
+  Test t;
+  t.x = a.d.drafts[r.start + i];
+  t.u = a.d.uniforms[r.start + b + i];
+  t.v[0] = t.v[1] = __builtin_nanf("");
+  if (t.x >= 0 && t.x < a.vocab) {
+    t.v[0] = a.rows[0][(r.start + b + i) * a.stride[0] + t.x];
+    if (a.kind[1] != kDistNone) t.v[1] = a.rows[1][(r.start + i) * a.stride[1] + t.x];
+  }
+  return t;
+}
 __device__ __forceinline__ Verdict judge_at(const VerifyArgs &a, int b, const Range &r, int i,
-                                            const VerifyStat &st, const VerifyStat &sq) {
-  const int x = a.d.drafts[r.start + i];
-  const double p = prob_at(row_of(a, 0, b, r.start + b + i, st), x, a.vocab);
-  const double q = a.kind[1] == kDistNone ? 1.0 : prob_at(row_of(a, 1, b, r.start + i, sq), x, a.vocab);
-  return judge(p, q, a.d.uniforms[r.start + b + i]);
+                                            const Test &t, const VerifyStat &st,
+                                            const VerifyStat &sq) {
+  // (a NaN, as for an id outside the vocabulary, weighs 0, but an id of -1 is
+  // also the maximum's where there is none)
+  const bool in = t.x >= 0 && t.x < a.vocab;
+  const double p = in ? prob(row_of(a, 0, b, r.start + b + i, st), t.v[0], t.x) : 0.0;
+  const double q = a.kind[1] == kDistNone ? 1.0
+                   : in ? prob(row_of(a, 1, b, r.start + i, sq), t.v[1], t.x) : 0.0;
+  return judge(p, q, t.u);
 }
 
 // A row's summary from its parts', by one wave.
@@ -359,8 +408,7 @@ __device__ __forceinline__ Scan block_scan(double own, VerifySmem &sm) {
     if (i < wave) start += sm.sum[i];
     total += sm.sum[i];
   }
-  const double up = __shfl_up(incl, 1);
-  return {start + (lane ? up : 0.0), start + incl, total};
+  return {start + lane_below(incl), start + incl, total};
 }
 // The first thread with `hit`, else the last with `any`, else -1.
 __device__ __forceinline__ int block_first(bool hit, bool any, bool *past, VerifySmem &sm) {
@@ -451,39 +499,59 @@ __device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, doub
   return who < 0 ? -1 : sm.pick;
 }
 
-// The outcome of a sequence whose final row's masses are the parts' sums that
-// the rows' workgroups published (no draft rows to take off), by the workgroup
-// that left last.
+// The token of a sequence whose final row's masses are the sums that the rows'
+// workgroups published (no draft rows to take off), by a whole workgroup.  A
+// rejected certain draft's own probability px is taken off its part's sum;
+// where little of the sum is left, so that the difference would keep less
+// than 42 of its bits, the part is summed again without it.
 __device__ __forceinline__ int draw_from_parts(const VerifyArgs &a, Final f, int64_t row, double u,
-                                               VerifySmem &sm) {
+                                               double px, VerifySmem &sm) {
   const VerifyPart *part = a.part[0] + row * a.parts;
-  // a certain draft's own id is taken out of its part
-  const int xp = f.residual && f.x >= 0 && f.x < a.vocab ? f.x / kVerifyPart : -1;
+  auto sum_of = [&](int c) {
+    const VerifyPart p = load_part(part + c);
+    return p.s * weight(p.m, f.p.m, f.p.c) * f.p.inv;
+  };
+  int xp = f.residual && f.x >= 0 && f.x < a.vocab ? f.x / kVerifyPart : -1;
   for (;;) {
     double without = 0.0;
-    if (f.residual && xp >= 0) {   // (each wave for itself: the same sum)
-      without = part_mass(a, f, xp);
+    if (xp >= 0) {
+      const double all = sum_of(xp);
+      without = all - px;
+      if (!(without >= all * 0x1p-10)) without = part_mass(a, f, xp);   // (each wave the same)
     }
-    const bool out = f.residual && xp >= 0;
-    const int id = draw_id(a, f, u, [&](int c) {
-      if (out && c == xp) return without;
-      const VerifyPart p = load_part(part + c);
-      return p.s * weight(p.m, f.p.m, f.p.c) * f.p.inv;
-    }, sm);
+    const int id = draw_id(a, f, u, [&](int c) { return c == xp ? without : sum_of(c); }, sm);
     if (id >= 0 || !f.residual) return max(id, 0);
     f.residual = false;   // all of p is x: from p itself
+    xp = -1;
     __syncthreads();
   }
 }
 
-// One workgroup per kVerifyBlock logits of a row, a wave for each part: its
-// maximum and the sum of its weights.  The rows of every sequence's first
-// position come first in the grid, then the second's and so on; the workgroup
-// that completes a position judges its draft, and a workgroup of a position
-// behind a rejection found by then ends at once: nothing of its rows is asked
-// for.  (Whether it is found in time changes what is read, never the outcome.)
-// The workgroup that leaves a sequence last writes its outcome, unless a
-// rejection leaves p - q to be summed (verify_open_kernel).
+__device__ __forceinline__ void store_verdict(Verdict *p, const Verdict &v) {
+  store_agent(&p->p, v.p);
+  const unsigned long long w =
+      (unsigned long long)__float_as_uint(v.ratio) | ((unsigned long long)(uint32_t)v.ok << 32);
+  __hip_atomic_store(reinterpret_cast<unsigned long long *>(&p->ratio), w, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ Verdict load_verdict(const Verdict *p) {
+  Verdict v;
+  v.p = __longlong_as_double((long long)load_agent64(&p->p));
+  const unsigned long long w = load_agent64(&p->ratio);
+  v.ratio = __uint_as_float((uint32_t)w);
+  v.ok = (int32_t)(w >> 32);
+  return v;
+}
+
+// `split` workgroups a row of logits, a wave for each part: its maximum and the
+// sum of its weights.  The rows of every sequence's first position come first
+// in the grid, then the second's and so on; the workgroup that completes a
+// position judges its draft, and workgroups of positions behind a rejection
+// ask for nothing more of their rows once it is found.  (Whether it is found
+// in time changes what is read, never the outcome: a position behind a
+// rejection does not count, whatever is made of it.)  The workgroup that
+// completes a sequence's last position writes its outcome, unless a rejection
+// leaves p - q to be summed (verify_open_kernel).
 __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -492,8 +560,8 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyA
   const int side = both ? blockIdx.z & 1 : a.kind[0] != kDistLogits;
   const int b = blockIdx.y;
   const Range r = drafts_of(a.d, b);
-  // (rows of draft logits beside target probabilities: none at position n)
-  if (pos > r.n || (side == 1 && pos == r.n && (both || pos > 0))) return;
+  // (beside target probabilities there are no logits at position n)
+  if (pos > r.n || (side == 1 && pos == r.n && pos > 0) || (both && side == 1 && pos == r.n)) return;
   if (a.d.done && a.d.done[b]) {   // done before this call
     if (blockIdx.x == 0 && blockIdx.z == 0 && wave == 0) {
       emit(a.d, b, r, -1, -1, 0.0f, 0);
@@ -501,20 +569,31 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyA
     }
     return;
   }
-  const int slot = b * (a.d.max_drafts + 1) + pos;
-  // (read once for the whole workgroup: the waves must agree on it, and it may
-  // change between two reads)
-  if (tid == 0) sm.acc = (int)load_agent32(a.rejected + b);
-  __syncthreads();
-  const int rej = sm.acc;
+  const int slot0 = b * (a.d.max_drafts + 1), slot = slot0 + pos;
   const int64_t row = side ? r.start + pos : r.start + b + pos;
-  const bool there = !(side == 1 && pos == r.n);   // (a sequence without drafts still leaves)
-  if (there && !(rej && 64 - rej < pos)) {
+  Test test = {};
+  if (tid == 0 && pos < r.n) test = test_of(a, b, r, pos);
+  if (side == 0 || pos < r.n) {   // (a sequence without drafts has no draft row)
     const double T = a.temps[side] ? a.temps[side][b] : 1.0;
-    const int part = (int)blockIdx.x * kWavesV + wave;
-    if (part < a.parts) {
+    const double c = log2_scale(T);
+    const bool greedy = greedy_temp(T);
+    const float *rowp = a.rows[side] + row * a.stride[side];
+    // each wave looks for itself: there is no barrier in here.  (Where all
+    // workgroups start at once there is nothing to see at first.)
+    int rej = a.look && pos > 0 ? (int)load_agent32(a.rejected + b) : 0;
+    int part = (int)blockIdx.x * kWavesV + wave;
+    // (the next part is on its way while one is summed: all waves start
+    // together, and would otherwise all read, then all compute)
+    Float4 next[kVerifyPer / 4];
+    if (part < a.parts && (rej == 0 || 64 - rej >= pos)) load_part_of(rowp, part, 0, a.vocab, next);
+    for (; part < a.parts && (rej == 0 || 64 - rej >= pos); part += a.split * kWavesV) {
       Float4 v[kVerifyPer / 4];
-      load_part_of(a.rows[side] + row * a.stride[side], part, 0, a.vocab, v);
+#pragma unroll
+      for (int j = 0; j < kVerifyPer / 4; ++j) v[j] = next[j];
+      if (part + a.split * kWavesV < a.parts) {
+        rej = (int)load_agent32(a.rejected + b);
+        load_part_of(rowp, part + a.split * kWavesV, 0, a.vocab, next);
+      }
       float m = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < kVerifyPer; ++i) m = fmaxf(m, v[i / 4].v[i % 4]);
@@ -523,7 +602,7 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyA
       out.s = 0.0;
       out.arg = -1;
       const float mm = max_or_nan(out.m);
-      if (greedy_temp(T)) {
+      if (greedy) {
         int arg = 0x7FFFFFFF;
 #pragma unroll
         for (int i = 0; i < kVerifyPer; ++i)
@@ -534,67 +613,71 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyA
 #pragma unroll
           for (int i = 0; i < kVerifyPer; ++i) out.s += v[i / 4].v[i % 4] == mm ? 1.0 : 0.0;
         } else {
-          const double c = log2_scale(T);
+          // (two chains)
+          double s1 = 0.0;
 #pragma unroll
-          for (int i = 0; i < kVerifyPer; ++i) out.s += weight_below(v[i / 4].v[i % 4], mm, c);
+          for (int i = 0; i < kVerifyPer; i += 2) {
+            out.s += weight_below(v[i / 4].v[i % 4], mm, c);
+            s1 += weight_below(v[i / 4].v[i % 4 + 1], mm, c);
+          }
+          out.s += s1;
         }
         out.s = wave_sum(out.s);
       }
       if (lane == 0) store_part(a.part[side] + row * a.parts + part, out);
     }
-    const bool two = both && pos < r.n;
-    if (arrive(a.arrived + slot, (uint32_t)a.blocks * (two ? 2u : 1u), &sm.last)) {
-      // both rows of the position are done
-      if (wave < 2) {
-        const int64_t wr = wave ? r.start + pos : r.start + b + pos;
-        if (a.kind[wave] == kDistLogits && (wave == 0 || pos < r.n)) {
-          const VerifyStat st = combine(a.part[wave] + wr * a.parts, a.parts,
-                                        a.temps[wave] ? a.temps[wave][b] : 1.0);
-          if (lane == 0) {
-            sm.stat[wave] = st;
-            store_part(a.stat[wave] + wr, st);
-          }
-        }
-      }
-      __syncthreads();
-      if (tid == 0 && pos < r.n) {
-        const Verdict vd = judge_at(a, b, r, pos, sm.stat[0], sm.stat[1]);
-        const unsigned long long w =
-            (unsigned long long)__float_as_uint(vd.ratio) | ((unsigned long long)(uint32_t)vd.ok << 32);
-        __hip_atomic_store(reinterpret_cast<unsigned long long *>(a.verdict + slot), w,
-                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (!vd.ok) atomicMax(a.rejected + b, (uint32_t)(64 - pos));
+  }
+  const bool two = both && pos < r.n;
+  if (!arrive(a.arrived + slot, (uint32_t)a.split * (two ? 2u : 1u), &sm.last)) return;
+  // the position is done: its rows' summaries, its draft's test
+  if (wave < 2) {
+    const int64_t wr = wave ? r.start + pos : r.start + b + pos;
+    if (a.kind[wave] == kDistLogits && (wave == 0 || pos < r.n)) {
+      const VerifyStat st = combine(a.part[wave] + wr * a.parts, a.parts,
+                                    a.temps[wave] ? a.temps[wave][b] : 1.0);
+      if (lane == 0) {
+        sm.stat[wave] = st;
+        store_part(a.stat[wave] + wr, st);
       }
     }
   }
-  // out of the sequence
-  const int rows = both ? 2 * r.n + 1 : side ? max(r.n, 1) : r.n + 1;
-  if (!arrive(a.left + b, (uint32_t)(a.blocks * rows), &sm.last)) return;
-  float ratio = 0.0f;
-  if (wave == 0) {
-    unsigned long long w = 0;
-    if (lane < r.n) w = load_agent64(a.verdict + slot - pos + lane);
-    ratio = __uint_as_float((uint32_t)w);
-    const int acc = first_rejected((w >> 32) != 0, r.n);
-    if (lane == 0) sm.acc = acc;
+  __syncthreads();
+  if (tid == 0) {
+    store_agent(a.arrived + slot, 0u);   // for the next call
+    if (pos < r.n) {
+      const Verdict vd = judge_at(a, b, r, pos, test, sm.stat[0], sm.stat[1]);
+      store_verdict(a.verdict + slot, vd);
+      if (!vd.ok) atomicMax(a.rejected + b, (uint32_t)(64 - pos));
+    }
   }
-  // zero for the next call
-  for (int i = tid; i <= a.d.max_drafts; i += kVerifyThreads)
-    store_agent(a.arrived + (int64_t)b * (a.d.max_drafts + 1) + i, 0u);
+  const uint32_t positions = (uint32_t)(a.kind[0] == kDistLogits ? r.n + 1 : max(r.n, 1));
+  if (!arrive(a.left + b, positions, &sm.last)) return;
+  // the sequence is done
   if (tid == 0) {
     store_agent(a.rejected + b, 0u);
     store_agent(a.left + b, 0u);
   }
-  __syncthreads();
-  const int acc = sm.acc;
+  Verdict v = {};
+  VerifyStat st = {};
+  int x = -1;
+  if (lane < r.n) {
+    v = load_verdict(a.verdict + slot0 + lane);
+    x = a.d.drafts[r.start + lane];
+  }
+  if (lane <= r.n && a.kind[0] == kDistLogits) st = load_part(a.stat[0] + r.start + b + lane);
+  const double u = a.d.uniforms[r.start + b + r.n];
+  const int acc = first_rejected(v.ok != 0, r.n);   // (each wave the same)
   // p - q, or a row of probabilities, is still to be summed
   const bool open = a.kind[0] != kDistLogits || (acc < r.n && a.kind[1] != kDistNone);
   Final f;
   const int64_t fr = r.start + b + acc;
-  if (a.kind[0] == kDistLogits) f.p = row_of(a, 0, b, fr, load_part(a.stat[0] + fr));
+  st.s = __shfl(st.s, acc);
+  st.m = __shfl(st.m, acc);
+  st.arg = __shfl(st.arg, acc);
+  f.p = row_of(a, 0, b, fr, st);
   // greedy: its one id.  No candidate at all: 0, as the sampler's
   const bool known = a.kind[0] == kDistLogits && (f.p.greedy || !(f.p.inv > 0.0));
-  if (tid == 0 && a.open) a.open[b] = open && !known ? acc : -1;
+  if (tid == 0) a.open[b] = open && !known ? acc : -1;
   if (open && !known) return;
   int token;
   if (known) {
@@ -602,10 +685,10 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyA
   } else {
     f.residual = acc < r.n;
     f.pair = false;
-    f.x = f.residual ? a.d.drafts[r.start + acc] : -1;
-    token = draw_from_parts(a, f, fr, a.d.uniforms[r.start + b + r.n], sm);
+    f.x = __shfl(x, acc);   // (-1 behind the last draft)
+    token = draw_from_parts(a, f, fr, u, __shfl(v.p, acc), sm);
   }
-  if (wave == 0) emit(a.d, b, r, acc, token, ratio, 0);
+  if (wave == 0) emit(a.d, b, r, acc, token, v.ratio, 0);
 }
 
 // The sequences that a rejection left open, and every one where no side has
@@ -618,7 +701,7 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_open_kernel(VerifyAr
   const Range r = drafts_of(a.d, b);
   const bool judged = a.kind[0] == kDistLogits || a.kind[1] == kDistLogits;
   const int slot = b * (a.d.max_drafts + 1);
-  Verdict v = {0.0f, 0};
+  Verdict v = {};
   int acc;
   if (judged) {
     acc = a.open[b];
@@ -630,7 +713,7 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_open_kernel(VerifyAr
       return;
     }
     const VerifyStat none = {};
-    if (lane < r.n) v = judge_at(a, b, r, lane, none, none);
+    if (lane < r.n) v = judge_at(a, b, r, lane, test_of(a, b, r, lane), none, none);
     acc = first_rejected(v.ok != 0, r.n);   // (each wave the same)
   }
   const VerifyStat none = {};
@@ -750,7 +833,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_lists_kernel(ListArgs a
     }
   }
   __syncthreads();
-  Verdict v = {0.0f, 0};
+  Verdict v = {};
   bool bad = false;
   if (lane < r.n) {
     v = sm.verdict[lane];
@@ -835,8 +918,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_lists_kernel(ListArgs a
       total += sm.sum[w];
     }
     const double at = u * total;
-    const double up = __shfl_up(incl, 1);
-    double run = before + (lane ? up : 0.0);
+    double run = before + lane_below(incl);
     const double end = before + incl;
     int first = 0x7FFFFFFF, live = -1;
     for (int i = i0; i < i1; ++i) {
@@ -884,7 +966,7 @@ hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream, hipEvent_t *ev
   const unsigned launches = verify_launches(a);
   if (launches & 1u) {
     const bool both = a.kind[0] == kDistLogits && a.kind[1] == kDistLogits;
-    const dim3 grid((unsigned)a.blocks, (unsigned)a.d.seqs,
+    const dim3 grid((unsigned)a.split, (unsigned)a.d.seqs,
                     (unsigned)((a.d.max_drafts + 1) * (both ? 2 : 1)));
     const hipError_t e = launch_v(verify_stats_kernel, grid, 0, stream, ev_stats,
                                   launches & 2u ? nullptr : done, a);
