@@ -1285,7 +1285,6 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
     }
   const size_t verdict = take(judged * sizeof(hs::Verdict));
   const size_t mass = take((size_t)a.d.seqs * (size_t)a.parts * sizeof(double));
-  const size_t open = take((size_t)a.d.seqs * sizeof(int32_t));
   const size_t counts = judged + 2 * (size_t)a.d.seqs;
   HS_LOCK(ctx);
   DeviceGuard guard(ctx->device);
@@ -1317,13 +1316,12 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
   a.arrived = static_cast<uint32_t *>(ctx->verify_cnt.b.p);
   a.rejected = a.arrived + judged;
   a.left = a.rejected + a.d.seqs;
-  a.open = reinterpret_cast<int32_t *>(ws + open);
   hipEvent_t *ev1 = nullptr, *ev2 = nullptr;
   if (!cap) {
     const unsigned launches = hs::verify_launches(a);
-    if (launches == 3u) rc = timed_pair(ctx, hs::kStatsTimedSlot, hs::kResolveTimedSlot, &ev1, &ev2);
+    if (launches == 3u) rc = timed_pair(ctx, hs::kStatsTimedSlot, hs::kFinalTimedSlot, &ev1, &ev2);
     else if (launches == 1u) rc = timed_slot(ctx, hs::kStatsTimedSlot, &ev1);
-    else rc = timed_slot(ctx, hs::kResolveTimedSlot, &ev2);
+    else rc = timed_slot(ctx, hs::kFinalTimedSlot, &ev2);
     if (rc) return rc;
   }
   const hipError_t e = hs::launch_verify(a, stream, ev1, ev2, cap ? nullptr : ctx->done_ev);

@@ -409,7 +409,7 @@ constexpr int kVerifyPart = 64 * kVerifyPer;   // a wave's, the unit of the sums
 constexpr int kVerifyBlock = kVerifyThreads * kVerifyPer;
 constexpr int kVerifyMaxVocab = 1 << 28;
 constexpr int kVerifyMaxList = 4096;     // candidates of a list
-constexpr int kStatsTimedSlot = 12, kResolveTimedSlot = 13, kListsTimedSlot = 14;
+constexpr int kStatsTimedSlot = 12, kFinalTimedSlot = 13, kListsTimedSlot = 14;
 enum DistKind : int32_t { kDistNone = -1, kDistLogits = 0, kDistProbs = 1 };
 
 // One part of a row of logits: its largest logit, that logit's lowest id
@@ -456,22 +456,22 @@ struct VerifyArgs {
   int32_t kind[2];           // DistKind
   int32_t vocab, parts;      // parts of a row
   int32_t split;             // workgroups of a row: the rows' sums,
-  int32_t blocks;            //   and the rows that are left open
+  int32_t blocks;            //   and the rows a final token is drawn from
   int32_t look;              // more workgroups than start at once: the later ones
                              //   look for a rejection before they read
   VerifyPart *part[2];       // [rows][parts] of the sides that are logits
   VerifyStat *stat[2];       // [rows]
   Verdict *verdict;          // [seqs][max_drafts + 1]
   double *mass;              // [seqs][parts]
-  int32_t *open;             // [seqs] the rejected position, -1: the outcome is written
-  // zero between calls: workgroups done with a position, positions done of a
-  // sequence, the first rejection found so far (64 - position)
+  // zero between calls: workgroups done with a position, the first rejection
+  // found so far (64 - position), positions done of a sequence (or workgroups
+  // done with its final row)
   uint32_t *arrived;         // [seqs][max_drafts + 1]
   uint32_t *rejected;        // [seqs]
   uint32_t *left;            // [seqs]
 };
 // The kernels of a call: bit 0 the rows' sums (logits on a side), bit 1 the
-// rows that a rejection leaves open (draft rows, or probabilities alone).
+// outcomes where those do not settle them (draft rows, target probabilities).
 inline unsigned verify_launches(const VerifyArgs &a) {
   const bool sums = a.kind[0] == kDistLogits || a.kind[1] == kDistLogits;
   return (sums ? 1u : 0u) | (!sums || a.kind[0] != kDistLogits || a.kind[1] != kDistNone ? 2u : 0u);
@@ -489,7 +489,7 @@ inline void verify_split(VerifyArgs &a) {
   a.look = rows * a.split > 4 * kSplitCUs;
 }
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream, hipEvent_t *ev_stats,
-                         hipEvent_t *ev_resolve, hipEvent_t done);
+                         hipEvent_t *ev_final, hipEvent_t done);
 
 struct ListArgs {
   DraftArgs d;

@@ -70,23 +70,24 @@ __device__ __forceinline__ bool arrive(uint32_t *cnt, uint32_t of, int32_t *last
   return *last != 0;
 }
 
-// 2^d for d <= 0 (NaN: 0), to 4e-14.  n = round(d), 2^(d - n) by a polynomial 1 + f g(f),
-// g the Chebyshev interpolant of (2^f - 1) / f of degree 8 on [-1/2, 1/2].
-// Exact at whole d.  (Rounding, scaling and conversions take no longer than a
-// multiplication here.)
+// 2^d for d <= 0 (NaN: 0), to 2.2e-12.  n = round(d), 2^(d - n) by a polynomial
+// 1 + f g(f), g the Chebyshev interpolant of (2^f - 1) / f of degree 7 on
+// [-1/2, 1/2].  Exact at whole d.  (A step of a running sum over a vocabulary is
+// 1e-5 of the whole on average, and 64 draws in 10^7 fall within 2.2e-12 of
+// one of 151936; a degree less would make that one call in some hundred.
+// Rounding, scaling and conversions take no longer than a multiplication here.)
 __device__ __forceinline__ double exp2_neg(double d) {
   d = fmax(d, -1100.0);   // (below 2^-1074; a NaN takes the other operand)
   const double n = rint(d);
   const double f = d - n;
-  double g = 0x1.b63880a30e9ffp-24;
-  g = __builtin_fma(g, f, 0x1.63d136366db24p-20);
-  g = __builtin_fma(g, f, 0x1.ffcb9515a8016p-17);
-  g = __builtin_fma(g, f, 0x1.4308ac85aa947p-13);
-  g = __builtin_fma(g, f, 0x1.5d87fe86fe88ep-10);
-  g = __builtin_fma(g, f, 0x1.3b2ab7181b755p-7);
-  g = __builtin_fma(g, f, 0x1.c6b08d7047e52p-5);
-  g = __builtin_fma(g, f, 0x1.ebfbdff823cedp-3);
-  g = __builtin_fma(g, f, 0x1.62e42fefa39efp-1);
+  double g = 0x1.63b2d7971923fp-20;
+  g = __builtin_fma(g, f, 0x1.00c0e4e15189cp-16);
+  g = __builtin_fma(g, f, 0x1.4308c7183d6a2p-13);
+  g = __builtin_fma(g, f, 0x1.5d877598350dep-10);
+  g = __builtin_fma(g, f, 0x1.3b2ab70ad2565p-7);
+  g = __builtin_fma(g, f, 0x1.c6b08da70cce3p-5);
+  g = __builtin_fma(g, f, 0x1.ebfbdff82a734p-3);
+  g = __builtin_fma(g, f, 0x1.62e42fef9cc69p-1);
   return __builtin_amdgcn_ldexp(__builtin_fma(g, f, 1.0), (int)n);
 }
 
@@ -543,47 +544,94 @@ __device__ __forceinline__ Verdict load_verdict(const Verdict *p) {
   return v;
 }
 
+// A sequence's outcome as far as its rows of logits settle it: the first
+// rejected position (or n) and what the final token is drawn from.  Lanes hold
+// their position's verdict.
+struct Outcome {
+  int acc;
+  float ratio;
+  double px;                 // the rejected draft's probability
+  Final f;
+  bool known;                // one id has it all (greedy), or none has anything
+};
+__device__ __forceinline__ Outcome outcome_of(const VerifyArgs &a, int b, const Range &r) {
+  const int lane = threadIdx.x & 63;
+  Verdict v = {};
+  VerifyStat st = {}, sq = {};
+  int x = -1;
+  if (lane < r.n) {
+    v = load_verdict(a.verdict + b * (a.d.max_drafts + 1) + lane);
+    x = a.d.drafts[r.start + lane];
+    if (a.kind[1] == kDistLogits) sq = load_part(a.stat[1] + r.start + lane);
+  }
+  if (lane <= r.n && a.kind[0] == kDistLogits) st = load_part(a.stat[0] + r.start + b + lane);
+  auto at = [](const VerifyStat &s, int l) {
+    VerifyStat o;
+    o.s = lane_of(s.s, l);
+    o.m = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s.m), l));
+    o.arg = __builtin_amdgcn_readlane(s.arg, l);
+    return o;
+  };
+  Outcome o;
+  const int acc = __builtin_amdgcn_readfirstlane(first_rejected(v.ok != 0, r.n));
+  o.acc = acc;
+  o.ratio = v.ratio;
+  o.px = lane_of(v.p, acc);
+  o.f.p = row_of(a, 0, b, r.start + b + acc, at(st, acc));
+  o.f.residual = acc < r.n;
+  o.f.pair = o.f.residual && a.kind[1] != kDistNone;
+  o.f.x = __builtin_amdgcn_readlane(x, acc);   // (-1 behind the last draft)
+  if (o.f.pair) o.f.q = row_of(a, 1, b, r.start + acc, at(sq, acc));
+  o.known = a.kind[0] == kDistLogits && (o.f.p.greedy || !(o.f.p.inv > 0.0));
+  return o;
+}
+
 // `split` workgroups a row of logits, a wave for each part: its maximum and the
 // sum of its weights.  The rows of every sequence's first position come first
 // in the grid, then the second's and so on; the workgroup that completes a
 // position judges its draft, and workgroups of positions behind a rejection
 // ask for nothing more of their rows once it is found.  (Whether it is found
 // in time changes what is read, never the outcome: a position behind a
-// rejection does not count, whatever is made of it.)  The workgroup that
-// completes a sequence's last position writes its outcome, unless a rejection
-// leaves p - q to be summed (verify_open_kernel).
+// rejection does not count, whatever is made of it.)
+// ALONE: no draft rows.  The workgroup that completes a sequence's last
+// position then writes its outcome; otherwise verify_final_kernel does.
+template <bool ALONE>
 __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const bool both = a.kind[0] == kDistLogits && a.kind[1] == kDistLogits;
+  const bool both = !ALONE && a.kind[0] == kDistLogits && a.kind[1] == kDistLogits;
   const int pos = both ? blockIdx.z >> 1 : blockIdx.z;
-  const int side = both ? blockIdx.z & 1 : a.kind[0] != kDistLogits;
+  const int side = both ? blockIdx.z & 1 : ALONE ? 0 : a.kind[0] != kDistLogits;
   const int b = blockIdx.y;
+  int rej = 0;
+  if (a.look && pos > 0) {
+    // behind a rejection: nothing to do.  (Read once for the whole workgroup:
+    // its waves must agree, and it may change between two reads.  Where all
+    // workgroups start at once there is nothing to see yet.)
+    if (tid == 0) sm.acc = (int)load_agent32(a.rejected + b);
+    __syncthreads();
+    rej = sm.acc;
+    if (!ALONE && rej && 64 - rej < pos) return;
+  }
   const Range r = drafts_of(a.d, b);
-  // (beside target probabilities there are no logits at position n)
-  if (pos > r.n || (side == 1 && pos == r.n && pos > 0) || (both && side == 1 && pos == r.n)) return;
+  if (pos + (side || (!ALONE && a.kind[0] != kDistLogits)) > r.n) return;
   if (a.d.done && a.d.done[b]) {   // done before this call
-    if (blockIdx.x == 0 && blockIdx.z == 0 && wave == 0) {
-      emit(a.d, b, r, -1, -1, 0.0f, 0);
-      if (lane == 0) a.open[b] = -1;
-    }
+    if (ALONE && blockIdx.x == 0 && blockIdx.z == 0 && wave == 0) emit(a.d, b, r, -1, -1, 0.0f, 0);
     return;
   }
-  const int slot0 = b * (a.d.max_drafts + 1), slot = slot0 + pos;
+  const int slot = b * (a.d.max_drafts + 1) + pos;
   const int64_t row = side ? r.start + pos : r.start + b + pos;
   Test test = {};
   if (tid == 0 && pos < r.n) test = test_of(a, b, r, pos);
-  if (side == 0 || pos < r.n) {   // (a sequence without drafts has no draft row)
+  {
     const double T = a.temps[side] ? a.temps[side][b] : 1.0;
     const double c = log2_scale(T);
     const bool greedy = greedy_temp(T);
     const float *rowp = a.rows[side] + row * a.stride[side];
-    // each wave looks for itself: there is no barrier in here.  (Where all
-    // workgroups start at once there is nothing to see at first.)
-    int rej = a.look && pos > 0 ? (int)load_agent32(a.rejected + b) : 0;
     int part = (int)blockIdx.x * kWavesV + wave;
     // (the next part is on its way while one is summed: all waves start
-    // together, and would otherwise all read, then all compute)
+    // together, and would otherwise all read, then all compute; from here on
+    // each wave looks for a rejection for itself: there is no barrier in here)
     Float4 next[kVerifyPer / 4];
     if (part < a.parts && (rej == 0 || 64 - rej >= pos)) load_part_of(rowp, part, 0, a.vocab, next);
     for (; part < a.parts && (rej == 0 || 64 - rej >= pos); part += a.split * kWavesV) {
@@ -642,115 +690,96 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyA
     }
   }
   __syncthreads();
-  if (tid == 0) {
-    store_agent(a.arrived + slot, 0u);   // for the next call
-    if (pos < r.n) {
-      const Verdict vd = judge_at(a, b, r, pos, test, sm.stat[0], sm.stat[1]);
-      store_verdict(a.verdict + slot, vd);
-      if (!vd.ok) atomicMax(a.rejected + b, (uint32_t)(64 - pos));
-    }
+  if (tid == 0 && pos < r.n) {
+    const Verdict vd = judge_at(a, b, r, pos, test, sm.stat[0], sm.stat[1]);
+    store_verdict(a.verdict + slot, vd);
+    if (!vd.ok) atomicMax(a.rejected + b, (uint32_t)(64 - pos));
   }
-  const uint32_t positions = (uint32_t)(a.kind[0] == kDistLogits ? r.n + 1 : max(r.n, 1));
-  if (!arrive(a.left + b, positions, &sm.last)) return;
+  if (!ALONE) return;
+  if (tid == 0) store_agent(a.arrived + slot, 0u);   // for the next call
+  if (!arrive(a.left + b, (uint32_t)(r.n + 1), &sm.last)) return;
   // the sequence is done
   if (tid == 0) {
     store_agent(a.rejected + b, 0u);
     store_agent(a.left + b, 0u);
   }
-  Verdict v = {};
-  VerifyStat st = {};
-  int x = -1;
-  if (lane < r.n) {
-    v = load_verdict(a.verdict + slot0 + lane);
-    x = a.d.drafts[r.start + lane];
-  }
-  if (lane <= r.n && a.kind[0] == kDistLogits) st = load_part(a.stat[0] + r.start + b + lane);
   const double u = a.d.uniforms[r.start + b + r.n];
-  const int acc = first_rejected(v.ok != 0, r.n);   // (each wave the same)
-  // p - q, or a row of probabilities, is still to be summed
-  const bool open = a.kind[0] != kDistLogits || (acc < r.n && a.kind[1] != kDistNone);
-  Final f;
-  const int64_t fr = r.start + b + acc;
-  st.s = __shfl(st.s, acc);
-  st.m = __shfl(st.m, acc);
-  st.arg = __shfl(st.arg, acc);
-  f.p = row_of(a, 0, b, fr, st);
-  // greedy: its one id.  No candidate at all: 0, as the sampler's
-  const bool known = a.kind[0] == kDistLogits && (f.p.greedy || !(f.p.inv > 0.0));
-  if (tid == 0) a.open[b] = open && !known ? acc : -1;
-  if (open && !known) return;
-  int token;
-  if (known) {
-    token = max(f.p.arg, 0);
-  } else {
-    f.residual = acc < r.n;
-    f.pair = false;
-    f.x = __shfl(x, acc);   // (-1 behind the last draft)
-    token = draw_from_parts(a, f, fr, u, __shfl(v.p, acc), sm);
-  }
-  if (wave == 0) emit(a.d, b, r, acc, token, v.ratio, 0);
+  const Outcome o = outcome_of(a, b, r);
+  const int token = o.known ? max(o.f.p.arg, 0)
+                            : draw_from_parts(a, o.f, r.start + b + o.acc, u, o.px, sm);
+  if (wave == 0) emit(a.d, b, r, o.acc, token, o.ratio, 0);
 }
 
-// The sequences that a rejection left open, and every one where no side has
-// logits: one workgroup per kVerifyBlock ids of the final row sums what the
-// final token is drawn from, and the one that completes the row draws.
-__global__ __launch_bounds__(kVerifyThreads, 4) void verify_open_kernel(VerifyArgs a) {
+// The outcome of every sequence that has draft rows, or probabilities for its
+// target.  After a rejection one workgroup per kVerifyBlock ids of the final
+// row sums what the final token is drawn from, and the one that completes the
+// row draws; without one, and logits for the target, the sums are there.
+__global__ __launch_bounds__(kVerifyThreads, 4) void verify_final_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.y;
   const Range r = drafts_of(a.d, b);
-  const bool judged = a.kind[0] == kDistLogits || a.kind[1] == kDistLogits;
-  const int slot = b * (a.d.max_drafts + 1);
-  Verdict v = {};
-  int acc;
-  if (judged) {
-    acc = a.open[b];
-    if (acc < 0) return;
-    if (lane < r.n) v = a.verdict[slot + lane];
-  } else {
-    if (a.d.done && a.d.done[b]) {   // done before this call
-      if (blockIdx.x == 0 && wave == 0) emit(a.d, b, r, -1, -1, 0.0f, 0);
-      return;
-    }
-    const VerifyStat none = {};
-    if (lane < r.n) v = judge_at(a, b, r, lane, test_of(a, b, r, lane), none, none);
-    acc = first_rejected(v.ok != 0, r.n);   // (each wave the same)
-  }
-  const VerifyStat none = {};
-  const int64_t row = r.start + b + acc, drow = r.start + acc;
-  Final f;
-  f.p = row_of(a, 0, b, row, a.kind[0] == kDistLogits ? a.stat[0][row] : none);
-  f.residual = acc < r.n;
-  f.pair = f.residual && a.kind[1] != kDistNone;
-  f.x = f.residual ? a.d.drafts[drow] : -1;
-  if (f.pair) f.q = row_of(a, 1, b, drow, a.kind[1] == kDistLogits ? a.stat[1][drow] : none);
-  double *mass = a.mass + (int64_t)b * a.parts;
   const double u = a.d.uniforms[r.start + b + r.n];
-  // this workgroup's parts; then, where nothing is left beyond q (or x), all
-  // of p's by the workgroup that found it so
-  int p0 = (int)blockIdx.x * kWavesV, p1 = min(p0 + kWavesV, a.parts), token;
-  for (int again = 0;; ++again) {
-    for (int p = p0 + wave; p < p1; p += kWavesV) {
-      const double s = part_mass(a, f, p);
-      if (lane == 0) store_agent(mass + p, s);
+  const bool first = blockIdx.x == 0;
+  if (a.d.done && a.d.done[b]) {   // done before this call
+    if (first && wave == 0) emit(a.d, b, r, -1, -1, 0.0f, 0);
+    return;
+  }
+  Outcome o;
+  if (a.kind[0] == kDistLogits || a.kind[1] == kDistLogits) {
+    if (first) {   // zero for the next call
+      for (int i = tid; i <= a.d.max_drafts; i += kVerifyThreads)
+        a.arrived[(int64_t)b * (a.d.max_drafts + 1) + i] = 0u;
+      if (tid == 0) a.rejected[b] = 0u;
     }
-    if (!again) {
-      if (!arrive(a.left + b, (uint32_t)a.blocks, &sm.last)) return;
-    } else {
-      __builtin_amdgcn_s_waitcnt(0);
+    o = outcome_of(a, b, r);
+  } else {
+    const VerifyStat none = {};
+    Verdict v = {};
+    if (lane < r.n) v = judge_at(a, b, r, lane, test_of(a, b, r, lane), none, none);
+    o.acc = first_rejected(v.ok != 0, r.n);   // (each wave the same)
+    o.ratio = v.ratio;
+    o.px = 0.0;
+    o.known = false;
+    o.f.p = row_of(a, 0, b, r.start + b + o.acc, none);
+    o.f.residual = o.acc < r.n;
+    o.f.pair = o.f.residual && a.kind[1] != kDistNone;
+    o.f.x = o.f.residual ? a.d.drafts[r.start + o.acc] : -1;
+    if (o.f.pair) o.f.q = row_of(a, 1, b, r.start + o.acc, none);
+  }
+  Final &f = o.f;
+  int token;
+  if (o.known || (a.kind[0] == kDistLogits && !f.residual)) {
+    if (!first) return;
+    token = o.known ? max(f.p.arg, 0) : draw_from_parts(a, f, r.start + b + o.acc, u, 0.0, sm);
+  } else {
+    double *mass = a.mass + (int64_t)b * a.parts;
+    // this workgroup's parts; then, where nothing is left beyond q (or x), all
+    // of p's by the workgroup that found it so
+    int p0 = (int)blockIdx.x * kWavesV, p1 = min(p0 + kWavesV, a.parts);
+    for (int again = 0;; ++again) {
+      for (int p = p0 + wave; p < p1; p += kWavesV) {
+        const double s = part_mass(a, f, p);
+        if (lane == 0) store_agent(mass + p, s);
+      }
+      if (!again) {
+        if (!arrive(a.left + b, (uint32_t)a.blocks, &sm.last)) return;
+      } else {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+      }
+      token = draw_id(a, f, u, [&](int c) {
+        return __longlong_as_double((long long)load_agent64(mass + c));
+      }, sm);
+      if (token >= 0 || again) break;
+      f.residual = f.pair = false;
+      p0 = 0;
+      p1 = a.parts;
       __syncthreads();
     }
-    token = draw_id(a, f, u, [&](int c) {
-      return __longlong_as_double((long long)load_agent64(mass + c));
-    }, sm);
-    if (token >= 0 || again) break;
-    f.residual = f.pair = false;
-    p0 = 0;
-    p1 = a.parts;
-    __syncthreads();
+    if (tid == 0) store_agent(a.left + b, 0u);   // for the next call
   }
-  if (wave == 0) emit(a.d, b, r, acc, max(token, 0), v.ratio, 0);
-  if (tid == 0) store_agent(a.left + b, 0u);   // for the next call
+  if (wave == 0) emit(a.d, b, r, o.acc, max(token, 0), o.ratio, 0);
 }
 
 // ---- candidate lists
@@ -962,19 +991,20 @@ hipError_t launch_v(K kernel, dim3 grid, size_t lds, hipStream_t stream, hipEven
 }  // namespace
 
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream, hipEvent_t *ev_stats,
-                         hipEvent_t *ev_open, hipEvent_t done) {
+                         hipEvent_t *ev_final, hipEvent_t done) {
   const unsigned launches = verify_launches(a);
   if (launches & 1u) {
     const bool both = a.kind[0] == kDistLogits && a.kind[1] == kDistLogits;
     const dim3 grid((unsigned)a.split, (unsigned)a.d.seqs,
-                    (unsigned)((a.d.max_drafts + 1) * (both ? 2 : 1)));
-    const hipError_t e = launch_v(verify_stats_kernel, grid, 0, stream, ev_stats,
-                                  launches & 2u ? nullptr : done, a);
+                    (unsigned)(both ? 2 * a.d.max_drafts + 1 : a.d.max_drafts + 1));
+    const hipError_t e =
+        launches & 2u ? launch_v(verify_stats_kernel<false>, grid, 0, stream, ev_stats, nullptr, a)
+                      : launch_v(verify_stats_kernel<true>, grid, 0, stream, ev_stats, done, a);
     if (e != hipSuccess) return e;
   }
   if (launches & 2u)
-    return launch_v(verify_open_kernel, dim3((unsigned)a.blocks, (unsigned)a.d.seqs), 0, stream,
-                    ev_open, done, a);
+    return launch_v(verify_final_kernel, dim3((unsigned)a.blocks, (unsigned)a.d.seqs), 0, stream,
+                    ev_final, done, a);
   return hipSuccess;
 }
 

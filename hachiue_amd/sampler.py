@@ -329,7 +329,7 @@ class Sampler:
     KERNELS = ("pen_kernel", "row_kernel", "chunk_kernel", "finalize_kernel", "large_kernel",
                "mid_kernel", "argmax_kernel", "gemv_kernel", "large_fast_kernel",
                "large_replay_kernel", "large_replay_dev_kernel", "minp_kernel",
-               "verify_stats_kernel", "verify_open_kernel", "verify_lists_kernel",
+               "verify_stats_kernel", "verify_final_kernel", "verify_lists_kernel",
                "lora_shrink_kernel", "lora_expand_kernel")
 
     def kernel_times(self):

@@ -322,7 +322,7 @@ def test_streams_and_timing(sampler):
     hip.synchronize()
     sampler.set_timing(False)
     ms, calls = sampler.kernel_times()
-    assert calls == 6 and ms["verify_stats_kernel"] > 0 and ms["verify_open_kernel"] > 0
+    assert calls == 6 and ms["verify_stats_kernel"] > 0 and ms["verify_final_kernel"] > 0
     for b, t, d, _ in todo:
         b.check(expected(b, t, d))
     a.destroy()
