@@ -76,19 +76,27 @@ __device__ __forceinline__ bool arrive(uint32_t *cnt, uint32_t of, int32_t *last
 // 1e-5 of the whole on average, and 64 draws in 10^7 fall within 2.2e-12 of
 // one of 151936; a degree less would make that one call in some hundred.
 // Rounding, scaling and conversions take no longer than a multiplication here.)
-__device__ __forceinline__ double exp2_neg(double d) {
-  d = fmax(d, -1100.0);   // (below 2^-1074; a NaN takes the other operand)
-  const double n = rint(d);
-  const double f = d - n;
-  double g = 0x1.63b2d7971923fp-20;
-  g = __builtin_fma(g, f, 0x1.00c0e4e15189cp-16);
-  g = __builtin_fma(g, f, 0x1.4308c7183d6a2p-13);
-  g = __builtin_fma(g, f, 0x1.5d877598350dep-10);
-  g = __builtin_fma(g, f, 0x1.3b2ab70ad2565p-7);
-  g = __builtin_fma(g, f, 0x1.c6b08da70cce3p-5);
-  g = __builtin_fma(g, f, 0x1.ebfbdff82a734p-3);
-  g = __builtin_fma(g, f, 0x1.62e42fef9cc69p-1);
-  return __builtin_amdgcn_ldexp(__builtin_fma(g, f, 1.0), (int)n);
+// Four at a time, step by step: a multiplication's result is ready after some
+// three issue slots of a wave, and a wave alone on its SIMD would wait for each.
+template <int N>
+__device__ __forceinline__ void exp2_neg(double (&d)[N]) {
+  constexpr double coef[8] = {0x1.63b2d7971923fp-20, 0x1.00c0e4e15189cp-16, 0x1.4308c7183d6a2p-13, 0x1.5d877598350dep-10,
+                              0x1.3b2ab70ad2565p-7, 0x1.c6b08da70cce3p-5, 0x1.ebfbdff82a734p-3, 0x1.62e42fef9cc69p-1};
+  double n[N], g[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    d[i] = fmax(d[i], -1100.0);   // (below 2^-1074; a NaN takes the other operand)
+    n[i] = rint(d[i]);
+    d[i] -= n[i];
+    g[i] = coef[0];
+  }
+#pragma unroll
+  for (int k = 1; k < 8; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = __builtin_fma(g[i], d[i], coef[k]);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    d[i] = __builtin_amdgcn_ldexp(__builtin_fma(g[i], d[i], 1.0), (int)n[i]);
 }
 
 // log2(e) / T, at most 1e300 so that 0 times it stays 0.
@@ -97,15 +105,25 @@ __device__ __forceinline__ double log2_scale(double T) {
 }
 __device__ __forceinline__ bool greedy_temp(double T) { return !(T > 0.0); }
 
-// exp((l - m) / T) of a logit under a maximum m (NaN where the row has no
+// exp((l - m) / T) of logits under a maximum m (NaN where the row has no
 // candidate, which makes every weight 0).  The maximum weighs 1, also where it
 // is +infinity; a NaN or -infinity weighs 0.
-__device__ __forceinline__ double weight_below(float l, float m, double c) {   // (m finite or NaN)
-  return exp2_neg(((double)l - (double)m) * c);
+template <int N>
+__device__ __forceinline__ void weights_below(const float *l, float m, double c, double (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = ((double)l[i] - (double)m) * c;   // (m finite or NaN)
+  exp2_neg(w);
+}
+template <int N>
+__device__ __forceinline__ void weights(const float *l, float m, double c, double (&w)[N]) {
+  weights_below(l, m, c, w);
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = l[i] == m ? 1.0 : w[i];
 }
 __device__ __forceinline__ double weight(float l, float m, double c) {
-  const double e = weight_below(l, m, c);
-  return l == m ? 1.0 : e;
+  double w[1];
+  weights(&l, m, c, w);
+  return w[0];
 }
 __device__ __forceinline__ float max_or_nan(float m) {
   return m == -__builtin_inff() ? __builtin_nanf("") : m;
@@ -292,6 +310,20 @@ __device__ __forceinline__ Row row_of(const VerifyArgs &a, int side, int b, int6
   r.arg = st.arg;
   return r;
 }
+// Probabilities of four consecutive ids.
+__device__ __forceinline__ void probs4(const Row &r, const Float4 &v, int id, double (&p)[4]) {
+  if (r.kind == kDistProbs) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = given(v.v[i]);
+  } else if (r.greedy) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = id + i == r.arg ? 1.0 : 0.0;
+  } else {
+    weights(v.v, r.m, r.c, p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] *= r.inv;
+  }
+}
 __device__ __forceinline__ double prob(const Row &r, float v, int id) {
   if (r.kind == kDistProbs) return given(v);
   if (r.greedy) return id == r.arg ? 1.0 : 0.0;
@@ -370,25 +402,31 @@ struct Final {
   bool pair;                 // ... with draft rows
   int x;
 };
-__device__ __forceinline__ double final_weight(const Final &f, float vp, float vq, int id) {
-  const double p = prob(f.p, vp, id);
-  if (!f.residual) return p;
-  if (!f.pair) return id == f.x ? 0.0 : p;
-  return fmax(p - prob(f.q, vq, id), 0.0);
+__device__ __forceinline__ void final_weights(const Final &f, const Float4 &vp, const Float4 &vq,
+                                              int id, double (&w)[4]) {
+  probs4(f.p, vp, id, w);
+  if (f.pair) {
+    double q[4];
+    probs4(f.q, vq, id, q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = fmax(w[i] - q[i], 0.0);
+  } else if (f.residual) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = id + i == f.x ? 0.0 : w[i];
+  }
 }
 
 // The mass of a part, by one wave.
 __device__ __forceinline__ double part_mass(const VerifyArgs &a, const Final &f, int part) {
+  Float4 vp[kVerifyPer / 4], vq[kVerifyPer / 4];
+  load_part_of(f.p.p, part, 0, a.vocab, vp);
+  if (f.pair) load_part_of(f.q.p, part, 0, a.vocab, vq);
   double s = 0.0;
-#pragma unroll 1
-  for (int h = 0; h < kVerifyPer / 4; h += 4) {
-    Float4 vp[4], vq[4];
-    load_part_of(f.p.p, part, h, a.vocab, vp);
-    if (f.pair) load_part_of(f.q.p, part, h, a.vocab, vq);
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      s += final_weight(f, vp[i / 4].v[i % 4], f.pair ? vq[i / 4].v[i % 4] : 0.0f,
-                        part_id(part, h + i / 4) + i % 4);
+  for (int j = 0; j < kVerifyPer / 4; ++j) {
+    double w[4];
+    final_weights(f, vp[j], vq[j], part_id(part, j), w);
+    s += (w[0] + w[1]) + (w[2] + w[3]);
   }
   return wave_sum(s);
 }
@@ -474,12 +512,13 @@ __device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, doub
     vp[j] = load4(f.p.p, id0 + 4 * j, a.vocab);
     if (f.pair) vq[j] = load4(f.q.p, id0 + 4 * j, a.vocab);
   }
-  double w[8];
+  double w[2][4];
   own = 0.0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w[i] = final_weight(f, vp[i / 4].v[i % 4], f.pair ? vq[i / 4].v[i % 4] : 0.0f, id0 + i);
-    own += w[i];
+  for (int j = 0; j < 2; ++j) {
+    final_weights(f, vp[j], vq[j], id0 + 4 * j, w[j]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) own += w[j][i];
   }
   const Scan ids = block_scan(own, sm);
   who = block_first(own > 0.0 && ids.end > in, own > 0.0, &past, sm);
@@ -488,8 +527,8 @@ __device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, doub
     int first = -1, live = -1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      run += w[i];
-      if (w[i] > 0.0) {
+      run += w[i / 4][i % 4];
+      if (w[i / 4][i % 4] > 0.0) {
         live = id0 + i;
         if (first < 0 && run > in) first = live;
       }
@@ -596,7 +635,7 @@ __device__ __forceinline__ Outcome outcome_of(const VerifyArgs &a, int b, const 
 // ALONE: no draft rows.  The workgroup that completes a sequence's last
 // position then writes its outcome; otherwise verify_final_kernel does.
 template <bool ALONE>
-__global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool both = !ALONE && a.kind[0] == kDistLogits && a.kind[1] == kDistLogits;
@@ -661,14 +700,12 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyA
 #pragma unroll
           for (int i = 0; i < kVerifyPer; ++i) out.s += v[i / 4].v[i % 4] == mm ? 1.0 : 0.0;
         } else {
-          // (two chains)
-          double s1 = 0.0;
 #pragma unroll
-          for (int i = 0; i < kVerifyPer; i += 2) {
-            out.s += weight_below(v[i / 4].v[i % 4], mm, c);
-            s1 += weight_below(v[i / 4].v[i % 4 + 1], mm, c);
+          for (int j = 0; j < kVerifyPer / 4; ++j) {
+            double w[4];
+            weights_below(v[j].v, mm, c, w);
+            out.s += (w[0] + w[1]) + (w[2] + w[3]);
           }
-          out.s += s1;
         }
         out.s = wave_sum(out.s);
       }
@@ -714,7 +751,7 @@ __global__ __launch_bounds__(kVerifyThreads, 4) void verify_stats_kernel(VerifyA
 // target.  After a rejection one workgroup per kVerifyBlock ids of the final
 // row sums what the final token is drawn from, and the one that completes the
 // row draws; without one, and logits for the target, the sums are there.
-__global__ __launch_bounds__(kVerifyThreads, 4) void verify_final_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(kVerifyThreads, 3) void verify_final_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.y;
