@@ -32,22 +32,24 @@ __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(_Float16 v) { return (float)v; }
 __device__ __forceinline__ float widen(BF16 v) { return __uint_as_float((uint32_t)v.u << 16); }
 
-// n consecutive elements at any alignment of theirs.
+// n consecutive elements at any alignment of theirs, as they are stored.
 template <typename T, int n>
 struct __attribute__((packed, aligned(sizeof(T)))) Run {
   T v[n];
 };
-// Elements [0, left) of n, the others 0 and not read.
 template <int n, typename T>
-__device__ __forceinline__ void load_run(const T *p, int left, float (&out)[n]) {
-  if (left >= n) {
-    const Run<T, n> r = *reinterpret_cast<const Run<T, n> *>(p);
+__device__ __forceinline__ Run<T, n> load_run(const T *p) {
+  return *reinterpret_cast<const Run<T, n> *>(p);
+}
+// Elements [0, left) of n; the others are 0 and not read.
+template <int n, typename T>
+__device__ __forceinline__ Run<T, n> load_run(const T *p, int left) {
+  Run<T, n> r = {};
+  if (left >= n) return load_run<n>(p);
 #pragma unroll
-    for (int i = 0; i < n; ++i) out[i] = widen(r.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < n; ++i) out[i] = i < left ? widen(p[i]) : 0.0f;
-  }
+  for (int i = 0; i < n; ++i)
+    if (i < left) r.v[i] = p[i];
+  return r;
 }
 
 // The adapter of the tile's row `lane & 15`, -1: none.
@@ -57,48 +59,74 @@ __device__ __forceinline__ int slot_of(const LoraArgs &g, int m0) {
   return s >= 0 && s < g.count ? s : -1;
 }
 
-constexpr int kShrinkWaves = 8;
-
 // t = scale x A^T of one tile and one of its adapters (block x: the x-th
 // different one, in the order of the rows that name them).  K is cut over the
 // workgroup's waves; their sums meet in LDS.  JB blocks of 16 ranks a wave.
-// In a step of 32 k, lanes l, l + 16, ... hold 8 consecutive k each.
-template <typename T, int JB>
-__global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs g) {
-  __shared__ float sums[kShrinkWaves][JB][256];
+// In a step of 32 k, lanes l, l + 16, ... hold 8 consecutive k each; the next
+// step is on its way while one is multiplied.
+template <typename T, int JB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void lora_shrink_kernel(LoraArgs g) {
+  __shared__ float sums[WAVES][JB][256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int m0 = blockIdx.z * 16, j0 = blockIdx.y * (16 * JB);
   const int own = slot_of(g, m0);
   uint32_t todo = (uint32_t)__ballot(own >= 0) & 0xFFFFu;
   int s = -1;
   for (int i = 0; todo && i <= (int)blockIdx.x; ++i) {
-    s = __shfl(own, __ffs(todo) - 1);
+    s = __builtin_amdgcn_readlane(own, __ffs(todo) - 1);
     const uint32_t same = (uint32_t)__ballot(own == s) & 0xFFFFu;
     if (i < (int)blockIdx.x) s = -1;
     todo &= ~same;
   }
   if (s < 0) return;
   const int rank = g.ranks ? min(max(g.ranks[s], 0), g.rank) : g.rank;
-  f32x4 acc[JB];
-#pragma unroll
-  for (int j = 0; j < JB; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const float scale = g.scales ? g.scales[s] : 1.0f;
   const int i16 = lane & 15, grp = lane >> 4;
-  const float *x = g.x + (int64_t)min(m0 + i16, g.M - 1) * g.ldx;
-  const T *A = static_cast<const T *>(g.a) + (int64_t)s * g.rank * g.K;
+  const float *x = g.x + (int64_t)min(m0 + i16, g.M - 1) * g.ldx + grp * 8;
+  const T *A = static_cast<const T *>(g.a) + (int64_t)s * g.rank * g.K + grp * 8;
   const T *arow[JB];
 #pragma unroll
   for (int j = 0; j < JB; ++j) arow[j] = A + (int64_t)min(j0 + 16 * j + i16, g.rank - 1) * g.K;
-  for (int k0 = wave * 32; k0 < g.K; k0 += kShrinkWaves * 32) {
-    const int k = k0 + grp * 8, left = g.K - k;
-    float xv[8], av[JB][8];
-    load_run<8>(x + k, left, xv);
+  f32x4 acc[JB];
 #pragma unroll
-    for (int j = 0; j < JB; ++j) load_run<8>(arow[j] + k, left, av[j]);
+  for (int j = 0; j < JB; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto multiply = [&](const Run<float, 8> &xv, const Run<T, 8> (&av)[JB]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < JB; ++j)
-        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[i], av[j][i], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv.v[i], widen(av[j].v[i]), acc[j], 0, 0, 0);
+  };
+  const int whole = g.K / 32 * 32;
+  int k = wave * 32;
+  if (k < whole) {
+    Run<float, 8> xn = load_run<8>(x + k);
+    Run<T, 8> an[JB];
+#pragma unroll
+    for (int j = 0; j < JB; ++j) an[j] = load_run<8>(arow[j] + k);
+    for (;;) {
+      const Run<float, 8> xv = xn;
+      Run<T, 8> av[JB];
+#pragma unroll
+      for (int j = 0; j < JB; ++j) av[j] = an[j];
+      k += WAVES * 32;
+      const bool more = k < whole;
+      if (more) {
+        xn = load_run<8>(x + k);
+#pragma unroll
+        for (int j = 0; j < JB; ++j) an[j] = load_run<8>(arow[j] + k);
+      }
+      multiply(xv, av);
+      if (!more) break;
+    }
+  }
+  if (whole < g.K && whole / 32 % WAVES == wave) {   // the last, short step
+    const int left = g.K - whole - grp * 8;
+    const Run<float, 8> xv = load_run<8>(x + whole, left);
+    Run<T, 8> av[JB];
+#pragma unroll
+    for (int j = 0; j < JB; ++j) av[j] = load_run<8>(arow[j] + whole, left);
+    multiply(xv, av);
   }
   // acc: rows 4 grp + i of the tile, rank i16
 #pragma unroll
@@ -106,92 +134,140 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[wave][j][(4 * grp + i) * 16 + i16] = acc[j][i];
   __syncthreads();
-  const float scale = g.scales ? g.scales[s] : 1.0f;
-  for (int e = tid; e < JB * 256; e += kShrinkWaves * 64) {
+  for (int e = tid; e < JB * 256; e += WAVES * 64) {
     const int j = e >> 8, row = (e >> 4) & 15, jj = j0 + 16 * j + (e & 15);
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kShrinkWaves; ++w) v += sums[w][j][e & 255];
-    const int m = m0 + row;
-    const int ms = m < g.M ? g.slots[m] : -1;
+    for (int w = 0; w < WAVES; ++w) v += sums[w][j][e & 255];
     // (ranks that the adapter lacks: whatever its stack holds there, nothing)
-    if (ms == s && jj < g.rank_pad) g.t[(int64_t)m * g.rank_pad + jj] = jj < rank ? v * scale : 0.0f;
+    if (__shfl(own, row) == s && jj < g.rank_pad)
+      g.t[(int64_t)(m0 + row) * g.rank_pad + jj] = jj < rank ? v * scale : 0.0f;
   }
 }
 
 constexpr int kExpandWaves = 4;
 
 // y of one tile of 16 rows and NT tiles of 16 results a wave: for each adapter
-// that the rows name, its B times the tile's t.  In a step of 16 ranks, lanes
-// l, l + 16, ... hold 4 consecutive ones each; the rows' t stay in registers.
-// RB: steps of 16 ranks.
+// that the rows name, its B times the tile's t.  In a step of 4 VK ranks, lanes
+// l, l + 16, ... hold VK consecutive ones each; the rows' t stay in registers,
+// and the next step's B (of the next adapter after an adapter's last) is on
+// its way while one is multiplied.  RB: blocks of 16 ranks.
 template <typename T, int RB, int NT>
 __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs g) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int VK = RB == 1 ? 4 : 8, STEPS = RB * 4 / VK;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i16 = lane & 15, grp = lane >> 4;
-  const int m0 = blockIdx.y * 16;
+  const int m0 = blockIdx.y * 16, m = m0 + i16;
   const int n0 = ((int)blockIdx.x * kExpandWaves + wave) * (16 * NT);
   if (n0 >= g.N) return;
   const int own = slot_of(g, m0);
   uint32_t todo = (uint32_t)__ballot(own >= 0) & 0xFFFFu;
-  const int m = m0 + i16;
+  const int64_t mr = min(m, g.M - 1);
+  float *y = g.y + mr * g.ldy + n0 + 4 * grp;
+  const float *base = g.base ? g.base + mr * g.ldb + n0 + 4 * grp : nullptr;
+  const bool whole = n0 + 16 * NT <= g.N;
+  Run<float, 4> old[NT] = {};
+  if (base && whole) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) old[n] = load_run<4>(base + 16 * n);
+  }
   f32x4 out[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) out[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (todo) {
-    f32x4 t[RB];
-    const float *tp = g.t + (int64_t)min(m, g.M - 1) * g.rank_pad + grp * 4;
+    float t[STEPS][VK];
+    const float *tp = g.t + mr * g.rank_pad + grp * VK;
 #pragma unroll
-    for (int r = 0; r < RB; ++r) t[r] = *reinterpret_cast<const f32x4 *>(tp + 16 * r);
-    while (todo) {
-      const int s = __shfl(own, __ffs(todo) - 1);
+    for (int r = 0; r < STEPS; ++r)
+#pragma unroll
+      for (int i = 0; i < VK; i += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(tp + r * 4 * VK + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[r][i + e] = v[e];
+      }
+    const T *B = static_cast<const T *>(g.b);
+    int64_t brow[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) brow[n] = (int64_t)min(n0 + 16 * n + i16, g.N - 1) * g.rank;
+    // A run of VK may pass its row's end, and is masked there, but not the
+    // stack's: rows whose runs could are read element by element.
+    const int64_t per = (int64_t)g.N * g.rank, end = per * g.count;
+    const int64_t reach = (int64_t)(min(n0 + 16 * NT, g.N) - 1) * g.rank + (g.rank - 1) / VK * VK + VK;
+    auto load = [&](int s, int r, Run<T, VK> (&v)[NT]) {
+      const int k = r * 4 * VK + grp * VK;
+      const T *Bs = B + s * per;
+      if (s * per + reach <= end) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) v[n] = load_run<VK>(Bs + brow[n] + (k < g.rank ? k : 0));
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) v[n] = load_run<VK>(Bs + brow[n] + k, g.rank - k);
+      }
+    };
+    auto take = [&](int &rank) {   // the next adapter of the tile, its ranks
+      const int s = __builtin_amdgcn_readlane(own, __ffs(todo) - 1);
       todo &= ~((uint32_t)__ballot(own == s) & 0xFFFFu);
-      const int rank = g.ranks ? min(max(g.ranks[s], 0), g.rank) : g.rank;
-      const T *B = static_cast<const T *>(g.b) + (int64_t)s * g.N * g.rank;
+      rank = g.ranks ? min(max(g.ranks[s], 0), g.rank) : g.rank;
+      return s;
+    };
+    int rank, s = take(rank);
+    Run<T, VK> next[NT];
+    load(s, 0, next);
+    for (;;) {
+      const bool more = todo != 0;
+      int rank2 = 0, s2 = s;
+      if (more) s2 = take(rank2);
       f32x4 acc[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        if (16 * r < rank) {
-          float bv[NT][4];
+      for (int r = 0; r < STEPS; ++r) {
+        Run<T, VK> b[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) b[n] = next[n];
+        if (r + 1 < STEPS) load(s, r + 1, next);
+        else if (more) load(s2, 0, next);
+        const int k = r * 4 * VK + grp * VK;
+        const bool full = (r + 1) * 4 * VK <= rank;
+#pragma unroll
+        for (int i = 0; i < VK; ++i)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const T *p = B + (int64_t)min(n0 + 16 * n + i16, g.N - 1) * g.rank + 16 * r + grp * 4;
-            load_run<4>(p, rank - 16 * r - grp * 4, bv[n]);
+            float w = widen(b[n].v[i]);
+            if (!full) w = k + i < rank ? w : 0.0f;   // (t is 0 there too; B may be anything)
+            acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, t[r][i], acc[n], 0, 0, 0);
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[n][i], t[r][i], acc[n], 0, 0, 0);
-        }
       }
       // acc: results 4 grp + i of a tile, row i16
 #pragma unroll
       for (int n = 0; n < NT; ++n)
         if (own == s) out[n] = acc[n];
+      if (!more) break;
+      s = s2;
+      rank = rank2;
     }
   }
-  if (m >= g.M) return;
-  float *y = g.y + (int64_t)m * g.ldy;
-  const float *base = g.base ? g.base + (int64_t)m * g.ldb : nullptr;
-  if (own < 0 && base == y) return;
+  if (m >= g.M || (own < 0 && base == y)) return;
+  if (whole) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int c = n0 + 16 * n + 4 * grp, left = g.N - c;
-    if (left <= 0) continue;
-    Run<float, 4> o;
-    if (left >= 4) {
-      if (base) o = *reinterpret_cast<const Run<float, 4> *>(base + c);
+    for (int n = 0; n < NT; ++n) {
+      Run<float, 4> o;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o.v[i] = base ? (own < 0 ? o.v[i] : o.v[i] + out[n][i]) : out[n][i];
-      *reinterpret_cast<Run<float, 4> *>(y + c) = o;
-    } else {
-      for (int i = 0; i < left; ++i)
-        y[c + i] = base ? (own < 0 ? base[c + i] : base[c + i] + out[n][i]) : out[n][i];
+      for (int i = 0; i < 4; ++i)
+        o.v[i] = own < 0 ? old[n].v[i] : base ? old[n].v[i] + out[n][i] : out[n][i];
+      *reinterpret_cast<Run<float, 4> *>(y + 16 * n) = o;
     }
+    return;
   }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n0 + 16 * n + 4 * grp + i >= g.N) continue;
+      const float b = base ? base[16 * n + i] : 0.0f;
+      y[16 * n + i] = own < 0 ? b : base ? b + out[n][i] : out[n][i];
+    }
 }
 
 template <typename K>
@@ -211,14 +287,15 @@ template <typename T>
 hipError_t shrink(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev) {
   const int blocks = g.rank_pad / 16;
   const unsigned tiles = (unsigned)((g.M + 15) / 16), kinds = (unsigned)std::min({16, g.M, g.count});
-  if (blocks == 1)
-    return launch_l(lora_shrink_kernel<T, 1>, dim3(kinds, 1, tiles), kShrinkWaves * 64, stream, ev,
-                    nullptr, g);
-  if (blocks == 2)
-    return launch_l(lora_shrink_kernel<T, 2>, dim3(kinds, 1, tiles), kShrinkWaves * 64, stream, ev,
-                    nullptr, g);
-  return launch_l(lora_shrink_kernel<T, 4>, dim3(kinds, (unsigned)((blocks + 3) / 4), tiles),
-                  kShrinkWaves * 64, stream, ev, nullptr, g);
+  // as many blocks of ranks a wave (each reads x once) as leave a workgroup
+  // for every compute unit
+  const int per = blocks >= 4 && tiles * (unsigned)(blocks / 4) >= (unsigned)kSplitCUs   ? 4
+                  : blocks >= 2 && tiles * (unsigned)(blocks / 2) >= (unsigned)kSplitCUs ? 2
+                                                                                         : 1;
+  const dim3 grid(kinds, (unsigned)(blocks / per), tiles);
+  if (per == 4) return launch_l(lora_shrink_kernel<T, 4, 8>, grid, 512, stream, ev, nullptr, g);
+  if (per == 2) return launch_l(lora_shrink_kernel<T, 2, 8>, grid, 512, stream, ev, nullptr, g);
+  return launch_l(lora_shrink_kernel<T, 1, 8>, grid, 512, stream, ev, nullptr, g);
 }
 
 template <typename T, int NT>
