@@ -52,6 +52,12 @@ __device__ __forceinline__ Run<T, n> load_run(const T *p, int left) {
   return r;
 }
 
+// The same in LDS, 16-byte aligned.
+template <typename T, int n>
+struct alignas(16) Lane {
+  T v[n];
+};
+
 // The adapter of the tile's row `lane & 15`, -1: none.
 __device__ __forceinline__ int slot_of(const LoraArgs &g, int m0) {
   const int m = m0 + (threadIdx.x & 15);
@@ -59,89 +65,136 @@ __device__ __forceinline__ int slot_of(const LoraArgs &g, int m0) {
   return s >= 0 && s < g.count ? s : -1;
 }
 
-// t = scale x A^T of one tile and one of its adapters (block x: the x-th
-// different one, in the order of the rows that name them).  K is cut over the
-// workgroup's waves; their sums meet in LDS.  JB blocks of 16 ranks a wave.
-// In a step of 32 k, lanes l, l + 16, ... hold 8 consecutive k each; the next
-// step is on its way while one is multiplied.
-template <typename T, int JB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void lora_shrink_kernel(LoraArgs g) {
-  __shared__ float sums[WAVES][JB][256];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int m0 = blockIdx.z * 16, j0 = blockIdx.y * (16 * JB);
+// The sum of the shares' t (1 to 4 of them, `share` floats apart): all reads on
+// their way together.
+__device__ __forceinline__ f32x4 t_of(const float *p, int64_t share, int splits) {
+  f32x4 v = *reinterpret_cast<const f32x4 *>(p);
+  if (splits > 1) {
+    const f32x4 a = *reinterpret_cast<const f32x4 *>(p + share);
+    const f32x4 b = *reinterpret_cast<const f32x4 *>(p + min(2, splits - 1) * share);
+    const f32x4 c = *reinterpret_cast<const f32x4 *>(p + (splits - 1) * share);
+    v += a;
+    if (splits > 2) v += b;
+    if (splits > 3) v += c;
+  }
+  return v;
+}
+
+constexpr int kShrinkWaves = 8;
+constexpr int kShrinkK = kShrinkWaves * 32;   // k of a stage
+
+// t = scale x A^T of one tile and the adapters that its rows name, in the order
+// of the rows (block z takes every gridDim.z-th of them).  A workgroup takes JB blocks of 16 ranks and one of `splits` shares of K, in
+// stages of 256 k through LDS: rows are read along k, a wave instruction 1 KB
+// of one row, because the matrix operand's own order (16 rows side by side in
+// the lanes) makes the cache look up a line per lane: 2048 rows x 4096 with
+// rank 64 took 33 us that way.  The next stage is on its way while one is
+// multiplied, each wave 32 of its k, lanes l, l + 16, ... 8 consecutive ones
+// each; the waves' sums meet in LDS.
+template <typename T, int JB>
+__global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs g) {
+  // (rows 16 bytes longer than a stage: the operands' reads meet no bank twice)
+  constexpr int XS = kShrinkK + 4, AS = kShrinkK + 16 / (int)sizeof(T);
+  constexpr int PER = 16 / (int)sizeof(T);        // elements of a 16-byte read
+  constexpr int RPI = 64 * PER / kShrinkK;        // rows of A an instruction
+  constexpr int AI = 16 * JB / RPI / kShrinkWaves > 0 ? 16 * JB / RPI / kShrinkWaves : 1;
+  union alignas(16) Lds {
+    struct {
+      float x[16][XS];
+      T a[16 * JB][AS];
+    } in;
+    float sums[kShrinkWaves][JB][256];
+  };
+  __shared__ Lds lds;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = g.rank_pad / (16 * JB);
+  const int m0 = blockIdx.x * 16, j0 = (int)blockIdx.y % groups * (16 * JB);
+  const int split = (int)blockIdx.y / groups;
   const int own = slot_of(g, m0);
   uint32_t todo = (uint32_t)__ballot(own >= 0) & 0xFFFFu;
-  int s = -1;
-  for (int i = 0; todo && i <= (int)blockIdx.x; ++i) {
-    s = __builtin_amdgcn_readlane(own, __ffs(todo) - 1);
-    const uint32_t same = (uint32_t)__ballot(own == s) & 0xFFFFu;
-    if (i < (int)blockIdx.x) s = -1;
-    todo &= ~same;
-  }
-  if (s < 0) return;
-  const int rank = g.ranks ? min(max(g.ranks[s], 0), g.rank) : g.rank;
-  const float scale = g.scales ? g.scales[s] : 1.0f;
   const int i16 = lane & 15, grp = lane >> 4;
-  const float *x = g.x + (int64_t)min(m0 + i16, g.M - 1) * g.ldx + grp * 8;
-  const T *A = static_cast<const T *>(g.a) + (int64_t)s * g.rank * g.K + grp * 8;
-  const T *arow[JB];
+  // this share's stages
+  const int stages = (g.K + kShrinkK - 1) / kShrinkK, per = (stages + g.splits - 1) / g.splits;
+  const int k0 = split * per * kShrinkK, k1 = min(k0 + per * kShrinkK, g.K);
+  float *t = g.t + (int64_t)split * g.M * g.rank_pad;
+  for (int turn = 0; todo; ++turn) {
+    const int s = __builtin_amdgcn_readlane(own, __ffs(todo) - 1);
+    todo &= ~((uint32_t)__ballot(own == s) & 0xFFFFu);
+    if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
+    const int rank = g.ranks ? min(max(g.ranks[s], 0), g.rank) : g.rank;
+    const float scale = g.scales ? g.scales[s] : 1.0f;
+    int k = k0;
+    // what this thread reads of a stage: two rows of x, AI times PER elements of A
+    const int xk = lane * 4, ak = lane * PER % kShrinkK, ar = lane * PER / kShrinkK;
+    const float *xrow[2];
 #pragma unroll
-  for (int j = 0; j < JB; ++j) arow[j] = A + (int64_t)min(j0 + 16 * j + i16, g.rank - 1) * g.K;
-  f32x4 acc[JB];
+    for (int h = 0; h < 2; ++h)
+      xrow[h] = g.x + (int64_t)min(m0 + 2 * wave + h, g.M - 1) * g.ldx + xk;
+    const T *arow[AI];
+    int ai[AI];
 #pragma unroll
-  for (int j = 0; j < JB; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  auto multiply = [&](const Run<float, 8> &xv, const Run<T, 8> (&av)[JB]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < JB; ++j)
-        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv.v[i], widen(av[j].v[i]), acc[j], 0, 0, 0);
-  };
-  const int whole = g.K / 32 * 32;
-  int k = wave * 32;
-  if (k < whole) {
-    Run<float, 8> xn = load_run<8>(x + k);
-    Run<T, 8> an[JB];
-#pragma unroll
-    for (int j = 0; j < JB; ++j) an[j] = load_run<8>(arow[j] + k);
-    for (;;) {
-      const Run<float, 8> xv = xn;
-      Run<T, 8> av[JB];
-#pragma unroll
-      for (int j = 0; j < JB; ++j) av[j] = an[j];
-      k += WAVES * 32;
-      const bool more = k < whole;
-      if (more) {
-        xn = load_run<8>(x + k);
-#pragma unroll
-        for (int j = 0; j < JB; ++j) an[j] = load_run<8>(arow[j] + k);
-      }
-      multiply(xv, av);
-      if (!more) break;
+    for (int h = 0; h < AI; ++h) {
+      ai[h] = (wave + h * kShrinkWaves) * RPI + ar;
+      arow[h] = static_cast<const T *>(g.a) +
+                ((int64_t)s * g.rank + min(j0 + ai[h], g.rank - 1)) * g.K + ak;
     }
-  }
-  if (whole < g.K && whole / 32 % WAVES == wave) {   // the last, short step
-    const int left = g.K - whole - grp * 8;
-    const Run<float, 8> xv = load_run<8>(x + whole, left);
-    Run<T, 8> av[JB];
+    Run<float, 4> xn[2];
+    Run<T, PER> an[AI];
+    auto read = [&](int k) {
+      const bool whole = k + kShrinkK <= g.K;
 #pragma unroll
-    for (int j = 0; j < JB; ++j) av[j] = load_run<8>(arow[j] + whole, left);
-    multiply(xv, av);
-  }
-  // acc: rows 4 grp + i of the tile, rank i16
+      for (int h = 0; h < 2; ++h)
+        xn[h] = whole ? load_run<4>(xrow[h] + k) : load_run<4>(xrow[h] + k, g.K - k - xk);
 #pragma unroll
-  for (int j = 0; j < JB; ++j)
+      for (int h = 0; h < AI; ++h)
+        if (ai[h] < 16 * JB)
+          an[h] = whole ? load_run<PER>(arow[h] + k) : load_run<PER>(arow[h] + k, g.K - k - ak);
+    };
+    f32x4 acc[JB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[wave][j][(4 * grp + i) * 16 + i16] = acc[j][i];
-  __syncthreads();
-  for (int e = tid; e < JB * 256; e += WAVES * 64) {
-    const int j = e >> 8, row = (e >> 4) & 15, jj = j0 + 16 * j + (e & 15);
-    float v = 0.0f;
+    for (int j = 0; j < JB; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // (one stage ahead: two took 37 us where this takes 28)
+    if (k < k1) read(k);
+    while (k < k1) {
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) v += sums[w][j][e & 255];
-    // (ranks that the adapter lacks: whatever its stack holds there, nothing)
-    if (__shfl(own, row) == s && jj < g.rank_pad)
-      g.t[(int64_t)(m0 + row) * g.rank_pad + jj] = jj < rank ? v * scale : 0.0f;
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<Lane<float, 4> *>(&lds.in.x[2 * wave + h][xk]) =
+            __builtin_bit_cast(Lane<float, 4>, xn[h]);
+#pragma unroll
+      for (int h = 0; h < AI; ++h)
+        if (ai[h] < 16 * JB)
+          *reinterpret_cast<Lane<T, PER> *>(&lds.in.a[ai[h]][ak]) =
+              __builtin_bit_cast(Lane<T, PER>, an[h]);
+      __syncthreads();
+      k += kShrinkK;
+      if (k < k1) read(k);
+      const int kk = wave * 32 + grp * 8;
+      const Lane<float, 8> xv = *reinterpret_cast<const Lane<float, 8> *>(&lds.in.x[i16][kk]);
+#pragma unroll
+      for (int j = 0; j < JB; ++j) {
+        const Lane<T, 8> av = *reinterpret_cast<const Lane<T, 8> *>(&lds.in.a[16 * j + i16][kk]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv.v[i], widen(av.v[i]), acc[j], 0, 0, 0);
+      }
+      __syncthreads();
+    }
+    // acc: rows 4 grp + i of the tile, rank i16
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lds.sums[wave][j][(4 * grp + i) * 16 + i16] = acc[j][i];
+    __syncthreads();
+    for (int e = tid; e < JB * 256; e += kShrinkWaves * 64) {
+      const int j = e >> 8, row = (e >> 4) & 15, jj = j0 + 16 * j + (e & 15);
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kShrinkWaves; ++w) v += lds.sums[w][j][e & 255];
+      // (ranks that the adapter lacks: whatever its stack holds there, nothing)
+      if (__shfl(own, row) == s) t[(int64_t)(m0 + row) * g.rank_pad + jj] = jj < rank ? v * scale : 0.0f;
+    }
+    if (todo) __syncthreads();   // (the sums are read; the next adapter's stage goes there)
   }
 }
 
@@ -162,7 +215,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs
   const int n0 = ((int)blockIdx.x * kExpandWaves + wave) * (16 * NT);
   if (n0 >= g.N) return;
   const int own = slot_of(g, m0);
-  uint32_t todo = (uint32_t)__ballot(own >= 0) & 0xFFFFu;
+  // what does not wait for the slots
   const int64_t mr = min(m, g.M - 1);
   float *y = g.y + mr * g.ldy + n0 + 4 * grp;
   const float *base = g.base ? g.base + mr * g.ldb + n0 + 4 * grp : nullptr;
@@ -172,20 +225,22 @@ __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs
 #pragma unroll
     for (int n = 0; n < NT; ++n) old[n] = load_run<4>(base + 16 * n);
   }
+  float t[STEPS][VK];
+#pragma unroll
+  for (int r = 0; r < STEPS; ++r)
+#pragma unroll
+    for (int i = 0; i < VK; i += 4) {
+      f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (g.count > 0)
+        v = t_of(g.t + mr * g.rank_pad + grp * VK + r * 4 * VK + i, (int64_t)g.M * g.rank_pad, g.splits);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[r][i + e] = v[e];
+    }
+  uint32_t todo = (uint32_t)__ballot(own >= 0) & 0xFFFFu;
   f32x4 out[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) out[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (todo) {
-    float t[STEPS][VK];
-    const float *tp = g.t + mr * g.rank_pad + grp * VK;
-#pragma unroll
-    for (int r = 0; r < STEPS; ++r)
-#pragma unroll
-      for (int i = 0; i < VK; i += 4) {
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(tp + r * 4 * VK + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t[r][i + e] = v[e];
-      }
     const T *B = static_cast<const T *>(g.b);
     int64_t brow[NT];
 #pragma unroll
@@ -270,6 +325,131 @@ __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs
     }
 }
 
+// The same for prompts, a workgroup a tile of 16 rows and 256 results: B goes
+// through LDS in chunks of 128 bytes of each of its rows, and the results back
+// through it, so that every read and write of memory runs along rows (the
+// operands' own order, a lane a row, costs the cache a look-up per lane, which
+// bounds the kernel above where few adapters' B is read over and over).  The
+// next chunk (of the next adapter after an adapter's last) is on its way while
+// one is multiplied.
+template <typename T>
+__global__ __launch_bounds__(256, 3) void lora_expand_wide_kernel(LoraArgs g) {
+  constexpr int CH = 128 / (int)sizeof(T), PER = 16 / (int)sizeof(T);   // a chunk's ranks, a read's
+  constexpr int BS = CH + PER, TS = CH + 4, OS = 256 + 4;               // LDS row strides (no bank twice)
+  union alignas(16) Lds {
+    struct {
+      T b[256][BS];
+      float t[16][TS];
+    } in;
+    float out[16][OS];
+  };
+  __shared__ Lds lds;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane & 15, grp = lane >> 4;
+  const int m0 = blockIdx.y * 16, n0 = blockIdx.x * 256;
+  const int own = slot_of(g, m0);
+  // this thread's results: rows 4 wave + j, four of them from column c on
+  const int c = n0 + lane * 4;
+  Run<float, 4> old[4] = {};
+  if (g.base) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      old[j] = load_run<4>(g.base + (int64_t)min(m0 + 4 * wave + j, g.M - 1) * g.ldb + c, g.N - c);
+  }
+  uint32_t todo = (uint32_t)__ballot(own >= 0) & 0xFFFFu;
+  int s = -1, rank = 0, at = 0;   // the chunk that is on its way: its adapter, first rank
+  // the next one: false where there is none
+  auto step = [&]() {
+    at += CH;
+    while (at >= rank) {          // (adapters of no rank give 0)
+      if (!todo) return false;
+      s = __builtin_amdgcn_readlane(own, __ffs(todo) - 1);
+      todo &= ~((uint32_t)__ballot(own == s) & 0xFFFFu);
+      rank = g.ranks ? min(max(g.ranks[s], 0), g.rank) : g.rank;
+      at = 0;
+    }
+    return true;
+  };
+  // a chunk: rows tid / 8 + 32 h, PER ranks from PER (tid % 8) on; t: row
+  // tid / (CH / 4), four ranks
+  const int br = tid >> 3, bk = (tid & 7) * PER;
+  const int tr = tid / (CH / 4), tk = tid % (CH / 4) * 4;
+  Run<T, PER> bn[8];
+  f32x4 tn;
+  auto read = [&]() {
+    const T *B = static_cast<const T *>(g.b) + (int64_t)s * g.N * g.rank + at + bk;
+    const int left = rank - at - bk;   // (ranks that the adapter lacks: 0)
+#pragma unroll
+    for (int h = 0; h < 8; ++h)
+      bn[h] = load_run<PER>(B + (int64_t)min(n0 + br + 32 * h, g.N - 1) * g.rank, left);
+    tn = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (tr < 16 && at + tk < g.rank_pad)
+      tn = t_of(g.t + (int64_t)min(m0 + tr, g.M - 1) * g.rank_pad + at + tk,
+                (int64_t)g.M * g.rank_pad, g.splits);
+  };
+  f32x4 out[4], acc[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) out[n] = acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  bool more = step();
+  if (more) read();
+  while (more) {
+    const int s1 = s, live = rank - at;
+#pragma unroll
+    for (int h = 0; h < 8; ++h)
+      *reinterpret_cast<Lane<T, PER> *>(&lds.in.b[br + 32 * h][bk]) =
+          __builtin_bit_cast(Lane<T, PER>, bn[h]);
+    if (tr < 16) *reinterpret_cast<f32x4 *>(&lds.in.t[tr][tk]) = tn;
+    __syncthreads();
+    more = step();
+    if (more) read();
+#pragma unroll
+    for (int k = 0; k < CH; k += 32) {
+      if (k >= live) break;
+      const Lane<float, 8> tv = *reinterpret_cast<const Lane<float, 8> *>(&lds.in.t[i16][k + grp * 8]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const Lane<T, 8> b =
+            *reinterpret_cast<const Lane<T, 8> *>(&lds.in.b[wave * 64 + 16 * n + i16][k + grp * 8]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(widen(b.v[i]), tv.v[i], acc[n], 0, 0, 0);
+      }
+    }
+    if (!more || s != s1) {   // the adapter's last chunk: results 4 grp + i, row i16
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if (own == s1) out[n] = acc[n];
+        acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+    *reinterpret_cast<f32x4 *>(&lds.out[i16][wave * 64 + 16 * n + 4 * grp]) = out[n];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = 4 * wave + j, m = m0 + row;
+    if (m >= g.M || c >= g.N) continue;
+    float *y = g.y + (int64_t)m * g.ldy + c;
+    const bool none = __builtin_amdgcn_readlane(own, row) < 0;
+    if (none && g.base == g.y) continue;
+    const f32x4 d = *reinterpret_cast<const f32x4 *>(&lds.out[row][lane * 4]);
+    Run<float, 4> o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.v[i] = none ? old[j].v[i] : g.base ? old[j].v[i] + d[i] : d[i];
+    if (c + 4 <= g.N) {
+      *reinterpret_cast<Run<float, 4> *>(y) = o;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < g.N) y[i] = o.v[i];
+    }
+  }
+}
+
 template <typename K>
 hipError_t launch_l(K kernel, dim3 grid, int threads, hipStream_t stream, hipEvent_t *ev,
                     hipEvent_t done, const LoraArgs &g) {
@@ -285,17 +465,18 @@ hipError_t launch_l(K kernel, dim3 grid, int threads, hipStream_t stream, hipEve
 
 template <typename T>
 hipError_t shrink(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev) {
-  const int blocks = g.rank_pad / 16;
-  const unsigned tiles = (unsigned)((g.M + 15) / 16), kinds = (unsigned)std::min({16, g.M, g.count});
-  // as many blocks of ranks a wave (each reads x once) as leave a workgroup
-  // for every compute unit
-  const int per = blocks >= 4 && tiles * (unsigned)(blocks / 4) >= (unsigned)kSplitCUs   ? 4
-                  : blocks >= 2 && tiles * (unsigned)(blocks / 2) >= (unsigned)kSplitCUs ? 2
-                                                                                         : 1;
-  const dim3 grid(kinds, (unsigned)(blocks / per), tiles);
-  if (per == 4) return launch_l(lora_shrink_kernel<T, 4, 8>, grid, 512, stream, ev, nullptr, g);
-  if (per == 2) return launch_l(lora_shrink_kernel<T, 2, 8>, grid, 512, stream, ev, nullptr, g);
-  return launch_l(lora_shrink_kernel<T, 1, 8>, grid, 512, stream, ev, nullptr, g);
+  const int blocks = g.rank_pad / 16, per = std::min(blocks, sizeof(T) == 4 ? 2 : 4);   // (48 KB of LDS)
+  // A tile's adapters side by side where there are few tiles, else in turn: a
+  // prompt's tiles have one or two, and workgroups that find nothing to do
+  // cost 10 us over 2048 rows with eight adapters.
+  const unsigned tiles = (unsigned)((g.M + 15) / 16), shares = (unsigned)(blocks / per * g.splits);
+  const unsigned kinds = (unsigned)std::min({16, g.M, g.count});
+  const dim3 grid(tiles, shares, std::min(kinds, std::max(1u, 2u * kSplitCUs / (tiles * shares))));
+  const int threads = kShrinkWaves * 64;
+  if (per == 1) return launch_l(lora_shrink_kernel<T, 1>, grid, threads, stream, ev, nullptr, g);
+  if constexpr (sizeof(T) == 2)
+    if (per == 4) return launch_l(lora_shrink_kernel<T, 4>, grid, threads, stream, ev, nullptr, g);
+  return launch_l(lora_shrink_kernel<T, 2>, grid, threads, stream, ev, nullptr, g);
 }
 
 template <typename T, int NT>
@@ -312,8 +493,19 @@ hipError_t expand_by_rank(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev,
   }
 }
 
+// Prompts: many rows an adapter, and ranks that fill a chunk.  us, a lane a row
+// and through LDS, N = 4096, 8 adapters: 2048 rows, rank 64 34, 26, rank 128 49, 37,
+// rank 32 21, 25; 256 rows, rank 64 7.5, 7.0; 64 rows of mixed adapters, rank 64 10,
+// 23 (a workgroup takes them one after the other).
+inline bool expand_wide(const LoraArgs &g) {
+  return g.rank_pad >= 64 && g.M >= 256 && g.M >= 32 * (int64_t)g.count;
+}
+
 template <typename T>
 hipError_t expand(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
+  if (expand_wide(g))
+    return launch_l(lora_expand_wide_kernel<T>, dim3((unsigned)((g.N + 255) / 256), (unsigned)((g.M + 15) / 16)),
+                    256, stream, ev, done, g);
   const int64_t tiles = (int64_t)((g.N + 15) / 16) * ((g.M + 15) / 16);
   return tiles >= 4096 ? expand_by_rank<T, 4>(g, stream, ev, done)
                        : expand_by_rank<T, 1>(g, stream, ev, done);

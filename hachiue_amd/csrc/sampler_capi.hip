@@ -185,7 +185,7 @@ constexpr size_t pin_align(size_t b) { return (b + 255) / 256 * 256; }
 // drafts over 262144 logits, and of 4096 rows with adapters of rank 64.
 constexpr size_t kVerifyWorkBytes = size_t(5) << 19;
 constexpr size_t kVerifyCountBytes = size_t(16) << 10;
-constexpr size_t kLoraWorkBytes = size_t(1) << 20;
+constexpr size_t kLoraWorkBytes = size_t(2) << 20;
 
 // Routing of rows to kernels, uploaded next to the plans.
 struct Routing {
@@ -1436,14 +1436,19 @@ int lora_args(const float *d_x, int32_t M, int64_t ldx, const hs_adapters *ad, c
   while (g.rank_pad < g.rank) g.rank_pad *= 2;
   g.count = ad->count;
   g.type = ad->type;
+  g.splits = hs::lora_splits(M, g.K, g.rank_pad);
   return HS_OK;
+}
+
+size_t lora_bytes(const hs::LoraArgs &g) {
+  return (size_t)g.splits * (size_t)g.M * (size_t)g.rank_pad * sizeof(float);
 }
 
 // (the context's lock is held)
 int lora_run(hs_context *ctx, hs::LoraArgs &g, hipStream_t stream) {
   DeviceGuard guard(ctx->device);
   const bool cap = is_capturing(stream);
-  int rc = kept_room(ctx->lora_t, (size_t)g.M * (size_t)g.rank_pad * sizeof(float), cap);
+  int rc = kept_room(ctx->lora_t, lora_bytes(g), cap);
   if (rc) return rc;
   g.t = static_cast<float *>(ctx->lora_t.b.p);
   if (!cap) rc = enter_stream(ctx, stream);
@@ -1492,7 +1497,7 @@ int gemv_lora(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const h
               float *d_y, int64_t ldy, hs::LoraArgs &g, bool skip, hipStream_t stream) {
   if (!skip) {
     DeviceGuard guard(ctx->device);
-    const int rc = kept_room(ctx->lora_t, (size_t)g.M * (size_t)g.rank_pad * sizeof(float),
+    const int rc = kept_room(ctx->lora_t, lora_bytes(g),
                              is_capturing(stream));
     if (rc) return rc;
   }

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace hs {
 
 // ---- row kernel: one 1024-thread workgroup streams a whole row: round 0 of
@@ -516,13 +518,22 @@ struct LoraArgs {
   const float *scales;       // [count] or null: 1
   const int32_t *ranks;      // [count] or null: rank
   const int32_t *slots;      // [M]; outside [0, count): no adapter
-  float *t;                  // [M][rank_pad] scale * x A^T
+  float *t;                  // [splits][M][rank_pad] scale * x A^T of each share of K
   const float *base;         // [M][ldb] or null: 0
   int64_t ldb;
   float *y;                  // [M][ldy]
   int64_t ldy;
   int32_t M, K, N, rank, rank_pad, count, type;
+  int32_t splits;
 };
+// Shares of K of the first product: stages of 256 k each while the tiles of 16
+// rows and 64 ranks alone do not give each compute unit a workgroup (a tile
+// with one adapter), 4 at most (the second product adds them up).
+inline int32_t lora_splits(int32_t M, int32_t K, int32_t rank_pad) {
+  const int64_t groups = (int64_t)((M + 15) / 16) * ((rank_pad + 63) / 64);
+  const int64_t want = kSplitCUs / groups, most = (K + 255) / 256;
+  return (int32_t)(std::max<int64_t>(1, std::min<int64_t>({want, most, 4})));
+}
 hipError_t launch_lora_shrink(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev);
 hipError_t launch_lora_expand(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev, hipEvent_t done);
 
