@@ -325,12 +325,12 @@ __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs
     }
 }
 
-// The same for prompts, a workgroup a tile of 16 rows and 256 results: B goes
-// through LDS in chunks of 128 bytes of each of its rows, and the results back
-// through it, so that every read and write of memory runs along rows (the
-// operands' own order, a lane a row, costs the cache a look-up per lane, which
-// bounds the kernel above where few adapters' B is read over and over).  The
-// next chunk (of the next adapter after an adapter's last) is on its way while
+// The same for longer ranks and many results, a workgroup a tile of 16 rows and
+// 256 results: B goes through LDS in chunks of 128 bytes of each of its rows, and
+// the results back through it, so that every read and write of memory runs along
+// rows (the operands' own order, a lane a row, costs the cache a look-up per lane,
+// which bounds the kernel above once a row of B is longer than a line).  The next
+// chunk (of the next adapter after an adapter's last) is on its way while
 // one is multiplied.
 template <typename T>
 __global__ __launch_bounds__(256, 3) void lora_expand_wide_kernel(LoraArgs g) {
@@ -493,12 +493,15 @@ hipError_t expand_by_rank(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev,
   }
 }
 
-// Prompts: many rows an adapter, and ranks that fill a chunk.  us, a lane a row
-// and through LDS, N = 4096, 8 adapters: 2048 rows, rank 64 34, 26, rank 128 49, 37,
-// rank 32 21, 25; 256 rows, rank 64 7.5, 7.0; 64 rows of mixed adapters, rank 64 10,
-// 23 (a workgroup takes them one after the other).
+// Through LDS where ranks fill a chunk and there are workgroups enough (each
+// takes its tile's adapters one after the other).  us, a lane a row and through
+// LDS:
+//   2048 x 4096, 8 adapters, rank 32 21, 25, rank 64 34, 26, rank 128 49, 37
+//   16 x 100000 (391 workgroups), 2 adapters, rank 64 15, 14, rank 128 25, 20; 16
+//   adapters 73, 69 and 147, 124; 64 x 32000 (500) 16 adapters, rank 83 135, 116
+//   32 x 32000 (250), 8 adapters, rank 64 24, 27; 16 x 8000 (32), 16 adapters 16, 45
 inline bool expand_wide(const LoraArgs &g) {
-  return g.rank_pad >= 64 && g.M >= 256 && g.M >= 32 * (int64_t)g.count;
+  return g.rank_pad >= 64 && (int64_t)((g.N + 255) / 256) * ((g.M + 15) / 16) >= 384;
 }
 
 template <typename T>

@@ -287,6 +287,14 @@ struct VerifySmem {
   double at;                 // the draw, within the part
 };
 
+// A sequence's temperatures, read once and first.
+struct Temps {
+  double t[2];
+};
+__device__ __forceinline__ Temps temps_of(const VerifyArgs &a, int b) {
+  return {{a.temps[0] ? a.temps[0][b] : 1.0, a.temps[1] ? a.temps[1][b] : 1.0}};
+}
+
 // One side's distribution at a position: what a row's elements are turned
 // into probabilities with.
 struct Row {
@@ -297,12 +305,12 @@ struct Row {
   double c, inv;             // log2(e) / T, 1 / sum of weights
   int arg;
 };
-__device__ __forceinline__ Row row_of(const VerifyArgs &a, int side, int b, int64_t row,
+__device__ __forceinline__ Row row_of(const VerifyArgs &a, int side, const Temps &temps, int64_t row,
                                       const VerifyStat &st) {
   Row r;
   r.p = a.rows[side] + row * a.stride[side];
   r.kind = a.kind[side];
-  const double T = a.temps[side] ? a.temps[side][b] : 1.0;
+  const double T = temps.t[side];
   r.greedy = r.kind == kDistLogits && greedy_temp(T);
   r.c = log2_scale(T);
   r.m = max_or_nan(st.m);
@@ -348,15 +356,15 @@ __device__ __forceinline__ Test test_of(const VerifyArgs &a, int b, const Range 
   }
   return t;
 }
-__device__ __forceinline__ Verdict judge_at(const VerifyArgs &a, int b, const Range &r, int i,
-                                            const Test &t, const VerifyStat &st,
+__device__ __forceinline__ Verdict judge_at(const VerifyArgs &a, int b, const Temps &temps,
+                                            const Range &r, int i, const Test &t, const VerifyStat &st,
                                             const VerifyStat &sq) {
   // (a NaN, as for an id outside the vocabulary, weighs 0, but an id of -1 is
   // also the maximum's where there is none)
   const bool in = t.x >= 0 && t.x < a.vocab;
-  const double p = in ? prob(row_of(a, 0, b, r.start + b + i, st), t.v[0], t.x) : 0.0;
+  const double p = in ? prob(row_of(a, 0, temps, r.start + b + i, st), t.v[0], t.x) : 0.0;
   const double q = a.kind[1] == kDistNone ? 1.0
-                   : in ? prob(row_of(a, 1, b, r.start + i, sq), t.v[1], t.x) : 0.0;
+                   : in ? prob(row_of(a, 1, temps, r.start + i, sq), t.v[1], t.x) : 0.0;
   return judge(p, q, t.u);
 }
 
@@ -593,7 +601,8 @@ struct Outcome {
   Final f;
   bool known;                // one id has it all (greedy), or none has anything
 };
-__device__ __forceinline__ Outcome outcome_of(const VerifyArgs &a, int b, const Range &r) {
+__device__ __forceinline__ Outcome outcome_of(const VerifyArgs &a, int b, const Temps &temps,
+                                              const Range &r) {
   const int lane = threadIdx.x & 63;
   Verdict v = {};
   VerifyStat st = {}, sq = {};
@@ -616,11 +625,11 @@ __device__ __forceinline__ Outcome outcome_of(const VerifyArgs &a, int b, const 
   o.acc = acc;
   o.ratio = v.ratio;
   o.px = lane_of(v.p, acc);
-  o.f.p = row_of(a, 0, b, r.start + b + acc, at(st, acc));
+  o.f.p = row_of(a, 0, temps, r.start + b + acc, at(st, acc));
   o.f.residual = acc < r.n;
   o.f.pair = o.f.residual && a.kind[1] != kDistNone;
   o.f.x = __builtin_amdgcn_readlane(x, acc);   // (-1 behind the last draft)
-  if (o.f.pair) o.f.q = row_of(a, 1, b, r.start + acc, at(sq, acc));
+  if (o.f.pair) o.f.q = row_of(a, 1, temps, r.start + acc, at(sq, acc));
   o.known = a.kind[0] == kDistLogits && (o.f.p.greedy || !(o.f.p.inv > 0.0));
   return o;
 }
@@ -642,6 +651,7 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
   const int pos = both ? blockIdx.z >> 1 : blockIdx.z;
   const int side = both ? blockIdx.z & 1 : ALONE ? 0 : a.kind[0] != kDistLogits;
   const int b = blockIdx.y;
+  const Temps temps = temps_of(a, b);
   int rej = 0;
   if (a.look && pos > 0) {
     // behind a rejection: nothing to do.  (Read once for the whole workgroup:
@@ -663,7 +673,7 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
   Test test = {};
   if (tid == 0 && pos < r.n) test = test_of(a, b, r, pos);
   {
-    const double T = a.temps[side] ? a.temps[side][b] : 1.0;
+    const double T = side ? temps.t[1] : temps.t[0];
     const double c = log2_scale(T);
     const bool greedy = greedy_temp(T);
     const float *rowp = a.rows[side] + row * a.stride[side];
@@ -719,7 +729,7 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
     const int64_t wr = wave ? r.start + pos : r.start + b + pos;
     if (a.kind[wave] == kDistLogits && (wave == 0 || pos < r.n)) {
       const VerifyStat st = combine(a.part[wave] + wr * a.parts, a.parts,
-                                    a.temps[wave] ? a.temps[wave][b] : 1.0);
+                                    wave ? temps.t[1] : temps.t[0]);
       if (lane == 0) {
         sm.stat[wave] = st;
         store_part(a.stat[wave] + wr, st);
@@ -728,7 +738,7 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
   }
   __syncthreads();
   if (tid == 0 && pos < r.n) {
-    const Verdict vd = judge_at(a, b, r, pos, test, sm.stat[0], sm.stat[1]);
+    const Verdict vd = judge_at(a, b, temps, r, pos, test, sm.stat[0], sm.stat[1]);
     store_verdict(a.verdict + slot, vd);
     if (!vd.ok) atomicMax(a.rejected + b, (uint32_t)(64 - pos));
   }
@@ -741,7 +751,7 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
     store_agent(a.left + b, 0u);
   }
   const double u = a.d.uniforms[r.start + b + r.n];
-  const Outcome o = outcome_of(a, b, r);
+  const Outcome o = outcome_of(a, b, temps, r);
   const int token = o.known ? max(o.f.p.arg, 0)
                             : draw_from_parts(a, o.f, r.start + b + o.acc, u, o.px, sm);
   if (wave == 0) emit(a.d, b, r, o.acc, token, o.ratio, 0);
@@ -756,6 +766,7 @@ __global__ __launch_bounds__(kVerifyThreads, 3) void verify_final_kernel(VerifyA
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.y;
   const Range r = drafts_of(a.d, b);
+  const Temps temps = temps_of(a, b);
   const double u = a.d.uniforms[r.start + b + r.n];
   const bool first = blockIdx.x == 0;
   if (a.d.done && a.d.done[b]) {   // done before this call
@@ -769,20 +780,20 @@ __global__ __launch_bounds__(kVerifyThreads, 3) void verify_final_kernel(VerifyA
         a.arrived[(int64_t)b * (a.d.max_drafts + 1) + i] = 0u;
       if (tid == 0) a.rejected[b] = 0u;
     }
-    o = outcome_of(a, b, r);
+    o = outcome_of(a, b, temps, r);
   } else {
     const VerifyStat none = {};
     Verdict v = {};
-    if (lane < r.n) v = judge_at(a, b, r, lane, test_of(a, b, r, lane), none, none);
+    if (lane < r.n) v = judge_at(a, b, temps, r, lane, test_of(a, b, r, lane), none, none);
     o.acc = first_rejected(v.ok != 0, r.n);   // (each wave the same)
     o.ratio = v.ratio;
     o.px = 0.0;
     o.known = false;
-    o.f.p = row_of(a, 0, b, r.start + b + o.acc, none);
+    o.f.p = row_of(a, 0, temps, r.start + b + o.acc, none);
     o.f.residual = o.acc < r.n;
     o.f.pair = o.f.residual && a.kind[1] != kDistNone;
     o.f.x = o.f.residual ? a.d.drafts[r.start + o.acc] : -1;
-    if (o.f.pair) o.f.q = row_of(a, 1, b, r.start + o.acc, none);
+    if (o.f.pair) o.f.q = row_of(a, 1, temps, r.start + o.acc, none);
   }
   Final &f = o.f;
   int token;
