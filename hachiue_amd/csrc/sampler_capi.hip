@@ -131,7 +131,11 @@ struct KeptBuf {
   hipError_t ensure(size_t need) {
     if (need <= b.bytes) return hipSuccess;
     DevBuf n;
-    left.reserve(left.size() + 1);   // (before anything is allocated)
+    try {
+      left.reserve(left.size() + 1);   // (before anything is allocated)
+    } catch (const std::bad_alloc &) {
+      return hipErrorOutOfMemory;
+    }
     const hipError_t e = n.ensure(need > 2 * b.bytes ? need : 2 * b.bytes);
     if (e != hipSuccess) return e;
     if (b.p) left.push_back(b.p);
@@ -1170,11 +1174,7 @@ int kept_room(KeptBuf &b, size_t need, bool cap) {
   if (cap)
     return fail(HS_ERR_UNSUPPORTED,
                 "a captured call of this size needs one outside of the capture first");
-  try {
-    HS_HIP(b.ensure(need));
-  } catch (const std::bad_alloc &) {
-    return fail(HS_ERR_OUT_OF_MEMORY, "host allocation failed");
-  }
+  HS_HIP(b.ensure(need));
   return HS_OK;
 }
 
@@ -1394,6 +1394,8 @@ int lora_args(const float *d_x, int32_t M, int64_t ldx, const hs_adapters *ad, c
                 ad->rows, ad->cols);
   if (ad->rank > hs::kLoraMaxRank)
     return fail(HS_ERR_UNSUPPORTED, "adapter rank %d above %d", ad->rank, hs::kLoraMaxRank);
+  if (ad->cols > (1 << 30) || ad->rows > (1 << 30))
+    return fail(HS_ERR_UNSUPPORTED, "adapters of %d x %d above 2^30", ad->rows, ad->cols);
   if (M < 0) return fail(HS_ERR_INVALID_ARGUMENT, "M must be >= 0 (got %d)", M);
   if (M > 65535) return fail(HS_ERR_UNSUPPORTED, "M %d above 65535", M);
   *skip = M == 0 || ad->rows == 0;

@@ -123,6 +123,57 @@ def test_ranks_slots_and_scales(sampler, kind, rank):
     check(plain, x[:5], [0, 1, 1, -1, 0], b, y)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rank,K,N", [(64, 300, 4100), (83, 17, 4353), (130, 256, 4096), (256, 64, 4097)])
+def test_many_results_of_long_ranks(sampler, kind, rank, K, N):
+    """The second product through LDS: chunks that an adapter's ranks fill, end
+    in or do not reach, columns that end in a workgroup's tile, prompts beside
+    rows without an adapter, and what is not finite."""
+    rng = np.random.default_rng(rank + N)
+    ranks = [rank, 0, rank // 2, 33, 1, rank - 1]
+    ad = Adapters(rng, kind, 6, rank, K, N, ranks=ranks)
+    M = 390
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    slots = np.concatenate([np.repeat([0, 5, -1, 2], [100, 37, 9, 64]), rng.integers(-1, 7, 180)]).astype(np.int32)
+    x[7, K // 2] = np.inf
+    for base, pad, skew in (("apart", 1, 1), ("in place", 0, 0), (None, 3, 2)):
+        y, b = run(sampler, ad, x, slots, base, pad, skew)
+        fine = np.arange(M) != 7
+        check(ad, x[fine], slots[fine], b[fine] if b is not None else None, y[fine])
+        assert not np.isfinite(y[7]).any()
+    # an adapter whose last row of B is not finite
+    bad = ad.b.copy()
+    bad[3, N - 1, 0] = np.nan
+    ad.arr[1].upload(stored(bad, kind)[0])
+    y, b = run(sampler, ad, x, slots)
+    rows = fine & (slots != 3)
+    check(ad, x[rows], slots[rows], b[rows], y[rows])
+    assert np.isnan(y[fine & (slots == 3)][:, N - 1]).all()
+
+
+def test_a_failed_allocation():
+    """The workspace cannot grow: the call says so, the next one works."""
+    import os
+    rng = np.random.default_rng(12)
+    ad = Adapters(rng, "bf16", 2, 200, 16, 8)
+    x = rng.standard_normal((5000, 16)).astype(np.float32)
+    old = os.environ.get("HS_INJECT_HIP_FAILURE")
+    os.environ["HS_INJECT_HIP_FAILURE"] = "0"
+    try:
+        ctx = Sampler(0)
+    finally:
+        if old is None:
+            del os.environ["HS_INJECT_HIP_FAILURE"]
+        else:
+            os.environ["HS_INJECT_HIP_FAILURE"] = old
+    with ctx:
+        with pytest.raises(SamplerError) as e:
+            run(ctx, ad, x, [1] * 5000)
+        assert e.value.status == 2
+        y, b = run(ctx, ad, x, [1] * 5000)
+        check(ad, x[-40:], [1] * 40, b[-40:], y[-40:])
+
+
 def test_no_adapters_at_all(sampler):
     rng = np.random.default_rng(1)
     ad = Adapters(rng, "bf16", 1, 4, 8, 100)

@@ -55,6 +55,16 @@ def test_full_vocabulary(sampler):
     run(sampler, [4, 3, 4, 2], 151936, 1, temps=temps, dtemps=np.maximum(temps, 0.5))
 
 
+@pytest.mark.parametrize("draft", ["logits", "probs", None])
+def test_more_rows_than_start_at_once(sampler, draft):
+    """Rows behind a rejection that was found in time are left out, rows in the
+    middle of it given up: over several calls, whatever was left out."""
+    temps = np.where(np.arange(64) % 9 == 4, 0.0, 0.9)
+    for seed in range(3):
+        run(sampler, [8] * 60 + [0, 3, 1, 5], 40007, seed, draft is not None, dkind=draft or "logits",
+            temps=temps, dtemps=np.maximum(temps, 0.5))
+
+
 def test_one_long_row(sampler):
     """More chunks than a wave has lanes."""
     run(sampler, [1, 0], 700001, 2)

@@ -168,6 +168,8 @@ def test_bad_adapters():
     for kw in (dict(count=-1), dict(rank=0), dict(K=0), dict(N=-1)):
         refused(call(ad(**kw)), "adapters of count")
     refused(call(ad(rank=257)), "rank 257", 4)
+    for kw in (dict(K=(1 << 30) + 1), dict(N=2 ** 31 - 1)):
+        refused(call(ad(**kw), ldx=1 << 31, ldy=1 << 31), "above 2^30", 4)
     refused(call(ad(), M=-1), "M must")
     refused(call(ad(), M=65536), "65535", 4)
     for kw in (dict(x=None), dict(slots=None), dict(y=None)):
