@@ -1266,9 +1266,7 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
     if (rc) return rc;
   }
   a.vocab = vocab;
-  a.parts = (vocab + hs::kVerifyPart - 1) / hs::kVerifyPart;
-  a.blocks = (vocab + hs::kVerifyBlock - 1) / hs::kVerifyBlock;
-  hs::verify_split(a);
+  hs::verify_cut(a);
   const size_t rows[2] = {(size_t)a.d.n_drafts + (size_t)a.d.seqs, (size_t)a.d.n_drafts};
   const size_t judged = (size_t)a.d.seqs * (size_t)(a.d.max_drafts + 1);
   size_t need = 0;
@@ -1284,7 +1282,7 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
       stat[i] = take(rows[i] * sizeof(hs::VerifyStat));
     }
   const size_t verdict = take(judged * sizeof(hs::Verdict));
-  const size_t mass = take((size_t)a.d.seqs * (size_t)a.parts * sizeof(double));
+  const size_t mass = take((size_t)a.d.seqs * (size_t)a.fparts * sizeof(double));
   const size_t counts = judged + 2 * (size_t)a.d.seqs;
   HS_LOCK(ctx);
   DeviceGuard guard(ctx->device);

@@ -406,9 +406,11 @@ int kq_sample_grid(const GemvArgs &g);
 // ---- verification of drafted tokens (verify_kernels.hip)
 constexpr int kVerifyMaxDrafts = 63;     // a sequence's tokens fit one wave
 constexpr int kVerifyThreads = 256;
-constexpr int kVerifyPer = 32;           // values of a row a thread holds
-constexpr int kVerifyPart = 64 * kVerifyPer;   // a wave's, the unit of the sums
-constexpr int kVerifyBlock = kVerifyThreads * kVerifyPer;
+// Values of a row a lane holds, 64 times which is a wave's part, the unit of the
+// sums: 32, or 16 where a call has few waves (fewer than kVerifyFew would be
+// busy), which then end sooner: 16 sequences' outcomes over 151936 logits 13.8 us
+// (15.4), but 32 sequences' 19 (14).
+constexpr int kVerifyPer = 32, kVerifyPerFew = 16, kVerifyFew = 2048;
 constexpr int kVerifyMaxVocab = 1 << 28;
 constexpr int kVerifyMaxList = 4096;     // candidates of a list
 constexpr int kStatsTimedSlot = 12, kFinalTimedSlot = 13, kListsTimedSlot = 14;
@@ -456,15 +458,16 @@ struct VerifyArgs {
   int64_t stride[2];
   const double *temps[2];    // [seqs] or null: 1
   int32_t kind[2];           // DistKind
-  int32_t vocab, parts;      // parts of a row
-  int32_t split;             // workgroups of a row: the rows' sums,
-  int32_t blocks;            //   and the rows a final token is drawn from
+  int32_t vocab;
+  int32_t per, parts;        // a lane's values and the parts of a row: the rows' sums,
+  int32_t fper, fparts;      //   and the rows a final token is drawn from
+  int32_t split, blocks;     // workgroups of a row in either
   int32_t look;              // more workgroups than start at once: the later ones
                              //   look for a rejection before they read
   VerifyPart *part[2];       // [rows][parts] of the sides that are logits
   VerifyStat *stat[2];       // [rows]
   Verdict *verdict;          // [seqs][max_drafts + 1]
-  double *mass;              // [seqs][parts]
+  double *mass;              // [seqs][fparts]
   // zero between calls: workgroups done with a position, the first rejection
   // found so far (64 - position), positions done of a sequence (or workgroups
   // done with its final row)
@@ -478,16 +481,25 @@ inline unsigned verify_launches(const VerifyArgs &a) {
   const bool sums = a.kind[0] == kDistLogits || a.kind[1] == kDistLogits;
   return (sums ? 1u : 0u) | (!sums || a.kind[0] != kDistLogits || a.kind[1] != kDistNone ? 2u : 0u);
 }
-// Workgroups of a row whose logits are summed: enough that all rows together
-// give each compute unit four, but each has up to kVerifyDeep blocks of
-// kVerifyBlock logits to itself.
+// How rows are cut.  Workgroups of a row whose logits are summed: enough that
+// all rows together give each compute unit four, but each has up to kVerifyDeep
+// turns of its four waves to itself (4: verify of 64 sequences 145 us; 2: 152).
 constexpr int kVerifyDeep = 4;
-inline void verify_split(VerifyArgs &a) {
+inline void verify_cut(VerifyArgs &a) {
+  auto parts = [&](int per) { return (a.vocab + 64 * per - 1) / (64 * per); };
+  auto cut = [&](int64_t rows, int32_t &per, int32_t &n) {
+    per = rows * parts(kVerifyPer) < kVerifyFew ? kVerifyPerFew : kVerifyPer;
+    n = parts(per);
+  };
   const int64_t rows = (a.kind[0] == kDistLogits ? a.d.n_drafts + a.d.seqs : 0) +
                        (a.kind[1] == kDistLogits ? a.d.n_drafts : 0);
+  cut(rows, a.per, a.parts);
+  cut(a.d.seqs, a.fper, a.fparts);
+  const int waves = kVerifyThreads / 64;
+  a.blocks = (a.fparts + waves - 1) / waves;
+  const int64_t blocks = (a.parts + waves - 1) / waves;
   const int64_t want = rows > 0 ? 4 * kSplitCUs / rows : 1;
-  const int64_t least = (a.blocks + kVerifyDeep - 1) / kVerifyDeep;
-  a.split = (int32_t)(want < least ? least : want > a.blocks ? a.blocks : want);
+  a.split = (int32_t)std::max((blocks + kVerifyDeep - 1) / kVerifyDeep, std::min(want, blocks));
   a.look = rows * a.split > 4 * kSplitCUs;
 }
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream, hipEvent_t *ev_stats,

@@ -263,18 +263,20 @@ __device__ __forceinline__ Float4 load4(const float *row, int i, int vocab) {
 }
 // A wave's part of a row: float4 j of lane l is ids 256 j + 4 l of the part.
 // (One test per part, so that its loads are all on their way together.)
+template <int PER>
 __device__ __forceinline__ int part_id(int part, int j) {
-  return part * kVerifyPart + j * 256 + (int)(threadIdx.x & 63) * 4;
+  return part * (64 * PER) + j * 256 + (int)(threadIdx.x & 63) * 4;
 }
-template <int n>
-__device__ __forceinline__ void load_part_of(const float *row, int part, int j0, int vocab,
-                                             Float4 (&v)[n]) {
-  if ((part + 1) * kVerifyPart <= vocab) {
+template <int PER>
+__device__ __forceinline__ void load_part_of(const float *row, int part, int vocab,
+                                             Float4 (&v)[PER / 4]) {
+  if ((part + 1) * (64 * PER) <= vocab) {
 #pragma unroll
-    for (int j = 0; j < n; ++j) v[j] = *reinterpret_cast<const Float4 *>(row + part_id(part, j0 + j));
+    for (int j = 0; j < PER / 4; ++j)
+      v[j] = *reinterpret_cast<const Float4 *>(row + part_id<PER>(part, j));
   } else {
 #pragma unroll
-    for (int j = 0; j < n; ++j) v[j] = load4(row, part_id(part, j0 + j), vocab);
+    for (int j = 0; j < PER / 4; ++j) v[j] = load4(row, part_id<PER>(part, j), vocab);
   }
 }
 
@@ -374,15 +376,15 @@ __device__ __forceinline__ VerifyStat combine(const VerifyPart *part, int parts,
   const double c = log2_scale(T);
   const bool greedy = greedy_temp(T);
   VerifyStat r;
-  // (most rows have at most two parts a lane: those stay in registers)
-  VerifyPart own[2];
+  // (most rows have at most three parts a lane: those stay in registers)
+  VerifyPart own[3];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 3; ++i) {
     own[i] = {0.0, -__builtin_inff(), 0x7FFFFFFF};
     if (lane + 64 * i < parts) own[i] = load_part(part + lane + 64 * i);
   }
-  float m = fmaxf(own[0].m, own[1].m);
-  for (int i = lane + 128; i < parts; i += 64) m = fmaxf(m, load_part(part + i).m);
+  float m = fmaxf(fmaxf(own[0].m, own[1].m), own[2].m);
+  for (int i = lane + 192; i < parts; i += 64) m = fmaxf(m, load_part(part + i).m);
   r.m = wave_max(m);
   const float mm = max_or_nan(r.m);
   double s = 0.0;
@@ -393,7 +395,8 @@ __device__ __forceinline__ VerifyStat combine(const VerifyPart *part, int parts,
   };
   add(own[0]);
   add(own[1]);
-  for (int i = lane + 128; i < parts; i += 64) add(load_part(part + i));
+  add(own[2]);
+  for (int i = lane + 192; i < parts; i += 64) add(load_part(part + i));
   r.s = greedy ? 1.0 : wave_sum(s);
   r.arg = greedy ? wave_min(arg) : -1;
   if (r.m == -__builtin_inff()) {
@@ -425,15 +428,16 @@ __device__ __forceinline__ void final_weights(const Final &f, const Float4 &vp, 
 }
 
 // The mass of a part, by one wave.
+template <int PER>
 __device__ __forceinline__ double part_mass(const VerifyArgs &a, const Final &f, int part) {
-  Float4 vp[kVerifyPer / 4], vq[kVerifyPer / 4];
-  load_part_of(f.p.p, part, 0, a.vocab, vp);
-  if (f.pair) load_part_of(f.q.p, part, 0, a.vocab, vq);
+  Float4 vp[PER / 4], vq[PER / 4];
+  load_part_of<PER>(f.p.p, part, a.vocab, vp);
+  if (f.pair) load_part_of<PER>(f.q.p, part, a.vocab, vq);
   double s = 0.0;
 #pragma unroll
-  for (int j = 0; j < kVerifyPer / 4; ++j) {
+  for (int j = 0; j < PER / 4; ++j) {
     double w[4];
-    final_weights(f, vp[j], vq[j], part_id(part, j), w);
+    final_weights(f, vp[j], vq[j], part_id<PER>(part, j), w);
     s += (w[0] + w[1]) + (w[2] + w[3]);
   }
   return wave_sum(s);
@@ -478,13 +482,14 @@ __device__ __forceinline__ int block_first(bool hit, bool any, bool *past, Verif
 // The first id whose running sum is above u times the whole, from the parts'
 // masses (mass(part)); -1 where the whole is 0.  Every thread of the workgroup:
 // each takes consecutive parts, the one the draw falls to finds its part, then
-// each takes eight consecutive ids of that part.
-template <typename Mass>
-__device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, double u, Mass mass,
-                                       VerifySmem &sm) {
+// each takes consecutive ids of that part.
+template <int PER, typename Mass>
+__device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, int parts, double u,
+                                       Mass mass, VerifySmem &sm) {
+  constexpr int EACH = 64 * PER / kVerifyThreads;   // ids of a part a thread
   const int tid = threadIdx.x;
-  const int per = (a.parts + kVerifyThreads - 1) / kVerifyThreads;
-  const int c0 = min(tid * per, a.parts), c1 = min(c0 + per, a.parts);
+  const int per = (parts + kVerifyThreads - 1) / kVerifyThreads;
+  const int c0 = min(tid * per, parts), c1 = min(c0 + per, parts);
   const double one = c0 < c1 ? mass(c0) : 0.0;
   double own = one;
   for (int c = c0 + 1; c < c1; ++c) own += mass(c);
@@ -513,17 +518,17 @@ __device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, doub
   __syncthreads();
   const int part = sm.pick;
   const double in = sm.at;
-  const int id0 = part * kVerifyPart + tid * 8;
-  Float4 vp[2], vq[2];
+  const int id0 = part * (64 * PER) + tid * EACH;
+  Float4 vp[EACH / 4], vq[EACH / 4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < EACH / 4; ++j) {
     vp[j] = load4(f.p.p, id0 + 4 * j, a.vocab);
     if (f.pair) vq[j] = load4(f.q.p, id0 + 4 * j, a.vocab);
   }
-  double w[2][4];
+  double w[EACH / 4][4];
   own = 0.0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < EACH / 4; ++j) {
     final_weights(f, vp[j], vq[j], id0 + 4 * j, w[j]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) own += w[j][i];
@@ -534,7 +539,7 @@ __device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, doub
     double run = ids.before;
     int first = -1, live = -1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       run += w[i / 4][i % 4];
       if (w[i / 4][i % 4] > 0.0) {
         live = id0 + i;
@@ -552,6 +557,7 @@ __device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, doub
 // rejected certain draft's own probability px is taken off its part's sum;
 // where little of the sum is left, so that the difference would keep less
 // than 42 of its bits, the part is summed again without it.
+template <int PER>
 __device__ __forceinline__ int draw_from_parts(const VerifyArgs &a, Final f, int64_t row, double u,
                                                double px, VerifySmem &sm) {
   const VerifyPart *part = a.part[0] + row * a.parts;
@@ -559,15 +565,16 @@ __device__ __forceinline__ int draw_from_parts(const VerifyArgs &a, Final f, int
     const VerifyPart p = load_part(part + c);
     return p.s * weight(p.m, f.p.m, f.p.c) * f.p.inv;
   };
-  int xp = f.residual && f.x >= 0 && f.x < a.vocab ? f.x / kVerifyPart : -1;
+  int xp = f.residual && f.x >= 0 && f.x < a.vocab ? f.x / (64 * PER) : -1;
   for (;;) {
     double without = 0.0;
     if (xp >= 0) {
       const double all = sum_of(xp);
       without = all - px;
-      if (!(without >= all * 0x1p-10)) without = part_mass(a, f, xp);   // (each wave the same)
+      if (!(without >= all * 0x1p-10)) without = part_mass<PER>(a, f, xp);   // (each wave the same)
     }
-    const int id = draw_id(a, f, u, [&](int c) { return c == xp ? without : sum_of(c); }, sm);
+    const int id =
+        draw_id<PER>(a, f, a.parts, u, [&](int c) { return c == xp ? without : sum_of(c); }, sm);
     if (id >= 0 || !f.residual) return max(id, 0);
     f.residual = false;   // all of p is x: from p itself
     xp = -1;
@@ -643,7 +650,7 @@ __device__ __forceinline__ Outcome outcome_of(const VerifyArgs &a, int b, const 
 // rejection does not count, whatever is made of it.)
 // ALONE: no draft rows.  The workgroup that completes a sequence's last
 // position then writes its outcome; otherwise verify_final_kernel does.
-template <bool ALONE>
+template <bool ALONE, int PER>
 __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -681,19 +688,19 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
     // (the next part is on its way while one is summed: all waves start
     // together, and would otherwise all read, then all compute; from here on
     // each wave looks for a rejection for itself: there is no barrier in here)
-    Float4 next[kVerifyPer / 4];
-    if (part < a.parts && (rej == 0 || 64 - rej >= pos)) load_part_of(rowp, part, 0, a.vocab, next);
+    Float4 next[PER / 4];
+    if (part < a.parts && (rej == 0 || 64 - rej >= pos)) load_part_of<PER>(rowp, part, a.vocab, next);
     for (; part < a.parts && (rej == 0 || 64 - rej >= pos); part += a.split * kWavesV) {
-      Float4 v[kVerifyPer / 4];
+      Float4 v[PER / 4];
 #pragma unroll
-      for (int j = 0; j < kVerifyPer / 4; ++j) v[j] = next[j];
+      for (int j = 0; j < PER / 4; ++j) v[j] = next[j];
       if (part + a.split * kWavesV < a.parts) {
         rej = (int)load_agent32(a.rejected + b);
-        load_part_of(rowp, part + a.split * kWavesV, 0, a.vocab, next);
+        load_part_of<PER>(rowp, part + a.split * kWavesV, a.vocab, next);
       }
       float m = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < kVerifyPer; ++i) m = fmaxf(m, v[i / 4].v[i % 4]);
+      for (int i = 0; i < PER; ++i) m = fmaxf(m, v[i / 4].v[i % 4]);
       VerifyPart out;
       out.m = wave_max(m);
       out.s = 0.0;
@@ -702,16 +709,16 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
       if (greedy) {
         int arg = 0x7FFFFFFF;
 #pragma unroll
-        for (int i = 0; i < kVerifyPer; ++i)
-          if (v[i / 4].v[i % 4] == mm) arg = min(arg, part_id(part, i / 4) + i % 4);
+        for (int i = 0; i < PER; ++i)
+          if (v[i / 4].v[i % 4] == mm) arg = min(arg, part_id<PER>(part, i / 4) + i % 4);
         out.arg = wave_min(arg);
       } else {
         if (mm == __builtin_inff()) {
 #pragma unroll
-          for (int i = 0; i < kVerifyPer; ++i) out.s += v[i / 4].v[i % 4] == mm ? 1.0 : 0.0;
+          for (int i = 0; i < PER; ++i) out.s += v[i / 4].v[i % 4] == mm ? 1.0 : 0.0;
         } else {
 #pragma unroll
-          for (int j = 0; j < kVerifyPer / 4; ++j) {
+          for (int j = 0; j < PER / 4; ++j) {
             double w[4];
             weights_below(v[j].v, mm, c, w);
             out.s += (w[0] + w[1]) + (w[2] + w[3]);
@@ -753,14 +760,16 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
   const double u = a.d.uniforms[r.start + b + r.n];
   const Outcome o = outcome_of(a, b, temps, r);
   const int token = o.known ? max(o.f.p.arg, 0)
-                            : draw_from_parts(a, o.f, r.start + b + o.acc, u, o.px, sm);
+                            : draw_from_parts<PER>(a, o.f, r.start + b + o.acc, u, o.px, sm);
   if (wave == 0) emit(a.d, b, r, o.acc, token, o.ratio, 0);
 }
 
 // The outcome of every sequence that has draft rows, or probabilities for its
-// target.  After a rejection one workgroup per kVerifyBlock ids of the final
-// row sums what the final token is drawn from, and the one that completes the
+// target.  After a rejection one workgroup per four parts of the final row
+// sums what the final token is drawn from, and the one that completes the
 // row draws; without one, and logits for the target, the sums are there.
+// PER: the rows' sums', FPER: its own.
+template <int PER, int FPER>
 __global__ __launch_bounds__(kVerifyThreads, 3) void verify_final_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -799,15 +808,15 @@ __global__ __launch_bounds__(kVerifyThreads, 3) void verify_final_kernel(VerifyA
   int token;
   if (o.known || (a.kind[0] == kDistLogits && !f.residual)) {
     if (!first) return;
-    token = o.known ? max(f.p.arg, 0) : draw_from_parts(a, f, r.start + b + o.acc, u, 0.0, sm);
+    token = o.known ? max(f.p.arg, 0) : draw_from_parts<PER>(a, f, r.start + b + o.acc, u, 0.0, sm);
   } else {
-    double *mass = a.mass + (int64_t)b * a.parts;
+    double *mass = a.mass + (int64_t)b * a.fparts;
     // this workgroup's parts; then, where nothing is left beyond q (or x), all
     // of p's by the workgroup that found it so
-    int p0 = (int)blockIdx.x * kWavesV, p1 = min(p0 + kWavesV, a.parts);
+    int p0 = (int)blockIdx.x * kWavesV, p1 = min(p0 + kWavesV, a.fparts);
     for (int again = 0;; ++again) {
       for (int p = p0 + wave; p < p1; p += kWavesV) {
-        const double s = part_mass(a, f, p);
+        const double s = part_mass<FPER>(a, f, p);
         if (lane == 0) store_agent(mass + p, s);
       }
       if (!again) {
@@ -816,13 +825,13 @@ __global__ __launch_bounds__(kVerifyThreads, 3) void verify_final_kernel(VerifyA
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
       }
-      token = draw_id(a, f, u, [&](int c) {
+      token = draw_id<FPER>(a, f, a.fparts, u, [&](int c) {
         return __longlong_as_double((long long)load_agent64(mass + c));
       }, sm);
       if (token >= 0 || again) break;
       f.residual = f.pair = false;
       p0 = 0;
-      p1 = a.parts;
+      p1 = a.fparts;
       __syncthreads();
     }
     if (tid == 0) store_agent(a.left + b, 0u);   // for the next call
@@ -1045,15 +1054,23 @@ hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream, hipEvent_t *ev
     const bool both = a.kind[0] == kDistLogits && a.kind[1] == kDistLogits;
     const dim3 grid((unsigned)a.split, (unsigned)a.d.seqs,
                     (unsigned)(both ? 2 * a.d.max_drafts + 1 : a.d.max_drafts + 1));
-    const hipError_t e =
-        launches & 2u ? launch_v(verify_stats_kernel<false>, grid, 0, stream, ev_stats, nullptr, a)
-                      : launch_v(verify_stats_kernel<true>, grid, 0, stream, ev_stats, done, a);
+    const bool few = a.per == kVerifyPerFew;
+    hipError_t e;
+    if (launches & 2u)
+      e = few ? launch_v(verify_stats_kernel<false, kVerifyPerFew>, grid, 0, stream, ev_stats, nullptr, a)
+              : launch_v(verify_stats_kernel<false, kVerifyPer>, grid, 0, stream, ev_stats, nullptr, a);
+    else
+      e = few ? launch_v(verify_stats_kernel<true, kVerifyPerFew>, grid, 0, stream, ev_stats, done, a)
+              : launch_v(verify_stats_kernel<true, kVerifyPer>, grid, 0, stream, ev_stats, done, a);
     if (e != hipSuccess) return e;
   }
-  if (launches & 2u)
-    return launch_v(verify_final_kernel, dim3((unsigned)a.blocks, (unsigned)a.d.seqs), 0, stream,
-                    ev_final, done, a);
-  return hipSuccess;
+  if (!(launches & 2u)) return hipSuccess;
+  const dim3 grid((unsigned)a.blocks, (unsigned)a.d.seqs);
+  if (a.fper == kVerifyPer)   // (target logits: at least as many rows are summed as drawn from)
+    return launch_v(verify_final_kernel<kVerifyPer, kVerifyPer>, grid, 0, stream, ev_final, done, a);
+  return a.per == kVerifyPer
+             ? launch_v(verify_final_kernel<kVerifyPer, kVerifyPerFew>, grid, 0, stream, ev_final, done, a)
+             : launch_v(verify_final_kernel<kVerifyPerFew, kVerifyPerFew>, grid, 0, stream, ev_final, done, a);
 }
 
 // (the longest lists' table and the kernel's own LDS pass 64 KB)
