@@ -218,8 +218,8 @@ struct hs_context {
   // workspace
   DevBuf plans, cand, cand_count, info;
   DevBuf split_list, split_meta, split_cnt;   // split rows (split_cnt: zero between calls)
-  DevBuf gemv_part, gemv_cnt;   // Q4_K/Q6_K GEMV tiles cut between waves (gemv_cnt: zero between calls)
-  DevBuf gemv_rot;              // the Hadamard-rotated input of a folded weight (see gemv_setup)
+  KeptBuf gemv_part, gemv_cnt;  // Q4_K/Q6_K GEMV tiles cut between waves (gemv_cnt: zero between calls)
+  KeptBuf gemv_rot;             // the Hadamard-rotated input of a folded weight (see gemv_setup)
   DevBuf gemv_tab;              // limb tables of several activation rows (from creation on, in
                                 //   one size: a first call may be captured, and a captured
                                 //   graph's address stays good)
@@ -485,6 +485,20 @@ int ensure_zeroed(DevBuf &b, size_t need, hipStream_t stream) {
   if (e != hipSuccess) {
     b.release();
     return fail(HS_ERR_HIP, "hipMemset(counters) failed: %s", hipGetErrorString(e));
+  }
+  return HS_OK;
+}
+
+int ensure_zeroed(KeptBuf &k, size_t need, hipStream_t stream) {
+  if (k.b.bytes >= need) return HS_OK;
+  HS_HIP(k.ensure(need));
+  const hipError_t e = inject_failure()
+                           ? hipErrorOutOfMemory
+                           : hs::launch_fill_u32(static_cast<uint32_t *>(k.b.p),
+                                                 (int64_t)(k.b.bytes / sizeof(uint32_t)), 0u, stream);
+  if (e != hipSuccess) {
+    k.b.release();
+    return fail(HS_ERR_HIP, "clearing the counters failed: %s", hipGetErrorString(e));
   }
   return HS_OK;
 }
@@ -834,15 +848,15 @@ int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const 
     HS_HIP(ctx->gemv_part.ensure(slots * 16 * sizeof(float)));
     const int rz = ensure_zeroed(ctx->gemv_cnt, slots * sizeof(uint32_t), stream);
     if (rz) return rz;
-    g.part = static_cast<float *>(ctx->gemv_part.p);
-    g.tile_cnt = static_cast<uint32_t *>(ctx->gemv_cnt.p);
+    g.part = static_cast<float *>(ctx->gemv_part.b.p);
+    g.tile_cnt = static_cast<uint32_t *>(ctx->gemv_cnt.b.p);
   }
   if (wt->hadamard && planar && !g.tab) {   // rotated by the GEMV itself
     g.rotate = 1;
     g.signs = wt->signs;
   } else if (wt->hadamard) {   // src/engine.ts:1121-1145: the input is rotated first
     HS_HIP(ctx->gemv_rot.ensure((size_t)M * (size_t)K * sizeof(float)));
-    float *rot = static_cast<float *>(ctx->gemv_rot.p);
+    float *rot = static_cast<float *>(ctx->gemv_rot.b.p);
     const hipError_t e = hs::launch_hadamard(d_x, ldx, wt->signs, rot, M, K, stream);
     if (e != hipSuccess) return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
     g.x = rot;
@@ -1291,18 +1305,9 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
   if (rc) return rc;
   if (!cap) rc = enter_stream(ctx, stream);
   if (rc) return rc;
-  if (counts * sizeof(uint32_t) > ctx->verify_cnt.b.bytes) {
-    rc = kept_room(ctx->verify_cnt, counts * sizeof(uint32_t), cap);
-    if (rc) return rc;
-    const hipError_t e = inject_failure()
-                             ? hipErrorOutOfMemory
-                             : hs::launch_fill_u32(static_cast<uint32_t *>(ctx->verify_cnt.b.p),
-                                                   (int64_t)(ctx->verify_cnt.b.bytes / 4), 0u, stream);
-    if (e != hipSuccess) {
-      ctx->verify_cnt.b.release();
-      return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
-    }
-  }
+  if (cap) rc = kept_room(ctx->verify_cnt, counts * sizeof(uint32_t), cap);
+  else rc = ensure_zeroed(ctx->verify_cnt, counts * sizeof(uint32_t), stream);
+  if (rc) return rc;
   char *ws = static_cast<char *>(ctx->verify_ws.b.p);
   for (int i = 0; i < 2; ++i)
     if (a.kind[i] == hs::kDistLogits) {

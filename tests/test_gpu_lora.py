@@ -350,6 +350,43 @@ def test_streams_timing_and_graphs():
         s.destroy()
 
 
+@pytest.mark.parametrize("fmt,hadamard,M", [("q6_k", False, 1), ("q4_0", True, 5)])
+def test_captured_projection_before_a_larger_one(fmt, hadamard, M):
+    """A graph keeps the addresses of the projection's own workspaces (the
+    hand-over of split tiles, the rotated rows): calls that need larger ones
+    leave them where they are."""
+    from tests.test_oracle_lmhead import random_blocks
+    wt = {"q6_k": 14, "q4_0": 2}[fmt]
+    rng = np.random.default_rng(40 + M)
+    K, N, more = 1024, 3001, 40
+    dw = dev(np.ascontiguousarray(random_blocks(wt, N, K, rng)).reshape(-1))
+    w = hs.weights(wt, N, K, dw.addr, None, hadamard, None)
+    ad = Adapters(rng, "f16", 3, 12, K, N)
+    x = rng.standard_normal((more, K)).astype(np.float32)
+    dx, ds = dev(x), dev(rng.integers(-1, 3, more).astype(np.int32))
+    y, yl = hip.DeviceArray((M, N), np.float32), hip.DeviceArray((more, N), np.float32)
+    st = hip.Stream()
+    with Sampler(0) as ctx:
+        call = lambda: ctx.gemv_lora_device(dx.addr, M, K, w, ad.desc, ds.addr, y.addr, N, stream=st)
+        print(f"[gpu] captured gemv + lora {fmt} M={M}, then M={more}", flush=True)
+        call()
+        st.synchronize()
+        want = y.download()
+        g = Graph(st, call)
+        for _ in range(3):
+            ctx.gemv_lora_device(dx.addr, more, K, w, ad.desc, ds.addr, yl.addr, N, stream=st)
+            filler = [hip.DeviceArray((more, K), np.float32) for _ in range(4)]   # (in freed memory, if any)
+            for f in filler:
+                f.upload(np.full((more, K), np.nan, np.float32))
+            y.upload(np.zeros((M, N), np.float32))
+            hip.synchronize()
+            g.launch()
+            st.synchronize()
+            assert np.array_equal(y.download().view(np.uint32), want.view(np.uint32))
+        g.destroy()
+    st.destroy()
+
+
 @pytest.mark.parametrize("captured", [False, True])
 def test_a_speculative_step_with_adapters(captured):
     """Hidden states of all drafted positions, through a shared lm_head with
