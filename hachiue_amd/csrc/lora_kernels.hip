@@ -6,8 +6,10 @@
 // binary32, binary16 or bfloat16.
 //
 // Two launches: x A^T into a workspace (binary32, the scale on it), then B.
-// Both run on the matrix cores' binary32 products (16 x 16 x 4): the adapters
-// widen to binary32 exactly, so nothing is rounded but the sums.  Rows go in
+// Binary16 and binary32 adapters run on the matrix cores' binary32 products
+// (16 x 16 x 4), to which they widen exactly; bfloat16 ones on bfloat16 products
+// with x and t as three exact parts.  Nothing is rounded but the binary32 sums,
+// either way.  Rows go in
 // tiles of 16 as they come.  A tile is computed once for every adapter that
 // its rows name and each row keeps the result of its own: rows of one prompt
 // follow each other and share one pass, a batch with an adapter per row reads
@@ -19,6 +21,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace hs {
 namespace {
@@ -58,6 +61,59 @@ struct alignas(16) Lane {
   T v[n];
 };
 
+// A binary32 value as the exact sum of three bfloat16 ones (its leading 8 bits,
+// the next 8, the last 8; below 2^-110 the last may underflow): its products
+// with a bfloat16 are then three bfloat16 products, which the matrix cores
+// sum in binary32 at sixteen times the rate of binary32 ones.  An infinity is
+// one part, a NaN stays one.  (2048 rows x 4096, rank 64: 42 us a call, 55 with
+// binary32 products.  A binary16 value is two bfloat16 ones, which would have to
+// be parted in every workgroup that reads it: twice the products and that.)
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short bf16x4 __attribute__((ext_vector_type(4)));
+template <int n>
+struct Operand;
+template <>
+struct Operand<8> {
+  typedef bf16x8 V;
+};
+template <>
+struct Operand<4> {
+  typedef bf16x4 V;
+};
+__device__ __forceinline__ f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_bf16(bf16x4 a, bf16x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+}
+template <int n>
+struct Parts {
+  typename Operand<n>::V v[3];   // the leading first
+};
+template <int n>
+__device__ __forceinline__ Parts<n> parts_of(const float (&x)[n]) {
+  union {
+    uint32_t u[n / 2];
+    typename Operand<n>::V v;
+  } p[3];
+#pragma unroll
+  for (int i = 0; i < n; i += 2) {
+    uint32_t u[3][2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float f = x[i + e];
+      u[0][e] = __float_as_uint(f);
+      float r = f - __uint_as_float(u[0][e] & 0xFFFF0000u);
+      r = __builtin_fabsf(f) == __builtin_inff() ? 0.0f : r;
+      u[1][e] = __float_as_uint(r);
+      u[2][e] = __float_as_uint(r - __uint_as_float(u[1][e] & 0xFFFF0000u));
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) p[j].u[i / 2] = __builtin_amdgcn_perm(u[j][1], u[j][0], 0x07060302u);
+  }
+  return {{p[0].v, p[1].v, p[2].v}};
+}
+
 // The adapter of the tile's row `lane & 15`, -1: none.
 __device__ __forceinline__ int slot_of(const LoraArgs &g, int m0) {
   const int m = m0 + (threadIdx.x & 15);
@@ -84,20 +140,25 @@ constexpr int kShrinkWaves = 8;
 constexpr int kShrinkK = kShrinkWaves * 32;   // k of a stage
 
 // t = scale x A^T of one tile and the adapters that its rows name, in the order
-// of the rows (block z takes every gridDim.z-th of them).  A workgroup takes JB blocks of 16 ranks and one of `splits` shares of K, in
-// stages of 256 k through LDS: rows are read along k, a wave instruction 1 KB
-// of one row, because the matrix operand's own order (16 rows side by side in
-// the lanes) makes the cache look up a line per lane: 2048 rows x 4096 with
-// rank 64 took 33 us that way.  The next stage is on its way while one is
+// of the rows (block z takes every gridDim.z-th of them).  A workgroup takes JB
+// blocks of 16 ranks and one of `splits` shares of K, in stages of 256 k through
+// LDS: rows are read along k, a wave instruction 1 KB of one row, because the
+// matrix operand's own order (16 rows side by side in the lanes) makes the cache
+// look up a line per lane.  The next stage is on its way while one is
 // multiplied, each wave 32 of its k, lanes l, l + 16, ... 8 consecutive ones
 // each; the waves' sums meet in LDS.
+// Bound: for prompts a stage's latency (2048 rows x 4096, rank 64, bfloat16:
+// 17 us, of which 8 stages 1.4 each; x at 2 TB/s, A from L2), for a few rows that
+// of the one chain over K (one row x 2048 4.5 us, 32 rows with an adapter each
+// 6.0).
 template <typename T, int JB>
 __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs g) {
   // (rows 16 bytes longer than a stage: the operands' reads meet no bank twice)
   constexpr int XS = kShrinkK + 4, AS = kShrinkK + 16 / (int)sizeof(T);
   constexpr int PER = 16 / (int)sizeof(T);        // elements of a 16-byte read
   constexpr int RPI = 64 * PER / kShrinkK;        // rows of A an instruction
-  constexpr int AI = 16 * JB / RPI / kShrinkWaves > 0 ? 16 * JB / RPI / kShrinkWaves : 1;
+  constexpr int AI = 16 * JB / RPI / kShrinkWaves;
+  static_assert(AI * RPI * kShrinkWaves == 16 * JB, "a stage of A is whole reads");
   union alignas(16) Lds {
     struct {
       float x[16][XS];
@@ -109,7 +170,10 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int groups = g.rank_pad / (16 * JB);
-  const int m0 = blockIdx.x * 16, j0 = (int)blockIdx.y % groups * (16 * JB);
+  // tiles that follow each other, which share adapters, go to one XCD's cache
+  const int eighth = gridDim.x >> 3, xcd = blockIdx.x & 7;
+  const int tile = xcd * eighth + min(xcd, (int)gridDim.x & 7) + (int)(blockIdx.x >> 3);
+  const int m0 = tile * 16, j0 = (int)blockIdx.y % groups * (16 * JB);
   const int split = (int)blockIdx.y / groups;
   const int own = slot_of(g, m0);
   uint32_t todo = (uint32_t)__ballot(own >= 0) & 0xFFFFu;
@@ -124,7 +188,6 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
     if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
     const int rank = g.ranks ? min(max(g.ranks[s], 0), g.rank) : g.rank;
     const float scale = g.scales ? g.scales[s] : 1.0f;
-    int k = k0;
     // what this thread reads of a stage: two rows of x, AI times PER elements of A
     const int xk = lane * 4, ak = lane * PER % kShrinkK, ar = lane * PER / kShrinkK;
     const float *xrow[2];
@@ -139,38 +202,35 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
       arow[h] = static_cast<const T *>(g.a) +
                 ((int64_t)s * g.rank + min(j0 + ai[h], g.rank - 1)) * g.K + ak;
     }
-    Run<float, 4> xn[2];
-    Run<T, PER> an[AI];
-    auto read = [&](int k) {
-      const bool whole = k + kShrinkK <= g.K;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        xn[h] = whole ? load_run<4>(xrow[h] + k) : load_run<4>(xrow[h] + k, g.K - k - xk);
-#pragma unroll
-      for (int h = 0; h < AI; ++h)
-        if (ai[h] < 16 * JB)
-          an[h] = whole ? load_run<PER>(arow[h] + k) : load_run<PER>(arow[h] + k, g.K - k - ak);
-    };
     f32x4 acc[JB];
 #pragma unroll
     for (int j = 0; j < JB; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    // (one stage ahead: two took 37 us where this takes 28)
-    if (k < k1) read(k);
-    while (k < k1) {
+    Run<float, 4> xn[2];
+    Run<T, PER> an[AI];
+    auto put = [&]() {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<Lane<float, 4> *>(&lds.in.x[2 * wave + h][xk]) =
             __builtin_bit_cast(Lane<float, 4>, xn[h]);
 #pragma unroll
       for (int h = 0; h < AI; ++h)
-        if (ai[h] < 16 * JB)
-          *reinterpret_cast<Lane<T, PER> *>(&lds.in.a[ai[h]][ak]) =
-              __builtin_bit_cast(Lane<T, PER>, an[h]);
-      __syncthreads();
-      k += kShrinkK;
-      if (k < k1) read(k);
+        *reinterpret_cast<Lane<T, PER> *>(&lds.in.a[ai[h]][ak]) =
+            __builtin_bit_cast(Lane<T, PER>, an[h]);
+    };
+    auto multiply = [&]() {
       const int kk = wave * 32 + grp * 8;
       const Lane<float, 8> xv = *reinterpret_cast<const Lane<float, 8> *>(&lds.in.x[i16][kk]);
+      if constexpr (std::is_same_v<T, BF16>) {
+        const Parts<8> xp = parts_of(xv.v);
+#pragma unroll
+        for (int j = 0; j < JB; ++j) {
+          const bf16x8 av = *reinterpret_cast<const bf16x8 *>(&lds.in.a[16 * j + i16][kk]);
+#pragma unroll
+          for (int i = 2; i >= 0; --i)
+            acc[j] = mfma_bf16(xp.v[i], av, acc[j]);
+        }
+        return;
+      }
 #pragma unroll
       for (int j = 0; j < JB; ++j) {
         const Lane<T, 8> av = *reinterpret_cast<const Lane<T, 8> *>(&lds.in.a[16 * j + i16][kk]);
@@ -178,6 +238,36 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
         for (int i = 0; i < 8; ++i)
           acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv.v[i], widen(av.v[i]), acc[j], 0, 0, 0);
       }
+    };
+    // Whole stages: the reads are never skipped (behind the last they repeat
+    // it).  One stage ahead: two take the registers of the second workgroup of
+    // a compute unit, 24 us where this takes 17.
+    const int whole = max(k1 - k0, 0) / kShrinkK;
+    if (whole > 0) {
+      auto read = [&](int stage) {
+        const int k = k0 + min(stage, whole - 1) * kShrinkK;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) xn[h] = load_run<4>(xrow[h] + k);
+#pragma unroll
+        for (int h = 0; h < AI; ++h) an[h] = load_run<PER>(arow[h] + k);
+      };
+      read(0);
+      for (int stage = 1; stage <= whole; ++stage) {
+        put();
+        __syncthreads();
+        read(stage);
+        multiply();
+        __syncthreads();
+      }
+    }
+    if (const int k = k0 + whole * kShrinkK; k < k1) {   // what is left of K
+#pragma unroll
+      for (int h = 0; h < 2; ++h) xn[h] = load_run<4>(xrow[h] + k, g.K - k - xk);
+#pragma unroll
+      for (int h = 0; h < AI; ++h) an[h] = load_run<PER>(arow[h] + k, g.K - k - ak);
+      put();
+      __syncthreads();
+      multiply();
       __syncthreads();
     }
     // acc: rows 4 grp + i of the tile, rank i16
@@ -205,6 +295,8 @@ constexpr int kExpandWaves = 4;
 // l, l + 16, ... hold VK consecutive ones each; the rows' t stay in registers,
 // and the next step's B (of the next adapter after an adapter's last) is on
 // its way while one is multiplied.  RB: blocks of 16 ranks.
+// Bound: memory; 32 rows with an adapter each over 151936 results at rank 16
+// (194 MB) 45 us, 4.3 TB/s.  One row (6 MB) 4.5 us, which is a launch.
 template <typename T, int RB, int NT>
 __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs g) {
   constexpr int VK = RB == 1 ? 4 : 8, STEPS = RB * 4 / VK;
@@ -236,6 +328,12 @@ __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs
 #pragma unroll
       for (int e = 0; e < 4; ++e) t[r][i + e] = v[e];
     }
+  constexpr bool parted = std::is_same_v<T, BF16>;
+  Parts<VK> tp[parted ? STEPS : 1];
+  if constexpr (parted) {
+#pragma unroll
+    for (int r = 0; r < STEPS; ++r) tp[r] = parts_of(t[r]);
+  }
   uint32_t todo = (uint32_t)__ballot(own >= 0) & 0xFFFFu;
   f32x4 out[NT];
 #pragma unroll
@@ -285,6 +383,19 @@ __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs
         else if (more) load(s2, 0, next);
         const int k = r * 4 * VK + grp * VK;
         const bool full = (r + 1) * 4 * VK <= rank;
+        if constexpr (parted) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (!full) {
+#pragma unroll
+              for (int i = 0; i < VK; ++i) b[n].v[i].u = k + i < rank ? b[n].v[i].u : (uint16_t)0;
+            }
+            const auto w = __builtin_bit_cast(typename Operand<VK>::V, b[n]);
+#pragma unroll
+            for (int i = 2; i >= 0; --i) acc[n] = mfma_bf16(w, tp[r].v[i], acc[n]);
+          }
+          continue;
+        }
 #pragma unroll
         for (int i = 0; i < VK; ++i)
 #pragma unroll
@@ -331,7 +442,8 @@ __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs
 // rows (the operands' own order, a lane a row, costs the cache a look-up per lane,
 // which bounds the kernel above once a row of B is longer than a line).  The next
 // chunk (of the next adapter after an adapter's last) is on its way while
-// one is multiplied.
+// one is multiplied.  2048 rows x 4096 at rank 64, bfloat16:
+// 22 us, 3.1 TB/s of base and y.
 template <typename T>
 __global__ __launch_bounds__(256, 3) void lora_expand_wide_kernel(LoraArgs g) {
   constexpr int CH = 128 / (int)sizeof(T), PER = 16 / (int)sizeof(T);   // a chunk's ranks, a read's
@@ -407,6 +519,18 @@ __global__ __launch_bounds__(256, 3) void lora_expand_wide_kernel(LoraArgs g) {
     for (int k = 0; k < CH; k += 32) {
       if (k >= live) break;
       const Lane<float, 8> tv = *reinterpret_cast<const Lane<float, 8> *>(&lds.in.t[i16][k + grp * 8]);
+      if constexpr (std::is_same_v<T, BF16>) {
+        const Parts<8> tp = parts_of(tv.v);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const bf16x8 b =
+              *reinterpret_cast<const bf16x8 *>(&lds.in.b[wave * 64 + 16 * n + i16][k + grp * 8]);
+#pragma unroll
+          for (int i = 2; i >= 0; --i)
+            acc[n] = mfma_bf16(b, tp.v[i], acc[n]);
+        }
+        continue;
+      }
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const Lane<T, 8> b =
@@ -494,12 +618,14 @@ hipError_t expand_by_rank(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev,
 }
 
 // Through LDS where ranks fill a chunk and there are workgroups enough (each
-// takes its tile's adapters one after the other).  us, a lane a row and through
-// LDS:
-//   2048 x 4096, 8 adapters, rank 32 21, 25, rank 64 34, 26, rank 128 49, 37
-//   16 x 100000 (391 workgroups), 2 adapters, rank 64 15, 14, rank 128 25, 20; 16
-//   adapters 73, 69 and 147, 124; 64 x 32000 (500) 16 adapters, rank 83 135, 116
-//   32 x 32000 (250), 8 adapters, rank 64 24, 27; 16 x 8000 (32), 16 adapters 16, 45
+// takes its tile's adapters one after the other).  us of bfloat16, a lane a row
+// and through LDS:
+//   2048 x 4096 (2048 workgroups), 8 adapters, rank 32 17, 24, rank 64 24, 21, rank
+//   128 33, 25; 512 x 4096 (512), 4 adapters, rank 64 7.1, 6.8
+//   16 x 100000 (391), 2 adapters, rank 64 8.8, 7.8, rank 128 13.5, 12; 16 adapters
+//   35, 33 and 89, 70; 64 x 32000 (500), 16 adapters, rank 83 110, 83
+//   32 x 32000 (250), 8 adapters, rank 64 13.6, 15.4; 16 x 8000 (32), 16 adapters
+//   8.9, 22.6
 inline bool expand_wide(const LoraArgs &g) {
   return g.rank_pad >= 64 && (int64_t)((g.N + 255) / 256) * ((g.M + 15) / 16) >= 384;
 }

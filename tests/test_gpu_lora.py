@@ -211,6 +211,28 @@ def test_what_is_not_finite_stays_in_its_rows(sampler, kind):
         assert np.isnan(y[m, 7]) and np.isfinite(np.delete(y[m], 7)).all(), m
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rank,N", [(12, 77), (40, 300), (64, 98400)])
+def test_scales_and_infinities(sampler, kind, rank, N):
+    """Far from 1 the error stays relative (2^-100 keeps every term's last bit a
+    normal number but for terms that are themselves that much smaller); an
+    infinity times positive elements is one, a NaN one whatever its bits."""
+    rng = np.random.default_rng(rank)
+    ad = Adapters(rng, kind, 2, rank, 300, N)
+    x = rng.standard_normal((5, 300)).astype(np.float32)
+    slots = [1, 0, 0, 1, 1]
+    for e in (-100, 100):
+        y, _ = run(sampler, ad, np.ldexp(x, e).astype(np.float32), slots, None)
+        check(ad, np.ldexp(x, e).astype(np.float32), slots, None, y)
+    arr = [dev(stored(np.full(shape, 0.5), kind)[0]) for shape in ((2, rank, 300), (2, N, rank))]
+    ad.arr, ad.desc = arr, hs.adapters(TYPES[kind], 2, rank, 300, N, arr[0].addr, arr[1].addr)
+    x[0, 3] = np.array([0x7F800001], np.uint32).view(np.float32)[0]
+    x[1, 299], x[2, 255], x[3, 8] = np.inf, -np.inf, np.nan
+    y, _ = run(sampler, ad, x, slots, None)
+    assert np.isnan(y[0]).all() and (y[1] == np.inf).all() and (y[2] == -np.inf).all()
+    assert np.isnan(y[3]).all() and np.isfinite(y[4]).all()
+
+
 def test_a_row_is_the_same_in_any_company(sampler):
     """Bit for bit, whatever rows and adapters share its tile."""
     rng = np.random.default_rng(4)
