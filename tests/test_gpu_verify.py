@@ -412,3 +412,37 @@ def test_contexts_side_by_side():
     for i in range(2):
         ctx[i].close()
         st[i].destroy()
+
+
+def test_threads_share_a_context():
+    """Calls of several threads on streams of their own, of sizes that make the
+    workspace grow: one after another on the context's workspace."""
+    import threading
+    rng = np.random.default_rng(16)
+    V, todo = 20021, []
+    for lens, draft in (([3, 5], "logits"), ([2] * 30, "probs"), ([4], None)):
+        t, d, ids, u = random_case(rng, lens, V, draft is not None, "logits", draft or "logits")
+        arr = dev(t), dev(d) if draft else None
+        td = hs.distribution(0, arr[0].addr, V)
+        qd = hs.distribution(0 if draft == "logits" else 1, arr[1].addr, V) if draft else None
+        todo.append((Drafts(lens, ids, u), t, d, draft, td, qd, hip.Stream(), arr))
+    hip.synchronize()
+    failed = []
+    with Sampler(0) as ctx:
+        def calls(b, td, qd, st):
+            try:
+                for _ in range(25):
+                    ctx.verify_drafts_device(td, qd, V, b.desc, stream=st)
+            except Exception as e:   # noqa: BLE001 (reported below)
+                failed.append(e)
+        threads = [threading.Thread(target=calls, args=(b, td, qd, st)) for b, _, _, _, td, qd, st, _ in todo]
+        for th in threads:
+            th.start()
+        for th in threads:
+            th.join()
+        hip.synchronize()
+        assert not failed, failed
+        for b, t, d, draft, *_ in todo:
+            b.check(expected(b, t, d, "logits", draft or "logits"))
+    for *_, st, _ in todo:
+        st.destroy()
