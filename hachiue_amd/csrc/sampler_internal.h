@@ -483,7 +483,8 @@ inline unsigned verify_launches(const VerifyArgs &a) {
 }
 // How rows are cut.  Workgroups of a row whose logits are summed: enough that
 // all rows together give each compute unit four, but each has up to kVerifyDeep
-// turns of its four waves to itself (4: verify of 64 sequences 145 us; 2: 152).
+// turns of its four waves to itself (4 takes 5 % less than 2
+// for 64 sequences of 8 drafts over 151936 logits).
 constexpr int kVerifyDeep = 4;
 inline void verify_cut(VerifyArgs &a) {
   auto parts = [&](int per) { return (a.vocab + 64 * per - 1) / (64 * per); };

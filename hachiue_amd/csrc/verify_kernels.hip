@@ -654,8 +654,8 @@ __device__ __forceinline__ Outcome outcome_of(const VerifyArgs &a, int b, const 
 // operations of 5.6 cycles a wave), at the small end the chain load -> sum ->
 // count in -> join.  A logit is read once: the sums are under each part's own
 // maximum and meet under the row's.  Over rows of 151936 logits: 64 sequences
-// of 8 drafts with draft rows 98 us (661 MB if no row were left out), 16 of 4
-// 35 us (88 MB, 2.5 TB/s), one of 3 without draft rows, outcome and all, 12 us.
+// of 8 drafts with draft rows 92 us (373 MB of the rows' 661, 4.0 TB/s), 16 of 4
+// 33 us (88 MB, 2.7 TB/s), one of 3 without draft rows, outcome and all, 12 us.
 template <bool ALONE, int PER>
 __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
@@ -776,8 +776,9 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
 // row draws; without one, and logits for the target, the sums are there.
 // PER: the rows' sums', FPER: its own.
 // Bound: the final rows' second read, 78 MB for 64 sequences of 151936 logits
-// in 32 us (2.4 TB/s; binary64 weights of two rows an id, and a draw behind the
-// last part), 32 sequences of probabilities (39 MB) 14.6 us.
+// in 28.5 us (2.7 TB/s; binary64 weights of two rows an id, and a draw behind the
+// last part), 32 sequences of probabilities (39 MB) 14.2 us.  Two parts a wave in
+// turn, with half the workgroups, took 30 and 16.5 us.
 template <int PER, int FPER>
 __global__ __launch_bounds__(kVerifyThreads, 3) void verify_final_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
