@@ -503,6 +503,27 @@ int ensure_zeroed(KeptBuf &k, size_t need, hipStream_t stream) {
   return HS_OK;
 }
 
+// Whether `s` is being captured.  Such a call neither waits for the context's
+// earlier calls nor leaves an event behind (neither may cross a capture's
+// border) and takes no timing events.
+bool is_capturing(hipStream_t s) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(s, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+}
+
+// Room in a workspace that captured calls share: they take what is there, as
+// nothing may be allocated in a capture, and a fill recorded into the graph
+// would leave counters uncleared until its first replay, then clear them in
+// every replay.
+int kept_room(KeptBuf &b, size_t need, bool cap) {
+  if (need <= b.b.bytes) return HS_OK;
+  if (cap)
+    return fail(HS_ERR_UNSUPPORTED,
+                "a captured call of this size needs one outside of the capture first");
+  HS_HIP(b.ensure(need));
+  return HS_OK;
+}
+
 int ensure_split(hs_context *ctx, int rows, int split, hipStream_t stream) {
   if (split <= 1) return HS_OK;
   const size_t parts = (size_t)rows * (size_t)split;
@@ -770,7 +791,7 @@ int argmax_device(hs_context *ctx, const float *d_logits, int32_t rows, int64_t 
 // here, into the workspace, except where the GEMV does it (planar formats, a
 // row at a time).  *skip: nothing to compute (M or N is 0).
 int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *wt,
-               float *d_y, int64_t ldy, hipStream_t stream, hs::GemvArgs &g, bool *skip) {
+               float *d_y, int64_t ldy, hipStream_t stream, bool cap, hs::GemvArgs &g, bool *skip) {
   *skip = false;
   if (!ctx) return fail(HS_ERR_INVALID_ARGUMENT, "null context");
   if (!wt) return fail(HS_ERR_INVALID_ARGUMENT, "null weights");
@@ -840,22 +861,28 @@ int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const 
   g.blocks = (int32_t)std::min<int64_t>((steps + wpb - 1) / wpb, 1 << 20);
   if (M > 65535) return fail(HS_ERR_UNSUPPORTED, "M %d above 65535", M);
   if (hs::gemv_batched(w_type, M, N, K)) g.tab = ctx->gemv_tab.p;   // several rows: their limb tables
+  const bool rotate = wt->hadamard && !(planar && !g.tab);   // (planar rows: by the GEMV itself)
+  if (rotate) {
+    const int rc = kept_room(ctx->gemv_rot, (size_t)M * (size_t)K * sizeof(float), cap);
+    if (rc) return rc;
+  }
   if (!g.tab && (w_type == hs::kW_Q6_K || w_type == hs::kW_Q4_K)) {   // the hand-over slots of tiles cut between waves
     int cus = 0;
     HS_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, ctx->device));
     g.part_cap = cus * hs::kGemvWavesPerCU;
     const size_t slots = (size_t)g.part_cap * (size_t)M;
-    HS_HIP(ctx->gemv_part.ensure(slots * 16 * sizeof(float)));
-    const int rz = ensure_zeroed(ctx->gemv_cnt, slots * sizeof(uint32_t), stream);
-    if (rz) return rz;
+    int rc = kept_room(ctx->gemv_part, slots * 16 * sizeof(float), cap);
+    if (rc) return rc;
+    if (cap) rc = kept_room(ctx->gemv_cnt, slots * sizeof(uint32_t), cap);
+    else rc = ensure_zeroed(ctx->gemv_cnt, slots * sizeof(uint32_t), stream);
+    if (rc) return rc;
     g.part = static_cast<float *>(ctx->gemv_part.b.p);
     g.tile_cnt = static_cast<uint32_t *>(ctx->gemv_cnt.b.p);
   }
-  if (wt->hadamard && planar && !g.tab) {   // rotated by the GEMV itself
+  if (wt->hadamard && !rotate) {
     g.rotate = 1;
     g.signs = wt->signs;
-  } else if (wt->hadamard) {   // src/engine.ts:1121-1145: the input is rotated first
-    HS_HIP(ctx->gemv_rot.ensure((size_t)M * (size_t)K * sizeof(float)));
+  } else if (rotate) {   // src/engine.ts:1121-1145: the input is rotated first
     float *rot = static_cast<float *>(ctx->gemv_rot.b.p);
     const hipError_t e = hs::launch_hadamard(d_x, ldx, wt->signs, rot, M, K, stream);
     if (e != hipSuccess) return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
@@ -863,14 +890,6 @@ int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const 
     g.ldx = K;
   }
   return HS_OK;
-}
-
-// Whether `s` is being captured.  Such a call neither waits for the context's
-// earlier calls nor leaves an event behind (neither may cross a capture's
-// border) and takes no timing events.
-bool is_capturing(hipStream_t s) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  return hipStreamIsCapturing(s, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
 }
 
 // Start/end events of timing slot `slot` for the call's one kernel, when
@@ -925,7 +944,7 @@ int gemv_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const
   if (rc) return rc;
   hs::GemvArgs g;
   bool skip = false;
-  rc = gemv_setup(ctx, d_x, M, ldx, wt, d_y, ldy, stream, g, &skip);
+  rc = gemv_setup(ctx, d_x, M, ldx, wt, d_y, ldy, stream, cap, g, &skip);
   if (rc || skip) return rc;   // nothing was enqueued
   hipEvent_t *ev = nullptr;
   if (!cap) rc = timed_slot(ctx, hs::kGemvTimedSlot, &ev);
@@ -1182,15 +1201,6 @@ int sample_host_zero_copy(hs_context *ctx, float *logits, size_t lbytes, int32_t
 
 
 // ---- verification of drafted tokens, low-rank adapters
-
-int kept_room(KeptBuf &b, size_t need, bool cap) {
-  if (need <= b.b.bytes) return HS_OK;
-  if (cap)
-    return fail(HS_ERR_UNSUPPORTED,
-                "a captured call of this size needs one outside of the capture first");
-  HS_HIP(b.ensure(need));
-  return HS_OK;
-}
 
 // The calls below check their arguments before they take the context.
 
@@ -1781,7 +1791,7 @@ int lm_head_sample(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, co
     if (rc) return rc;
     hs::GemvArgs g;
     bool skip = false;
-    rc = gemv_setup(ctx, d_x, M, ldx, w, d_logits, ldl, st, g, &skip);
+    rc = gemv_setup(ctx, d_x, M, ldx, w, d_logits, ldl, st, is_capturing(st), g, &skip);
     if (rc) return rc;
     const int blocks = skip     ? 0
                        : greedy ? hs::argmax_fused_grid(g)

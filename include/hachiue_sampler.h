@@ -242,7 +242,10 @@ typedef struct hs_weights {
  * largest |x|, so an element below about 2^-28 of that maximum counts as 0.
  * A non-finite element of an x row makes every result of that row NaN.
  * Asynchronous on `stream`; a folded weight's rotated input lives in the
- * context's workspace. */
+ * context's workspace.  May be captured as hs_verify_drafts_device may; calls
+ * that hand sums on in the workspace (Q4_K and Q6_K rows that are not computed
+ * together) or rotate into it need one call of that size outside of a capture
+ * first, and return HS_ERR_UNSUPPORTED otherwise. */
 int hs_gemv_device_ex(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
                       const hs_weights *w, float *d_y, int64_t ldy, void *stream);
 
@@ -444,7 +447,8 @@ int hs_lora_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
                    int64_t ldb, float *d_y, int64_t ldy, void *stream);
 
 /* hs_gemv_device_ex and the adapters on its result; the adapters' cols and rows
- * are the weights'.  (A Hadamard-folded weight's adapters see x as given.) */
+ * are the weights'.  (A Hadamard-folded weight's adapters see x as given.)
+ * Captured as both its steps may be. */
 int hs_gemv_lora_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
                         const hs_weights *w, const hs_adapters *adapters,
                         const int32_t *d_slots, float *d_y, int64_t ldy, void *stream);

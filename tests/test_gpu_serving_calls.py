@@ -1,0 +1,88 @@
+"""The calls around drafted tokens and adapters that the contexts' workspaces
+decide: captured first calls, allocations that fail, results that depend on
+how a call is cut."""
+import numpy as np
+import pytest
+
+from hachiue_amd import Sampler, SamplerError, hip
+from hachiue_amd import sampler as hs
+from tests.serving_util import Graph, dev
+from tests.test_gpu_lora import Adapters, check
+from tests.test_oracle_lmhead import random_blocks
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"q6_k": 14, "q4_k": 12, "q4_0": 2, "f32": 0}
+
+
+class Projection:
+    """Weights, adapters and rows of one gemv_lora_device call."""
+
+    def __init__(self, fmt, hadamard, M, K=1024, N=3001, seed=50):
+        rng = np.random.default_rng(seed + M)
+        if fmt == "f32":
+            raw = (rng.standard_normal((N, K)) / 32).astype(np.float32).view(np.uint8)
+        else:
+            raw = random_blocks(TYPES[fmt], N, K, rng)
+        self.M, self.K, self.N = M, K, N
+        self.dw = dev(np.ascontiguousarray(raw).reshape(-1))
+        self.w = hs.weights(TYPES[fmt], N, K, self.dw.addr, None, hadamard, None)
+        self.ad = Adapters(rng, "f16", 3, 12, K, N)
+        self.x, self.slots = rng.standard_normal((M, K)).astype(np.float32), rng.integers(-1, 3, M).astype(np.int32)
+        self.dx, self.ds = dev(self.x), dev(self.slots)
+        self.y, self.plain = hip.DeviceArray((M, N), np.float32), hip.DeviceArray((M, N), np.float32)
+
+    def gemv(self, ctx, st):
+        ctx.gemv_device_ex(self.dx.addr, self.M, self.K, self.w, self.plain.addr, self.N, stream=st)
+
+    def both(self, ctx, st):
+        ctx.gemv_lora_device(self.dx.addr, self.M, self.K, self.w, self.ad.desc, self.ds.addr, self.y.addr,
+                             self.N, stream=st)
+
+    def check(self, ctx, st):
+        """The eager calls of a context, one after the other, are right."""
+        for _ in range(3):
+            self.y.upload(np.zeros((self.M, self.N), np.float32))
+            self.plain.upload(np.zeros((self.M, self.N), np.float32))
+            hip.synchronize()
+            self.gemv(ctx, st)
+            self.both(ctx, st)
+            st.synchronize()
+            check(self.ad, self.x, self.slots, self.plain.download(), self.y.download())
+        return self.y.download()
+
+
+def refused(call, *args):
+    with pytest.raises(SamplerError) as e:
+        call(*args)
+    assert e.value.status == 4, str(e.value)
+    return str(e.value)
+
+
+@pytest.mark.parametrize("mode", [0, 2])          # global, relaxed
+@pytest.mark.parametrize("fmt,hadamard,M", [("q6_k", False, 1), ("q4_k", False, 2), ("q4_0", True, 5),
+                                            ("q6_k", True, 1)])
+def test_a_captured_first_projection_that_needs_workspace(fmt, hadamard, M, mode):
+    """Nothing is allocated or cleared in a capture: the call is refused, its
+    graph stays empty, the eager calls behind it count from zero, and once they
+    have been made the capture holds the call."""
+    p, st = Projection(fmt, hadamard, M), hip.Stream()
+    with Sampler(0) as ctx:
+        print(f"[gpu] first call captured {fmt} {hadamard} M={M} mode={mode}", flush=True)
+        for call in (p.gemv, p.both):
+            g = Graph(st, lambda call=call: pytest.fail("capture") if "capture" not in refused(call, ctx, st)
+                      else None, mode)
+            g.launch()
+            st.synchronize()
+            g.destroy()
+        want = p.check(ctx, st)
+        g = Graph(st, lambda: p.both(ctx, st), mode)
+        for _ in range(3):
+            p.y.upload(np.zeros((M, p.N), np.float32))
+            hip.synchronize()
+            g.launch()
+            st.synchronize()
+            assert np.array_equal(p.y.download().view(np.uint32), want.view(np.uint32))
+            assert np.array_equal(p.check(ctx, st).view(np.uint32), want.view(np.uint32))
+        g.destroy()
+    st.destroy()
