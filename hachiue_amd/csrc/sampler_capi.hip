@@ -1916,6 +1916,9 @@ int hs_lm_head_lora_sample_device(hs_context *ctx, const float *d_x, int32_t M, 
     return fail(HS_ERR_INVALID_ARGUMENT, "history ids and offsets must both be given or both null");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   HS_LOCK(ctx);
+  // (a graph would read the sampler's plans, which later calls rewrite)
+  if (!skip && is_capturing(st))
+    return fail(HS_ERR_UNSUPPORTED, "sampling must not be captured into a graph");
   rc = gemv_lora(ctx, d_x, M, ldx, w, d_logits, ldl, g, skip, st);
   if (rc) return rc;
   return sample_device(ctx, d_logits, M, ldl, w->rows, d_hist_ids, d_hist_offsets, configs,

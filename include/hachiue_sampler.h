@@ -453,7 +453,9 @@ int hs_gemv_lora_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ld
                         const hs_weights *w, const hs_adapters *adapters,
                         const int32_t *d_slots, float *d_y, int64_t ldy, void *stream);
 
-/* hs_lm_head_sample_device_ex with the adapters between its two steps. */
+/* hs_lm_head_sample_device_ex with the adapters between its two steps.  Not to
+ * be captured: a graph would read sampling plans that later calls rewrite (on a
+ * capturing stream: HS_ERR_UNSUPPORTED, nothing enqueued). */
 int hs_lm_head_lora_sample_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
                                   const hs_weights *w, const hs_adapters *adapters,
                                   const int32_t *d_slots, float *d_logits, int64_t ldl,

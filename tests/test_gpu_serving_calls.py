@@ -30,6 +30,8 @@ class Projection:
         self.ad = Adapters(rng, "f16", 3, 12, K, N)
         self.x, self.slots = rng.standard_normal((M, K)).astype(np.float32), rng.integers(-1, 3, M).astype(np.int32)
         self.dx, self.ds = dev(self.x), dev(self.slots)
+        self.cfg, self.u = hs.make_configs(dict(temperature=0.8, topK=30), M), dev(np.full(M, 0.5))
+        self.tok = dev(np.full(M, -7, np.int32))
         self.y, self.plain = hip.DeviceArray((M, N), np.float32), hip.DeviceArray((M, N), np.float32)
 
     def gemv(self, ctx, st):
@@ -38,6 +40,11 @@ class Projection:
     def both(self, ctx, st):
         ctx.gemv_lora_device(self.dx.addr, self.M, self.K, self.w, self.ad.desc, self.ds.addr, self.y.addr,
                              self.N, stream=st)
+
+    def sampled(self, ctx, st):
+        ctx.lm_head_lora_sample_device(self.dx.addr, self.M, self.K, self.w, self.ad.desc, self.ds.addr,
+                                       self.y.addr, self.N, None, None, self.cfg, self.u.addr, self.tok.addr,
+                                       stream=st)
 
     def check(self, ctx, st):
         """The eager calls of a context, one after the other, are right."""
@@ -85,4 +92,22 @@ def test_a_captured_first_projection_that_needs_workspace(fmt, hadamard, M, mode
             assert np.array_equal(p.y.download().view(np.uint32), want.view(np.uint32))
             assert np.array_equal(p.check(ctx, st).view(np.uint32), want.view(np.uint32))
         g.destroy()
+    st.destroy()
+
+
+def test_captured_sampling_with_adapters_is_refused():
+    """Before anything is enqueued, for a fresh context and a used one."""
+    p, st = Projection("f32", False, 5), hip.Stream()
+    with Sampler(0) as ctx:
+        for _ in range(2):
+            g = Graph(st, lambda: refused(p.sampled, ctx, st))
+            p.y.upload(np.full((p.M, p.N), 7.0, np.float32))
+            hip.synchronize()
+            g.launch()
+            st.synchronize()
+            assert (p.y.download() == 7.0).all()
+            g.destroy()
+            p.sampled(ctx, st)
+            st.synchronize()
+            assert (p.tok.download() >= 0).all()
     st.destroy()
