@@ -124,20 +124,29 @@ struct DevBuf {
 
 // Grow-only device buffer whose memory stays where it is, however it grows:
 // a captured graph keeps the addresses of its call.  (It doubles at least, so
-// what it left behind is less than what it holds.)
+// what it left behind is less than what it holds; where that much cannot be
+// had, it takes what the call needs.)
 struct KeptBuf {
   DevBuf b;
   std::vector<void *> left;
   hipError_t ensure(size_t need) {
     if (need <= b.bytes) return hipSuccess;
-    DevBuf n;
     try {
       left.reserve(left.size() + 1);   // (before anything is allocated)
     } catch (const std::bad_alloc &) {
       return hipErrorOutOfMemory;
     }
-    const hipError_t e = n.ensure(need > 2 * b.bytes ? need : 2 * b.bytes);
-    if (e != hipSuccess) return e;
+    DevBuf n;
+    for (size_t bytes : {std::max(need + need / 4, 2 * b.bytes), need}) {
+      const hipError_t e = inject_failure() ? hipErrorOutOfMemory : hipMalloc(&n.p, bytes);
+      if (e == hipSuccess) {
+        n.bytes = bytes;
+        break;
+      }
+      n.p = nullptr;
+      (void)hipGetLastError();   // (reported here: a later launch does not report it again)
+      if (e != hipErrorOutOfMemory || bytes == need) return e;
+    }
     if (b.p) left.push_back(b.p);
     b = n;
     return hipSuccess;
@@ -1585,9 +1594,9 @@ int hs_context_create(int device, hs_context **out) {
   if (e == hipSuccess) e = ctx->gemv_tab.ensure(hs::kBatchWorkBytes);
   if (e == hipSuccess) e = hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking);
   // (a first call may be captured: up to these sizes it needs no allocation)
-  if (e == hipSuccess) e = ctx->verify_ws.ensure(kVerifyWorkBytes);
-  if (e == hipSuccess) e = ctx->verify_cnt.ensure(kVerifyCountBytes);
-  if (e == hipSuccess) e = ctx->lora_t.ensure(kLoraWorkBytes);
+  if (e == hipSuccess) e = ctx->verify_ws.b.ensure(kVerifyWorkBytes);
+  if (e == hipSuccess) e = ctx->verify_cnt.b.ensure(kVerifyCountBytes);
+  if (e == hipSuccess) e = ctx->lora_t.b.ensure(kLoraWorkBytes);
   if (e == hipSuccess)
     e = hs::launch_fill_u32(static_cast<uint32_t *>(ctx->verify_cnt.b.p),
                             (int64_t)(ctx->verify_cnt.b.bytes / sizeof(uint32_t)), 0u, ctx->stream);

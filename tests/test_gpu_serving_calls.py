@@ -1,16 +1,27 @@
 """The calls around drafted tokens and adapters that the contexts' workspaces
 decide: captured first calls, allocations that fail, results that depend on
 how a call is cut."""
+import gc
+
 import numpy as np
 import pytest
 
 from hachiue_amd import Sampler, SamplerError, hip
 from hachiue_amd import sampler as hs
-from tests.serving_util import Graph, dev
-from tests.test_gpu_lora import Adapters, check
+from tests.conftest import _context
+from tests.serving_util import Drafts, Graph, dev, expected, random_case, verify
+from tests.test_gpu_lora import Adapters, check, run
 from tests.test_oracle_lmhead import random_blocks
 
 pytestmark = pytest.mark.gpu
+
+@pytest.fixture(autouse=True)
+def nothing_left():
+    """No array that only a traceback still holds is left to be collected, and
+    so freed, in a later capture."""
+    yield
+    gc.collect()
+
 
 TYPES = {"q6_k": 14, "q4_k": 12, "q4_0": 2, "f32": 0}
 
@@ -62,8 +73,18 @@ class Projection:
 def refused(call, *args):
     with pytest.raises(SamplerError) as e:
         call(*args)
-    assert e.value.status == 4, str(e.value)
-    return str(e.value)
+    assert e.value.status == 4 and "capture" in str(e.value), str(e.value)
+
+
+def captured(st, call, mode=0):
+    """The call's graph.  (An array of an earlier test that is collected, and so
+    freed, while a stream is captured would end the capture.)"""
+    gc.collect()
+    gc.disable()
+    try:
+        return Graph(st, call, mode)
+    finally:
+        gc.enable()
 
 
 @pytest.mark.parametrize("mode", [0, 2])          # global, relaxed
@@ -77,13 +98,12 @@ def test_a_captured_first_projection_that_needs_workspace(fmt, hadamard, M, mode
     with Sampler(0) as ctx:
         print(f"[gpu] first call captured {fmt} {hadamard} M={M} mode={mode}", flush=True)
         for call in (p.gemv, p.both):
-            g = Graph(st, lambda call=call: pytest.fail("capture") if "capture" not in refused(call, ctx, st)
-                      else None, mode)
+            g = captured(st, lambda call=call: refused(call, ctx, st), mode)
             g.launch()
             st.synchronize()
             g.destroy()
         want = p.check(ctx, st)
-        g = Graph(st, lambda: p.both(ctx, st), mode)
+        g = captured(st, lambda: p.both(ctx, st), mode)
         for _ in range(3):
             p.y.upload(np.zeros((M, p.N), np.float32))
             hip.synchronize()
@@ -100,7 +120,7 @@ def test_captured_sampling_with_adapters_is_refused():
     p, st = Projection("f32", False, 5), hip.Stream()
     with Sampler(0) as ctx:
         for _ in range(2):
-            g = Graph(st, lambda: refused(p.sampled, ctx, st))
+            g = captured(st, lambda: refused(p.sampled, ctx, st))
             p.y.upload(np.full((p.M, p.N), 7.0, np.float32))
             hip.synchronize()
             g.launch()
@@ -111,3 +131,47 @@ def test_captured_sampling_with_adapters_is_refused():
             st.synchronize()
             assert (p.tok.download() >= 0).all()
     st.destroy()
+
+
+# ---- allocations that fail
+
+def test_room_for_the_call_alone():
+    """A workspace that cannot have twice its size takes what the call needs;
+    one that cannot have that either says so, and the call behind it works."""
+    rng = np.random.default_rng(60)
+    ad = Adapters(rng, "bf16", 2, 200, 16, 8)
+    x = rng.standard_normal((5000, 16)).astype(np.float32)
+    # the checked calls of a first call that grows: the growth, then the two
+    # sizes that it asks for
+    for n, grows in ((1, True), (0, False)):
+        with _context({"HS_INJECT_HIP_FAILURE": str(n)}) as ctx:
+            print(f"[gpu] the larger allocation fails ({n})", flush=True)
+            if grows:
+                y, b = run(ctx, ad, x, [1] * 5000)
+                check(ad, x[-40:], [1] * 40, b[-40:], y[-40:])
+            else:
+                with pytest.raises(SamplerError) as e:
+                    run(ctx, ad, x, [1] * 5000)
+                assert e.value.status == 2
+            x2 = rng.standard_normal((9000, 16)).astype(np.float32)
+            y, b = run(ctx, ad, x2, [1] * 9000)
+            check(ad, x2[-40:], [1] * 40, b[-40:], y[-40:])
+    _context({"HS_INJECT_HIP_FAILURE": "-1"}).close()
+
+
+def test_an_allocation_that_the_card_refuses():
+    """A workspace larger than the card has: the call reports it, once, and the
+    next call's launches do not report it again."""
+    rng = np.random.default_rng(61)
+    ad = Adapters(rng, "bf16", 1, 4, 8, 6)
+    x = rng.standard_normal((3, 8)).astype(np.float32)
+    big = hs.draft_batch(65535, 63, 65535 * 63, None, ad.arr[0].addr, ad.arr[0].addr, ad.arr[0].addr,
+                         ad.arr[0].addr)
+    rows = hs.distribution(hs.DIST_LOGITS, ad.arr[0].addr, 1 << 28)
+    with Sampler(0) as ctx:
+        print("[gpu] a workspace of 8 TB", flush=True)
+        with pytest.raises(SamplerError) as e:     # (131072 parts of 16 bytes a row)
+            ctx.verify_drafts_device(rows, None, 1 << 28, big)
+        assert e.value.status == 2
+        y, b = run(ctx, ad, x, [0, 0, -1])
+        check(ad, x, [0, 0, -1], b, y)
