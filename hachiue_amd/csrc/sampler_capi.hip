@@ -498,8 +498,11 @@ int ensure_zeroed(DevBuf &b, size_t need, hipStream_t stream) {
   return HS_OK;
 }
 
+// The same where the memory stays: a failed clear drops the new buffer and goes
+// back to the one that was there.
 int ensure_zeroed(KeptBuf &k, size_t need, hipStream_t stream) {
   if (k.b.bytes >= need) return HS_OK;
+  const DevBuf old = k.b;
   HS_HIP(k.ensure(need));
   const hipError_t e = inject_failure()
                            ? hipErrorOutOfMemory
@@ -507,6 +510,8 @@ int ensure_zeroed(KeptBuf &k, size_t need, hipStream_t stream) {
                                                  (int64_t)(k.b.bytes / sizeof(uint32_t)), 0u, stream);
   if (e != hipSuccess) {
     k.b.release();
+    if (old.p) k.left.pop_back();
+    k.b = old;
     return fail(HS_ERR_HIP, "clearing the counters failed: %s", hipGetErrorString(e));
   }
   return HS_OK;

@@ -175,3 +175,51 @@ def test_an_allocation_that_the_card_refuses():
         assert e.value.status == 2
         y, b = run(ctx, ad, x, [0, 0, -1])
         check(ad, x, [0, 0, -1], b, y)
+
+
+def test_whatever_fails_leaves_the_counters_that_were_there():
+    """Every checked call of a batch that makes the counters grow fails in turn
+    (the clearing of the new ones among them): a captured call of a size that
+    the context has from its creation goes on, and so does the large one."""
+    rng = np.random.default_rng(62)
+    V, lens, many = 3001, [3, 1, 0, 2], [8] * 600
+    t, d, ids, u = random_case(rng, lens, V)
+    total = sum(many)
+    big_t = (rng.standard_normal((40, 300)) * 2).astype(np.float32)
+    small, st = Drafts(lens, ids, u), hip.Stream()
+    dt, dd = dev(t), dev(d)
+    td, qd = hs.distribution(0, dt.addr, V), hs.distribution(0, dd.addr, V)
+    row = np.arange(total + 600) % 40
+    failures = 0
+    for n in range(16):
+        big = Drafts(many, rng.integers(0, 300, total), rng.random(total + 600))
+        print(f"[gpu] verify, injected failure {n}", flush=True)
+        with _context({"HS_INJECT_HIP_FAILURE": str(n)}) as ctx:
+            try:
+                live = verify(ctx, big, 300, big_t[row], None)
+                injected = False
+            except SamplerError as e:
+                injected = True
+                assert e.status == 2, str(e)
+            hip.synchronize()
+            small.tokens.upload(np.full(small.tokens.shape, -77, np.int32))
+            hip.synchronize()
+            g = captured(st, lambda: ctx.verify_drafts_device(td, qd, V, small.desc, stream=st))
+            for _ in range(2):
+                g.launch()
+                st.synchronize()
+                small.check(expected(small, t, d), f"captured after {n}")
+            live = verify(ctx, big, 300, big_t[row], None)
+            hip.synchronize()
+            big.check(expected(big, big_t[row], None), f"large after {n}")
+            g.launch()
+            st.synchronize()
+            small.check(expected(small, t, d), f"replayed behind {n}")
+            g.destroy()
+            del live
+        if not injected and n > 4:
+            break
+        failures += injected
+    _context({"HS_INJECT_HIP_FAILURE": "-1"}).close()
+    assert failures >= 2, failures      # the counters' growth, their clearing
+    st.destroy()
