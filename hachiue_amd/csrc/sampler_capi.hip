@@ -499,8 +499,9 @@ int ensure_zeroed(DevBuf &b, size_t need, hipStream_t stream) {
 }
 
 // The same where the memory stays: a failed clear drops the new buffer and goes
-// back to the one that was there.
-int ensure_zeroed(KeptBuf &k, size_t need, hipStream_t stream) {
+// back to the one that was there.  The clear counts as a call of its own: if
+// the rest of this one fails, the next call, on whatever stream, comes behind it.
+int ensure_zeroed(hs_context *ctx, KeptBuf &k, size_t need, hipStream_t stream) {
   if (k.b.bytes >= need) return HS_OK;
   const DevBuf old = k.b;
   HS_HIP(k.ensure(need));
@@ -508,13 +509,14 @@ int ensure_zeroed(KeptBuf &k, size_t need, hipStream_t stream) {
                            ? hipErrorOutOfMemory
                            : hs::launch_fill_u32(static_cast<uint32_t *>(k.b.p),
                                                  (int64_t)(k.b.bytes / sizeof(uint32_t)), 0u, stream);
-  if (e != hipSuccess) {
+  const int rc = e == hipSuccess ? leave_stream(ctx, stream, false)
+                                 : fail(HS_ERR_HIP, "clearing the counters failed: %s", hipGetErrorString(e));
+  if (rc) {
     k.b.release();
     if (old.p) k.left.pop_back();
     k.b = old;
-    return fail(HS_ERR_HIP, "clearing the counters failed: %s", hipGetErrorString(e));
   }
-  return HS_OK;
+  return rc;
 }
 
 // Whether `s` is being captured.  Such a call neither waits for the context's
@@ -888,7 +890,7 @@ int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const 
     int rc = kept_room(ctx->gemv_part, slots * 16 * sizeof(float), cap);
     if (rc) return rc;
     if (cap) rc = kept_room(ctx->gemv_cnt, slots * sizeof(uint32_t), cap);
-    else rc = ensure_zeroed(ctx->gemv_cnt, slots * sizeof(uint32_t), stream);
+    else rc = ensure_zeroed(ctx, ctx->gemv_cnt, slots * sizeof(uint32_t), stream);
     if (rc) return rc;
     g.part = static_cast<float *>(ctx->gemv_part.b.p);
     g.tile_cnt = static_cast<uint32_t *>(ctx->gemv_cnt.b.p);
@@ -962,7 +964,10 @@ int gemv_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const
   if (rc || skip) return rc;   // nothing was enqueued
   hipEvent_t *ev = nullptr;
   if (!cap) rc = timed_slot(ctx, hs::kGemvTimedSlot, &ev);
-  if (rc) return rc;
+  if (rc) {
+    if (g.x != d_x) (void)leave_stream(ctx, stream, false);   // the rotation was enqueued
+    return rc;
+  }
   const hipError_t e = hs::launch_gemv(g, stream, ev, cap ? nullptr : ctx->done_ev);
   if (e != hipSuccess) {
     if (!cap) (void)leave_stream(ctx, stream, false);
@@ -1330,7 +1335,7 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
   if (!cap) rc = enter_stream(ctx, stream);
   if (rc) return rc;
   if (cap) rc = kept_room(ctx->verify_cnt, counts * sizeof(uint32_t), cap);
-  else rc = ensure_zeroed(ctx->verify_cnt, counts * sizeof(uint32_t), stream);
+  else rc = ensure_zeroed(ctx, ctx->verify_cnt, counts * sizeof(uint32_t), stream);
   if (rc) return rc;
   char *ws = static_cast<char *>(ctx->verify_ws.b.p);
   for (int i = 0; i < 2; ++i)

@@ -135,6 +135,11 @@ def test_captured_sampling_with_adapters_is_refused():
 
 # ---- allocations that fail
 
+def _reset():
+    """A context created with injection off resets the process-wide counter."""
+    _context({"HS_INJECT_HIP_FAILURE": "-1"}).close()
+
+
 def test_room_for_the_call_alone():
     """A workspace that cannot have twice its size takes what the call needs;
     one that cannot have that either says so, and the call behind it works."""
@@ -156,7 +161,7 @@ def test_room_for_the_call_alone():
             x2 = rng.standard_normal((9000, 16)).astype(np.float32)
             y, b = run(ctx, ad, x2, [1] * 9000)
             check(ad, x2[-40:], [1] * 40, b[-40:], y[-40:])
-    _context({"HS_INJECT_HIP_FAILURE": "-1"}).close()
+    _reset()
 
 
 def test_an_allocation_that_the_card_refuses():
@@ -220,6 +225,46 @@ def test_whatever_fails_leaves_the_counters_that_were_there():
         if not injected and n > 4:
             break
         failures += injected
-    _context({"HS_INJECT_HIP_FAILURE": "-1"}).close()
+    _reset()
     assert failures >= 2, failures      # the counters' growth, their clearing
     st.destroy()
+
+
+def test_the_next_stream_comes_behind_a_call_that_failed():
+    """A timed call whose events cannot be made has cleared the counters, or
+    rotated its rows, already: the next call on another stream waits for that."""
+    rng = np.random.default_rng(63)
+    total = 8 * 600
+    rows = (rng.standard_normal((40, 300)) * 2).astype(np.float32)[np.arange(total + 600) % 40]
+    a, b = hip.Stream(), hip.Stream()
+    p = Projection("q4_0", True, 5)
+    with Sampler(0) as ctx:
+        want = p.check(ctx, a)
+    verified = rotated = 0
+    for n in range(12):
+        big = Drafts([8] * 600, rng.integers(0, 300, total), rng.random(total + 600))
+        print(f"[gpu] two streams, injected failure {n}", flush=True)
+        with _context({"HS_INJECT_HIP_FAILURE": str(n)}) as ctx:
+            ctx.set_timing(True)
+            try:
+                live = [verify(ctx, big, 300, rows, None, stream=a)]
+            except SamplerError:
+                verified += 1
+            _reset()
+            live = [verify(ctx, big, 300, rows, None, stream=b)]
+            hip.synchronize()
+            big.check(expected(big, rows, None), f"behind failure {n}")
+        with _context({"HS_INJECT_HIP_FAILURE": str(n)}) as ctx:
+            ctx.set_timing(True)
+            try:
+                p.both(ctx, a)
+            except SamplerError:
+                rotated += 1
+            _reset()
+            p.both(ctx, b)
+            b.synchronize()
+            assert np.array_equal(p.y.download().view(np.uint32), want.view(np.uint32)), n
+        del live
+    assert verified >= 4 and rotated >= 4, (verified, rotated)
+    for st in (a, b):
+        st.destroy()
