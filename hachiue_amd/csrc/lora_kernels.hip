@@ -65,7 +65,10 @@ struct alignas(16) Lane {
 // the next 8, the last 8; below 2^-110 the last may underflow): its products
 // with a bfloat16 are then three bfloat16 products, which the matrix cores
 // sum in binary32 at sixteen times the rate of binary32 ones.  An infinity is
-// one part, a NaN stays one.  (2048 rows x 4096, rank 64: 42 us a call, 55 with
+// one part, a NaN stays one; where the bfloat16 value is infinite, the lower parts,
+// which are 0 in values of few bits, meet its largest finite neighbour instead
+// (0 times an infinity is NaN; the parts have one sign, so that the sum is the
+// leading part's infinity).  (2048 rows x 4096, rank 64: 42 us a call, 55 with
 // binary32 products.  A binary16 value is two bfloat16 ones, which would have to
 // be parted in every workgroup that reads it: twice the products and that.)
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -112,6 +115,35 @@ __device__ __forceinline__ Parts<n> parts_of(const float (&x)[n]) {
     for (int j = 0; j < 3; ++j) p[j].u[i / 2] = __builtin_amdgcn_perm(u[j][1], u[j][0], 0x07060302u);
   }
   return {{p[0].v, p[1].v, p[2].v}};
+}
+
+// bfloat16 values with the largest finite ones in place of infinities (and NaN,
+// which the leading part's product keeps).
+template <typename V>
+__device__ __forceinline__ V finite_of(V a) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  union {
+    V v;
+    u16x2 u[sizeof(V) / 4];
+  } r;
+  r.v = a;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(V) / 4); ++i) {
+    // as unsigned numbers the negative ones are the larger, as signed the positive
+    const u16x2 n = __builtin_elementwise_min(r.u[i], (u16x2)(unsigned short)0xFF7F);
+    r.u[i] = __builtin_bit_cast(u16x2, __builtin_elementwise_min(__builtin_bit_cast(i16x2, n), (i16x2)(short)0x7F7F));
+  }
+  return r.v;
+}
+// acc += x w (or w x: SWAP) of x in parts, the lower ones first.
+template <bool SWAP, int n>
+__device__ __forceinline__ f32x4 mfma_parts(const Parts<n> &x, typename Operand<n>::V w, f32x4 acc) {
+  const typename Operand<n>::V f = finite_of(w);
+#pragma unroll
+  for (int i = 2; i >= 0; --i)
+    acc = SWAP ? mfma_bf16(i ? f : w, x.v[i], acc) : mfma_bf16(x.v[i], i ? f : w, acc);
+  return acc;
 }
 
 // The adapter of the tile's row `lane & 15`, -1: none.
@@ -225,9 +257,7 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void lora_shrink_kernel(LoraArgs
 #pragma unroll
         for (int j = 0; j < JB; ++j) {
           const bf16x8 av = *reinterpret_cast<const bf16x8 *>(&lds.in.a[16 * j + i16][kk]);
-#pragma unroll
-          for (int i = 2; i >= 0; --i)
-            acc[j] = mfma_bf16(xp.v[i], av, acc[j]);
+          acc[j] = mfma_parts<false>(xp, av, acc[j]);
         }
         return;
       }
@@ -390,9 +420,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs
 #pragma unroll
               for (int i = 0; i < VK; ++i) b[n].v[i].u = k + i < rank ? b[n].v[i].u : (uint16_t)0;
             }
-            const auto w = __builtin_bit_cast(typename Operand<VK>::V, b[n]);
-#pragma unroll
-            for (int i = 2; i >= 0; --i) acc[n] = mfma_bf16(w, tp[r].v[i], acc[n]);
+            acc[n] = mfma_parts<true>(tp[r], __builtin_bit_cast(typename Operand<VK>::V, b[n]), acc[n]);
           }
           continue;
         }
@@ -525,9 +553,7 @@ __global__ __launch_bounds__(256, 3) void lora_expand_wide_kernel(LoraArgs g) {
         for (int n = 0; n < 4; ++n) {
           const bf16x8 b =
               *reinterpret_cast<const bf16x8 *>(&lds.in.b[wave * 64 + 16 * n + i16][k + grp * 8]);
-#pragma unroll
-          for (int i = 2; i >= 0; --i)
-            acc[n] = mfma_bf16(b, tp.v[i], acc[n]);
+          acc[n] = mfma_parts<true>(tp, b, acc[n]);
         }
         continue;
       }
