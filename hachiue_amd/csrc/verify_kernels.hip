@@ -70,18 +70,17 @@ __device__ __forceinline__ bool arrive(uint32_t *cnt, uint32_t of, int32_t *last
   return *last != 0;
 }
 
-// 2^d for d <= 0 (NaN: 0), to 2.2e-12.  n = round(d), 2^(d - n) by a polynomial
-// 1 + f g(f), g the Chebyshev interpolant of (2^f - 1) / f of degree 7 on
-// [-1/2, 1/2].  Exact at whole d.  (A step of a running sum over a vocabulary is
-// 1e-5 of the whole on average, and 64 draws in 10^7 fall within 2.2e-12 of
-// one of 151936; a degree less would make that one call in some hundred.
-// Rounding, scaling and conversions take no longer than a multiplication here.)
+// 2^d for d <= 0 (NaN: 0), to 1.1 2^-53.  n = round(d), 2^(d - n) by a polynomial
+// 1 + f g(f), g the Chebyshev interpolant of (2^f - 1) / f of degree 10 on
+// [-1/2, 1/2] (2.0e-17 off; a degree less 5.7e-16).  Exact at whole d.
+// Rounding, scaling and conversions take no longer than a multiplication here.
 // Four at a time, step by step: a multiplication's result is ready after some
 // three issue slots of a wave, and a wave alone on its SIMD would wait for each.
 template <int N>
 __device__ __forceinline__ void exp2_neg(double (&d)[N]) {
-  constexpr double coef[8] = {0x1.63b2d7971923fp-20, 0x1.00c0e4e15189cp-16, 0x1.4308c7183d6a2p-13, 0x1.5d877598350dep-10,
-                              0x1.3b2ab70ad2565p-7, 0x1.c6b08da70cce3p-5, 0x1.ebfbdff82a734p-3, 0x1.62e42fef9cc69p-1};
+  constexpr double coef[11] = {0x1.e9d3fe3952179p-32, 0x1.e6063f7217bc6p-28, 0x1.b524fae627834p-24, 0x1.62bfd47773353p-20,
+                               0x1.ffcbfc670dcd4p-17, 0x1.430913096fd9fp-13, 0x1.5d87fe78a5276p-10, 0x1.3b2ab6fba1ddap-7,
+                               0x1.c6b08d704a0c2p-5,  0x1.ebfbdff82c598p-3,  0x1.62e42fefa39efp-1};
   double n[N], g[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -91,7 +90,7 @@ __device__ __forceinline__ void exp2_neg(double (&d)[N]) {
     g[i] = coef[0];
   }
 #pragma unroll
-  for (int k = 1; k < 8; ++k)
+  for (int k = 1; k < 11; ++k)
 #pragma unroll
     for (int i = 0; i < N; ++i) g[i] = __builtin_fma(g[i], d[i], coef[k]);
 #pragma unroll
@@ -650,7 +649,7 @@ __device__ __forceinline__ Outcome outcome_of(const VerifyArgs &a, int b, const 
 // rejection does not count, whatever is made of it.)
 // ALONE: no draft rows.  The workgroup that completes a sequence's last
 // position then writes its outcome; otherwise verify_final_kernel does.
-// Bound: memory and the binary64 units together (a weight is 14 binary64
+// Bound: memory and the binary64 units together (a weight is 17 binary64
 // operations of 5.6 cycles a wave), at the small end the chain load -> sum ->
 // count in -> join.  A logit is read once: the sums are under each part's own
 // maximum and meet under the row's.  Over rows of 151936 logits: 64 sequences
