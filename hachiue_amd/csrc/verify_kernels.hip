@@ -555,14 +555,17 @@ __device__ __forceinline__ int draw_id(const VerifyArgs &a, const Final &f, int 
 // workgroups published (no draft rows to take off), by a whole workgroup.  A
 // rejected certain draft's own probability px is taken off its part's sum;
 // where little of the sum is left, so that the difference would keep less
-// than 42 of its bits, the part is summed again without it.
+// than 42 of its bits, the part is summed again without it.  A part has mass
+// where its largest logit's own probability is not 0 (nor, without x, a sum so
+// small that its ids' may be): a draw that falls to a part finds an id in it.
 template <int PER>
 __device__ __forceinline__ int draw_from_parts(const VerifyArgs &a, Final f, int64_t row, double u,
                                                double px, VerifySmem &sm) {
   const VerifyPart *part = a.part[0] + row * a.parts;
   auto sum_of = [&](int c) {
     const VerifyPart p = load_part(part + c);
-    return p.s * weight(p.m, f.p.m, f.p.c) * f.p.inv;
+    const double w = weight(p.m, f.p.m, f.p.c) * f.p.inv;
+    return w > 0.0 ? p.s * w : 0.0;
   };
   int xp = f.residual && f.x >= 0 && f.x < a.vocab ? f.x / (64 * PER) : -1;
   for (;;) {
@@ -570,7 +573,7 @@ __device__ __forceinline__ int draw_from_parts(const VerifyArgs &a, Final f, int
     if (xp >= 0) {
       const double all = sum_of(xp);
       without = all - px;
-      if (!(without >= all * 0x1p-10)) without = part_mass<PER>(a, f, xp);   // (each wave the same)
+      if (!(without >= fmax(all * 0x1p-10, 0x1p-1000))) without = part_mass<PER>(a, f, xp);   // (each wave the same)
     }
     const int id =
         draw_id<PER>(a, f, a.parts, u, [&](int c) { return c == xp ? without : sum_of(c); }, sm);

@@ -133,3 +133,23 @@ def test_acceptance_beside_its_step(sampler, draft):
     counts = b.outputs()[1]
     assert n > 100 and np.array_equal(counts, want), int((counts != np.array(want)).sum())
     del keep
+
+
+@pytest.mark.parametrize("draft", [None, 1500, 700, 2999])
+def test_a_uniform_of_0_where_weights_underflow(sampler, draft):
+    """A part whose sum is a denormal number while each of its ids' probabilities
+    rounds to 0: u = 0 takes the first id that has one, never a masked id."""
+    V, low = 3000, np.float32(-744.2)          # exp: 2^-1074, a third of which is 0
+    x = np.full(V, -np.inf, np.float32)
+    x[5:1024] = low
+    x[1500:1503] = 0.0
+    x[2990:] = low
+    if draft is None:
+        b, want, rows = Drafts([0, 0], [], [0.0, 0.0], max_drafts=1, slack=2), 1500, [x, x]
+    else:      # a certain draft, rejected: what is left of p without it
+        b, rows = Drafts([1, 1], [draft] * 2, [1.0 - 2.0 ** -53, 0.0] * 2), [x] * 4
+        want = 1501 if draft == 1500 else 1500
+    live = verify(sampler, b, V, np.stack(rows), None)
+    hip.synchronize()
+    assert [int(r[0]) for r in b.outputs()[0]] == [want] * 2
+    del live
