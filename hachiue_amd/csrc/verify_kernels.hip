@@ -706,9 +706,10 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
         rej = (int)load_agent32(a.rejected + b);
         load_part_of<PER>(rowp, part + a.split * kWavesV, a.vocab, next);
       }
+      // (a maximum passes a quiet NaN over, but makes a signalling one its result)
       float m = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < PER; ++i) m = fmaxf(m, v[i / 4].v[i % 4]);
+      for (int i = 0; i < PER; ++i) m = fmaxf(m, __builtin_canonicalizef(v[i / 4].v[i % 4]));
       VerifyPart out;
       out.m = wave_max(m);
       out.s = 0.0;
