@@ -14,7 +14,9 @@
 // its rows name and each row keeps the result of its own: rows of one prompt
 // follow each other and share one pass, a batch with an adapter per row reads
 // each adapter once.  No sorting, and a row's result does not depend on its
-// neighbours: an infinity or NaN in one adapter or row reaches no other.
+// neighbours: an infinity or NaN in one adapter or row reaches no other.  It
+// does depend on how many rows there are: the shares of K and the kernel of the
+// second product go by M, and with them the order of the binary32 sums.
 #include "sampler_internal.h"
 
 #include <hip/hip_ext.h>

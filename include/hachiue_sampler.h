@@ -426,7 +426,10 @@ int hs_verify_candidates_device(hs_context *ctx, const hs_candidates *target,
  * B [count][rows][rank] are stacked device arrays of F32 (0), F16 (1) or BF16
  * (30) elements, aligned as such; adapter s uses the first ranks[s] ranks of its stack
  * (rank where ranks is NULL), and nothing behind them matters.  x, base and y
- * are binary32; the products are summed in binary32. */
+ * are binary32; the products are summed in binary32, in an order that depends on
+ * the call's sizes: a row's result is the same whatever rows and adapters are
+ * beside it, but may differ by rounding between calls of different M.  With BF16
+ * adapters, bits of x and of scales[s] * x A_s^T below 2^-126 may count as 0. */
 typedef struct hs_adapters {
   int32_t type;                /* GGML type id: 0, 1 or 30 */
   int32_t count;

@@ -268,3 +268,26 @@ def test_the_next_stream_comes_behind_a_call_that_failed():
     assert verified >= 4 and rotated >= 4, (verified, rotated)
     for st in (a, b):
         st.destroy()
+
+
+# ---- how a call is cut
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_a_row_in_calls_of_other_sizes(sampler, kind):
+    """Four, three, two and one shares of K (1, 1100, 1400 and 4200 rows at rank
+    64) and the second product through LDS (from 384 workgroups on) or not: each
+    within the bound of binary32 sums, and the same bits for the same size."""
+    rng = np.random.default_rng(80)
+    K, N = 4096, 600
+    ad = Adapters(rng, kind, 3, 64, K, N)
+    x = rng.standard_normal((4200, K)).astype(np.float32)
+    slots = rng.integers(-1, 3, 4200).astype(np.int32)
+    slots[0] = 2
+    for M in (1, 17, 1100, 1400, 4200):
+        y, _ = run(sampler, ad, x[:M], slots[:M], None)
+        rows = np.unique(np.concatenate([[0], rng.integers(0, M, 12), [M - 1]]))
+        check(ad, x[rows], slots[rows], None, y[rows])
+        # other neighbours, the same row
+        order = np.concatenate([[0], 1 + rng.permutation(M - 1)])
+        y2, _ = run(sampler, ad, x[order], slots[order], None)
+        assert np.array_equal(y[order].view(np.uint32), y2.view(np.uint32)), M
