@@ -70,7 +70,7 @@ struct alignas(16) Lane {
 // one part, a NaN stays one; where the bfloat16 value is infinite, the lower parts,
 // which are 0 in values of few bits, meet its largest finite neighbour instead
 // (0 times an infinity is NaN; the parts have one sign, so that the sum is the
-// leading part's infinity).  (2048 rows x 4096, rank 64: 42 us a call, 55 with
+// leading part's infinity).  (2048 rows x 4096, rank 64: 42.7 us a call, 55 with
 // binary32 products.  A binary16 value is two bfloat16 ones, which would have to
 // be parted in every workgroup that reads it: twice the products and that.)
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -182,7 +182,7 @@ constexpr int kShrinkK = kShrinkWaves * 32;   // k of a stage
 // multiplied, each wave 32 of its k, lanes l, l + 16, ... 8 consecutive ones
 // each; the waves' sums meet in LDS.
 // Bound: for prompts a stage's latency (2048 rows x 4096, rank 64, bfloat16:
-// 17 us, of which 8 stages 1.4 each; x at 2 TB/s, A from L2), for a few rows that
+// 16.5 us, of which 8 stages 1.4 each; x at 2 TB/s, A from L2), for a few rows that
 // of the one chain over K (one row x 2048 4.5 us, 32 rows with an adapter each
 // 6.0).
 template <typename T, int JB>
@@ -473,7 +473,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void lora_expand_kernel(LoraArgs
 // which bounds the kernel above once a row of B is longer than a line).  The next
 // chunk (of the next adapter after an adapter's last) is on its way while
 // one is multiplied.  2048 rows x 4096 at rank 64, bfloat16:
-// 22 us, 3.1 TB/s of base and y.
+// 23 us, 2.9 TB/s of base and y.
 template <typename T>
 __global__ __launch_bounds__(256, 3) void lora_expand_wide_kernel(LoraArgs g) {
   constexpr int CH = 128 / (int)sizeof(T), PER = 16 / (int)sizeof(T);   // a chunk's ranks, a read's
@@ -646,14 +646,21 @@ hipError_t expand_by_rank(const LoraArgs &g, hipStream_t stream, hipEvent_t *ev,
 }
 
 // Through LDS where ranks fill a chunk and there are workgroups enough (each
-// takes its tile's adapters one after the other).  us of bfloat16, a lane a row
-// and through LDS:
+// takes its tile's adapters one after the other).  us, a lane a row and through
+// LDS, of bfloat16:
 //   2048 x 4096 (2048 workgroups), 8 adapters, rank 32 17, 24, rank 64 24, 21, rank
 //   128 33, 25; 512 x 4096 (512), 4 adapters, rank 64 7.1, 6.8
 //   16 x 100000 (391), 2 adapters, rank 64 8.8, 7.8, rank 128 13.5, 12; 16 adapters
 //   35, 33 and 89, 70; 64 x 32000 (500), 16 adapters, rank 83 110, 83
 //   32 x 32000 (250), 8 adapters, rank 64 13.6, 15.4; 16 x 8000 (32), 16 adapters
 //   8.9, 22.6
+// of binary16 and binary32 at the same sizes (timed with events, which add some 2):
+//   2048 x 4096: rank 32 22, 26 and 25, 22, rank 64 35, 27 and 39, 30, rank 128 50, 38
+//   and 55, 42; 512 x 4096: 11.4, 10.1 and 12.6, 9.7
+//   16 x 100000, 2 adapters: rank 64 15.1, 13.5 and 15.9, 14.5, rank 128 25, 20 and 32,
+//   29; 16 adapters: 75, 69 and 82, 87, then 146, 124 and 157, 164; 64 x 32000: 139,
+//   118 and 146, 147
+//   32 x 32000: 24, 28 and 26, 33; 16 x 8000: 16, 45 and 19, 52
 inline bool expand_wide(const LoraArgs &g) {
   return g.rank_pad >= 64 && (int64_t)((g.N + 255) / 256) * ((g.M + 15) / 16) >= 384;
 }

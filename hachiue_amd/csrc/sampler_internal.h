@@ -408,8 +408,9 @@ constexpr int kVerifyMaxDrafts = 63;     // a sequence's tokens fit one wave
 constexpr int kVerifyThreads = 256;
 // Values of a row a lane holds, 64 times which is a wave's part, the unit of the
 // sums: 32, or 16 where a call has few waves (fewer than kVerifyFew would be
-// busy), which then end sooner: 16 sequences' outcomes over 151936 logits 13.8 us
-// (15.4), but 32 sequences' 19 (14).
+// busy), which then end sooner.  us over 151936 logits, 32 and 16: 16 sequences'
+// outcomes 16.6, 14.9; 32 sequences' 20.7, 18.5 behind logits and 16.4, 21.4 behind
+// probabilities; the sums of 16 sequences of 4 drafts 35.8, 45.7.
 constexpr int kVerifyPer = 32, kVerifyPerFew = 16, kVerifyFew = 2048;
 constexpr int kVerifyMaxVocab = 1 << 28;
 constexpr int kVerifyMaxList = 4096;     // candidates of a list
@@ -483,8 +484,8 @@ inline unsigned verify_launches(const VerifyArgs &a) {
 }
 // How rows are cut.  Workgroups of a row whose logits are summed: enough that
 // all rows together give each compute unit four, but each has up to kVerifyDeep
-// turns of its four waves to itself (4 takes 5 % less than 2
-// for 64 sequences of 8 drafts over 151936 logits).
+// turns of its four waves to itself.  Sums over 151936 logits in us, 4 and 2: 16
+// sequences of 4 drafts 35.8, 44.7; 32 of 4 47.8, 45.9; 64 of 8 98.5, 91.2.
 constexpr int kVerifyDeep = 4;
 inline void verify_cut(VerifyArgs &a) {
   auto parts = [&](int per) { return (a.vocab + 64 * per - 1) / (64 * per); };

@@ -656,8 +656,8 @@ __device__ __forceinline__ Outcome outcome_of(const VerifyArgs &a, int b, const 
 // operations of 5.6 cycles a wave), at the small end the chain load -> sum ->
 // count in -> join.  A logit is read once: the sums are under each part's own
 // maximum and meet under the row's.  Over rows of 151936 logits: 64 sequences
-// of 8 drafts with draft rows 92 us (373 MB of the rows' 661, 4.0 TB/s), 16 of 4
-// 33 us (88 MB, 2.7 TB/s), one of 3 without draft rows, outcome and all, 12 us.
+// of 8 drafts with draft rows 99 us (366 MB of the rows' 661, 3.7 TB/s), 16 of 4
+// 36 us (88 MB, 2.5 TB/s), one of 3 without draft rows, outcome and all, 12 us.
 template <bool ALONE, int PER>
 __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
@@ -778,10 +778,10 @@ __global__ __launch_bounds__(kVerifyThreads, ALONE ? 3 : 4) void verify_stats_ke
 // sums what the final token is drawn from, and the one that completes the
 // row draws; without one, and logits for the target, the sums are there.
 // PER: the rows' sums', FPER: its own.
-// Bound: the final rows' second read, 78 MB for 64 sequences of 151936 logits
-// in 28.5 us (2.7 TB/s; binary64 weights of two rows an id, and a draw behind the
-// last part), 32 sequences of probabilities (39 MB) 14.2 us.  Two parts a wave in
-// turn, with half the workgroups, took 30 and 16.5 us.
+// Bound: the final rows' second read, 69 MB for 64 sequences of 151936 logits
+// in 32 us (2.1 TB/s; binary64 weights of two rows an id, and a draw behind the
+// last part), 32 sequences of probabilities (39 MB) 14 us.  Two parts a wave in
+// turn, with half the workgroups, took 5 % and 16 % longer.
 template <int PER, int FPER>
 __global__ __launch_bounds__(kVerifyThreads, 3) void verify_final_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
@@ -905,7 +905,7 @@ __device__ __forceinline__ uint32_t list_hash(int id, uint32_t mask) {
 // the list's order.  The draft's list goes into an LDS hash table of ids: a
 // look-up instead of a pass over it for each of the target's.  Bound: the chain
 // of dependent steps in one workgroup (offsets, lists, verdicts, table, sums):
-// 8 us for 256 sequences of 4 drafts over 20 candidates, 11.7 us for 32 over
+// 8 us for 256 sequences of 4 drafts over 20 candidates, 10.6 us for 32 over
 // 1024, of which an empty launch is 5.
 __global__ __launch_bounds__(kVerifyThreads) void verify_lists_kernel(ListArgs a, int bits) {
   extern __shared__ uint32_t table[];   // [2^bits] ids, [2^bits] probabilities
