@@ -4,10 +4,10 @@ device-resident buffers the way a serving loop calls them.
 Four operators:
   norm     Sampler.block_norm_device: the end of one block and the start of the
            next, s = residual + scale * act(gate) * after(x), out = before(s)
-  project  Sampler.matmul_i8_device (and, for the lm_head, Sampler.gemv_device_ex
+  project  Sampler.matmul_int_device (and, for the lm_head, Sampler.gemv_device_ex
            with int8 weights): the product in 8-bit integers with a scale for
            each token and each output channel
-  gated    Sampler.gated_i8_device: both projections of a gated feed-forward,
+  gated    Sampler.gated_int_device: both projections of a gated feed-forward,
            its activation and the product of the two
   ffn      a whole feed-forward block of them: the norm that quantises its
            tokens, the gated pair, the projection back, the norm behind it
@@ -337,17 +337,17 @@ def _calls(s):
                              after=norm("rms", s["after"]), before=norm("rms", s["next"]),
                              out=rows(s["out"]))
         return [(S.block_norm_device, (first, st)),
-                (S.gated_i8_device, (m, q, w, up, acts[c["act"]], h, st)),
-                (S.matmul_i8_device, (m, h, down, None, y, st)),
+                (S.gated_int_device, (m, q, w, up, acts[c["act"]], h, st)),
+                (S.matmul_int_device, (m, h, down, None, y, st)),
                 (S.block_norm_device, (last, st))]
     x, y = rows(s["x"], s.get("xs")), rows(s["y"])
     if c["op"] == "gated":
-        return [(S.gated_i8_device, (m, x, weights(s["w"]), weights(s["up"]), acts[c["act"]], y, st))]
+        return [(S.gated_int_device, (m, x, weights(s["w"]), weights(s["up"]), acts[c["act"]], y, st))]
     if c["head"]:
         return [(S.gemv_device_ex, (s["x"].data_ptr(), m, s["x"].shape[1], weights(s["w"]),
                                     s["y"].data_ptr(), c["n"], st))]
     bias = s["bias"].data_ptr() if c["bias"] else None
-    return [(S.matmul_i8_device, (m, x, weights(s["w"]), bias, y, st))]
+    return [(S.matmul_int_device, (m, x, weights(s["w"]), bias, y, st))]
 
 
 def run(s):
