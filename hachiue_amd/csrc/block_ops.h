@@ -1,0 +1,112 @@
+// What the kernels of a model's 8-bit block share: rows of several element
+// types, norms between blocks (norm_kernels.hip), products in 8-bit integers
+// (int8_kernels.hip).
+#pragma once
+
+#include "sampler_internal.h"
+
+#include <hip/hip_ext.h>
+
+namespace hs {
+
+// Element types of rows: GGML ids.
+constexpr int kT_F32 = 0, kT_F16 = 1, kT_I8 = 24, kT_BF16 = 30;
+constexpr int kNormTimedSlot = 17, kInt8TimedSlot = 18, kRequantTimedSlot = 19;
+constexpr int row_elem_bytes(int type) {
+  return type == kT_F32 ? 4 : type == kT_F16 || type == kT_BF16 ? 2 : type == kT_I8 ? 1 : 0;
+}
+
+// Rows of elements; an absent one has p null.
+struct RowsArg {
+  void *p;
+  int64_t ld;                // elements; 0: one row for all
+  float *scales;             // I8: a row's scale
+  int32_t type;
+};
+
+enum NormKind : int32_t { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
+enum Act : int32_t {
+  kActNone = 0, kActSilu = 1, kActGelu = 2, kActGeluTanh = 3, kActRelu = 4, kActSigmoid = 5, kActTanh = 6
+};
+struct NormArg {
+  int32_t kind;
+  float eps;
+  const float *w, *b;        // [C] or null: 1, 0
+};
+
+// s = res + scale * act(gate) * after(x); sum = s; out = before(s)
+constexpr int kNormMaxC = 32768;
+struct BlockNormArgs {
+  RowsArg x, gate, res, sum, out;
+  NormArg after, before;
+  int32_t M, C, act;
+  float scale;
+  int32_t vec;               // everything is aligned for 8 elements at a time
+};
+hipError_t launch_block_norm(const BlockNormArgs &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done);
+
+// y[m][n] = xs[m] * ws[n] * sum_k x[m][k] w[n][k] + bias[n], and with a second
+// weight act(the first's) * the second's.
+constexpr int kInt8MaxM = 1 << 20, kInt8MaxN = 1 << 24, kNormMaxM = 1 << 24;
+constexpr int kInt8MaxK = 65536;   // 2^16 * 2^14 below 2^31: the sums are exact
+struct Int8Args {
+  const int8_t *x;           // [M][ldx], 16-byte aligned rows
+  int64_t ldx;
+  const float *xs;           // [M]
+  const int8_t *w[2];        // [N][K]
+  const float *ws[2];        // [N]
+  const float *bias;         // [N] or null
+  RowsArg y;
+  int32_t M, N, K, pair, act;
+};
+hipError_t launch_int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done);
+
+#ifdef __HIPCC__
+// One launch; with events its start and end, else the end of it in `done`.
+template <typename F, typename A>
+hipError_t launch_timed(F kernel, dim3 grid, int threads, hipStream_t stream, hipEvent_t *ev, hipEvent_t done,
+                        const A &a) {
+  if (ev)
+    hipExtLaunchKernelGGL(kernel, grid, dim3(threads), 0u, stream, ev[0], ev[1], 0u, a);
+  else if (done)
+    hipExtLaunchKernelGGL(kernel, grid, dim3(threads), 0u, stream, nullptr, done, 0u, a);
+  else
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0u, stream, a);
+  return hipGetLastError();
+}
+
+// v / (1 + exp(-z)): the exponential never overflows, so that the result goes to
+// 0 as slowly as it should where z is far below 0.
+__device__ __forceinline__ float logistic(float v, float z) {
+  const float e = expf(-fabsf(z));
+  return v * (z < 0.0f ? e : 1.0f) / (1.0f + e);
+}
+
+__device__ __forceinline__ float activation(int act, float v) {
+  switch (act) {
+    case kActSilu: return logistic(v, v);
+    case kActGelu: return 0.5f * v * erfcf(v * -0.70710678f);   // (no cancellation for v << 0)
+    case kActGeluTanh:   // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u))
+      return logistic(v, 1.59576912f * fmaf(0.044715f * v * v, v, v));
+    case kActRelu: return v > 0.0f ? v : v != v ? v : 0.0f;
+    case kActSigmoid: return logistic(1.0f, v);
+    case kActTanh: return tanhf(v);
+    default: return v;
+  }
+}
+
+__device__ __forceinline__ uint16_t bits16(int type, float v) {
+  if (type == kT_F16) {
+    const _Float16 h = (_Float16)v;
+    return __builtin_bit_cast(uint16_t, h);
+  }
+  const __bf16 h = (__bf16)v;
+  return __builtin_bit_cast(uint16_t, h);
+}
+__device__ __forceinline__ float widen16(int type, uint16_t u) {
+  if (type == kT_F16) return (float)__builtin_bit_cast(_Float16, u);
+  return __uint_as_float((uint32_t)u << 16);
+}
+#endif
+
+}  // namespace hs

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "hachiue_sampler.h"
+#include "block_ops.h"
 #include "sampler_internal.h"
 
 // ---- workspace of hs_sample_batch_device_noalloc: one array per GPU, in
@@ -199,6 +200,8 @@ constexpr size_t pin_align(size_t b) { return (b + 255) / 256 * 256; }
 constexpr size_t kVerifyWorkBytes = size_t(5) << 19;
 constexpr size_t kVerifyCountBytes = size_t(16) << 10;
 constexpr size_t kLoraWorkBytes = size_t(2) << 20;
+// And for 8-bit products: 256 float rows of 8188, 64 rows of 8192 quantised results.
+constexpr size_t kInt8WorkBytes = size_t(2) << 20;
 
 // Routing of rows to kernels, uploaded next to the plans.
 struct Routing {
@@ -243,6 +246,8 @@ struct hs_context {
   int fuse = 1;
   KeptBuf verify_ws, verify_cnt;   // verification of drafts (verify_cnt: zero between calls)
   KeptBuf lora_t;               // x A^T of the adapters' rows
+  KeptBuf int8_x, int8_y;       // 8-bit products: rows quantised first (their scales behind
+                                //   them), results before they are quantised
   DevBuf minp_cand, minp_meta;  // split min-p rows' hand-over (counted in by split_cnt)
   DevBuf large_retry;           // two-pass large-k rows handed back
   DevBuf large_replay;          // slot-history replays asked for by the large-k kernel
@@ -908,6 +913,28 @@ int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const 
   return HS_OK;
 }
 
+// Start/end events of the slots of `mask` (one timed call), when timing is on:
+// slot k's are *ev + 2 k, and *ev is null otherwise.
+int timed_slots(hs_context *ctx, unsigned mask, hipEvent_t **ev) {
+  *ev = nullptr;
+  if (!ctx->timing) return HS_OK;
+  hs_context::TimedCall tc{};
+  tc.mask = mask;
+  for (int i = 0; i < 2 * hs::kTimedKernels; ++i) {
+    if (!(mask >> (i / 2) & 1u)) continue;
+    if (ctx->ev_free.empty()) {
+      hipEvent_t x;
+      HS_HIP(hipEventCreate(&x));
+      ctx->ev_free.push_back(x);
+    }
+    tc.ev[i] = ctx->ev_free.back();
+    ctx->ev_free.pop_back();
+  }
+  ctx->timed.push_back(tc);
+  *ev = ctx->timed.back().ev;
+  return HS_OK;
+}
+
 // Start/end events of timing slot `slot` for the call's one kernel, when
 // timing is on (null otherwise).
 int timed_slot(hs_context *ctx, int slot, hipEvent_t **ev) {
@@ -951,9 +978,14 @@ int timed_pair(hs_context *ctx, int first, int second, hipEvent_t **ev1, hipEven
   return HS_OK;
 }
 
+// (the 8-bit products' section)
+int int8_gemv(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *w, float *d_y,
+              int64_t ldy, hipStream_t stream);
+
 int gemv_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *wt,
                 float *d_y, int64_t ldy, hipStream_t stream) {
   if (!ctx) return fail(HS_ERR_INVALID_ARGUMENT, "null context");
+  if (wt && wt->type == hs::kT_I8) return int8_gemv(ctx, d_x, M, ldx, wt, d_y, ldy, stream);
   DeviceGuard guard(ctx->device);
   const bool cap = is_capturing(stream);
   int rc = cap ? HS_OK : enter_stream(ctx, stream);
@@ -1539,6 +1571,314 @@ int gemv_lora(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const h
   return rc || skip ? rc : lora_run(ctx, g, stream);
 }
 
+// ---- norms between blocks and 8-bit products
+
+// Rows [0, M) of `cols` elements as the memory they take: two of them overlap
+// unless one lies behind the other or, with the same distance from row to row,
+// between the other's rows.
+struct Span {
+  uintptr_t at;
+  uint64_t row, step, rows;   // bytes of a row, from row to row, rows
+  uint64_t size() const { return rows ? (rows - 1) * step + row : 0; }
+};
+Span rows_span(const hs::RowsArg &r, int64_t M, int64_t cols) {
+  const uint64_t e = (uint64_t)hs::row_elem_bytes(r.type);
+  return {reinterpret_cast<uintptr_t>(r.p), (uint64_t)cols * e, (uint64_t)r.ld * e, (uint64_t)(r.ld ? M : 1)};
+}
+bool overlap(const Span &a, const Span &b) {
+  if (!a.size() || !b.size() || a.at >= b.at + b.size() || b.at >= a.at + a.size()) return false;
+  if (a.step != b.step || a.rows < 2 || b.rows < 2) return true;
+  const uint64_t d = a.at < b.at ? b.at - a.at : a.at - b.at;
+  const uint64_t off = d % a.step, lower = a.at < b.at ? a.row : b.row, upper = a.at < b.at ? b.row : a.row;
+  return off < lower || off + upper > a.step;
+}
+
+// The checks of rows; i8: whether they may be 8-bit.
+int rows_arg(const hs_rows &r, const char *what, int64_t cols, bool i8, hs::RowsArg &a) {
+  memset(&a, 0, sizeof a);
+  const int bytes = hs::row_elem_bytes(r.type);
+  if (!bytes || (r.type == hs::kT_I8 && !i8))
+    return fail(HS_ERR_UNSUPPORTED, "%s of type %d are not supported", what, r.type);
+  if (!r.data) return fail(HS_ERR_INVALID_ARGUMENT, "%s must not be null", what);
+  if (r.stride < cols)
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s: stride %lld below %lld", what, (long long)r.stride, (long long)cols);
+  if (r.stride > (int64_t)1 << 40)
+    return fail(HS_ERR_UNSUPPORTED, "%s: stride %lld above 2^40", what, (long long)r.stride);
+  if (reinterpret_cast<uintptr_t>(r.data) % (uintptr_t)bytes || reinterpret_cast<uintptr_t>(r.scales) % 4)
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s must be aligned to their elements", what);
+  if ((r.type == hs::kT_I8) != (r.scales != nullptr))
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s: scales are for 8-bit rows, and those need them", what);
+  a.p = r.data;
+  a.ld = r.stride;
+  a.scales = r.scales;
+  a.type = r.type;
+  return HS_OK;
+}
+
+int norm_arg(const hs_norm &n, const char *what, hs::NormArg &a) {
+  memset(&a, 0, sizeof a);
+  if (n.kind < HS_NORM_NONE || n.kind > HS_NORM_LAYER)
+    return fail(HS_ERR_UNSUPPORTED, "%s: norm %d is not supported", what, n.kind);
+  a.kind = n.kind;
+  if (n.kind == HS_NORM_NONE) return HS_OK;
+  if (!(n.eps >= 0.0f)) return fail(HS_ERR_INVALID_ARGUMENT, "%s: eps %g below 0", what, (double)n.eps);
+  if ((reinterpret_cast<uintptr_t>(n.weight) | reinterpret_cast<uintptr_t>(n.bias)) & 3u)
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s: weight and bias must be 4-byte aligned", what);
+  a.eps = n.eps;
+  a.w = n.weight;
+  a.b = n.bias;
+  return HS_OK;
+}
+
+bool act_known(int32_t act) { return act >= HS_ACT_NONE && act <= HS_ACT_TANH; }
+
+// Whether a row kernel may take 8 elements at a time of each tensor.
+bool wide_rows(const hs::BlockNormArgs &g) {
+  if (g.C % 8) return false;
+  uintptr_t bits = 0;
+  for (const hs::RowsArg *r : {&g.x, &g.gate, &g.res, &g.sum, &g.out}) {
+    if (!r->p) continue;
+    // (8 8-bit elements are 8 bytes)
+    const uintptr_t b = reinterpret_cast<uintptr_t>(r->p) | (uintptr_t)(r->ld * hs::row_elem_bytes(r->type));
+    bits |= r->type == hs::kT_I8 ? b * 2 : b;
+  }
+  for (const hs::NormArg *n : {&g.after, &g.before})
+    bits |= reinterpret_cast<uintptr_t>(n->w) | reinterpret_cast<uintptr_t>(n->b);
+  return (bits & 15u) == 0;
+}
+
+// The checks of a block norm; *skip: nothing to do.
+int block_norm_args(const hs_block_norm *n, hs::BlockNormArgs &g, bool *skip) {
+  if (!n) return fail(HS_ERR_INVALID_ARGUMENT, "null norm");
+  const int64_t M = n->rows, C = n->cols;
+  if (M < 0 || C < 0) return fail(HS_ERR_INVALID_ARGUMENT, "a norm over %d x %d", n->rows, n->cols);
+  if (M > hs::kNormMaxM || C > hs::kNormMaxC)
+    return fail(HS_ERR_UNSUPPORTED, "a norm over %d x %d above 2^24 x %d", n->rows, n->cols, hs::kNormMaxC);
+  memset(&g, 0, sizeof g);
+  *skip = M == 0 || C == 0 || (!n->sum.data && !n->out.data);
+  if (*skip) return HS_OK;
+  int rc = rows_arg(n->x, "x", C, false, g.x);
+  if (!rc && n->gate.data) {
+    hs_rows gate = n->gate;
+    const bool one = gate.stride == 0;
+    if (one) gate.stride = C;
+    rc = rows_arg(gate, "gate", C, false, g.gate);
+    if (one) g.gate.ld = 0;
+    if (!rc && !act_known(n->gate_act))
+      rc = fail(HS_ERR_UNSUPPORTED, "activation %d is not supported", n->gate_act);
+  }
+  if (!rc && n->residual.data) rc = rows_arg(n->residual, "residual", C, false, g.res);
+  if (!rc && n->sum.data) rc = rows_arg(n->sum, "sum", C, false, g.sum);
+  if (!rc && n->out.data) rc = rows_arg(n->out, "out", C, true, g.out);
+  if (!rc) rc = norm_arg(n->after, "after", g.after);
+  if (!rc && n->out.data) rc = norm_arg(n->before, "before", g.before);
+  if (rc) return rc;
+  // a row is read whole before it is written: in place is fine, anything else
+  // would be read by another row's workgroup
+  for (const hs::RowsArg *o : {&g.sum, &g.out}) {
+    if (!o->p) continue;
+    const Span so = rows_span(*o, M, C);
+    for (const hs::RowsArg *i : {&g.x, &g.gate, &g.res}) {
+      if (!i->p || (i->p == o->p && i->type == o->type && i->ld == o->ld)) continue;
+      if (overlap(so, rows_span(*i, M, C))) return fail(HS_ERR_INVALID_ARGUMENT, "an output overlaps an input");
+    }
+    for (const hs::NormArg *p : {&g.after, &g.before})
+      for (const float *v : {p->w, p->b})
+        if (v && overlap(so, {reinterpret_cast<uintptr_t>(v), (uint64_t)C * 4, 0, 1}))
+          return fail(HS_ERR_INVALID_ARGUMENT, "an output overlaps a norm's parameters");
+  }
+  if (g.sum.p && g.out.p && overlap(rows_span(g.sum, M, C), rows_span(g.out, M, C)))
+    return fail(HS_ERR_INVALID_ARGUMENT, "sum overlaps out");
+  if (g.out.scales) {
+    const Span s = {reinterpret_cast<uintptr_t>(g.out.scales), (uint64_t)M * 4, 0, 1};
+    for (const hs::RowsArg *r : {&g.x, &g.gate, &g.res, &g.sum, &g.out})
+      if (r->p && overlap(s, rows_span(*r, M, C))) return fail(HS_ERR_INVALID_ARGUMENT, "scales overlap rows");
+  }
+  g.M = (int32_t)M;
+  g.C = (int32_t)C;
+  g.act = n->gate_act;
+  g.scale = n->scale;
+  g.vec = wide_rows(g);
+  return HS_OK;
+}
+
+// (the context's lock is held)
+int block_norm_run(hs_context *ctx, const hs::BlockNormArgs &g, hipStream_t stream) {
+  DeviceGuard guard(ctx->device);
+  const bool cap = is_capturing(stream);
+  hipEvent_t *ev = nullptr;
+  int rc = cap ? HS_OK : enter_stream(ctx, stream);
+  if (!rc && !cap) rc = timed_slot(ctx, hs::kNormTimedSlot, &ev);
+  if (rc) return rc;
+  const hipError_t e = inject_failure() ? hipErrorOutOfMemory
+                                        : hs::launch_block_norm(g, stream, ev, cap ? nullptr : ctx->done_ev);
+  if (e != hipSuccess) {
+    if (!cap) (void)leave_stream(ctx, stream, false);
+    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
+  }
+  return cap ? HS_OK : leave_stream(ctx, stream, ev == nullptr);
+}
+
+// A weight of an 8-bit product.
+int int8_weights(const hs_weights *w, const char *what) {
+  if (!w) return fail(HS_ERR_INVALID_ARGUMENT, "null %s", what);
+  if (w->type != hs::kT_I8) return fail(HS_ERR_UNSUPPORTED, "%s of type %d where I8 is needed", what, w->type);
+  if (w->rows < 0 || w->cols <= 0)
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s of %d x %d", what, w->rows, w->cols);
+  if (w->cols % 16) return fail(HS_ERR_INVALID_ARGUMENT, "%s: K %d is not a multiple of 16", what, w->cols);
+  if (w->cols > hs::kInt8MaxK || w->rows > hs::kInt8MaxN)
+    return fail(HS_ERR_UNSUPPORTED, "%s of %d x %d above 2^24 x 65536", what, w->rows, w->cols);
+  if (w->hadamard) return fail(HS_ERR_UNSUPPORTED, "%s of type I8 must not be Hadamard-folded", what);
+  if (w->rows && (!w->data || !w->scales16))
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s and their scales must not be null", what);
+  if ((reinterpret_cast<uintptr_t>(w->data) & 15u) || (reinterpret_cast<uintptr_t>(w->scales16) & 3u))
+    return fail(HS_ERR_INVALID_ARGUMENT, "%s must be 16-byte, their scales 4-byte aligned", what);
+  return HS_OK;
+}
+
+// An 8-bit product's kernels: the rows quantised first, the product, its
+// results quantised.
+struct Int8Call {
+  hs::Int8Args g;
+  hs::BlockNormArgs pre, post;   // M 0: not needed
+  bool skip;                     // nothing to do
+};
+
+int int8_args(int32_t M, const hs_rows *x, const hs_weights *w0, const hs_weights *w1, int32_t act,
+              const float *bias, const hs_rows *y, Int8Call &c) {
+  memset(&c, 0, sizeof c);
+  int rc = int8_weights(w0, w1 ? "gate" : "w");
+  if (!rc && w1) rc = int8_weights(w1, "up");
+  if (rc) return rc;
+  const int32_t N = w0->rows, K = w0->cols;
+  if (w1 && (w1->rows != N || w1->cols != K))
+    return fail(HS_ERR_INVALID_ARGUMENT, "gate of %d x %d and up of %d x %d", N, K, w1->rows, w1->cols);
+  if (w1 && !act_known(act)) return fail(HS_ERR_UNSUPPORTED, "activation %d is not supported", act);
+  if (M < 0) return fail(HS_ERR_INVALID_ARGUMENT, "M must be >= 0 (got %d)", M);
+  if (M > hs::kInt8MaxM) return fail(HS_ERR_UNSUPPORTED, "M %d above 2^20", M);
+  if (!x || !y) return fail(HS_ERR_INVALID_ARGUMENT, "x and y must not be null");
+  c.skip = M == 0 || N == 0;
+  if (c.skip) return HS_OK;
+  hs::RowsArg xr, yr;
+  rc = rows_arg(*x, "x", K, true, xr);
+  if (!rc) rc = rows_arg(*y, "y", N, true, yr);
+  if (rc) return rc;
+  if (xr.type == hs::kT_I8 && ((reinterpret_cast<uintptr_t>(xr.p) | (uintptr_t)xr.ld) & 15u))
+    return fail(HS_ERR_INVALID_ARGUMENT, "x in 8 bits must be 16-byte aligned, its stride a multiple of 16");
+  if (xr.type != hs::kT_I8 && K > hs::kNormMaxC)
+    return fail(HS_ERR_UNSUPPORTED, "K %d of float rows above %d", K, hs::kNormMaxC);
+  if (yr.type == hs::kT_I8 && N > hs::kNormMaxC)
+    return fail(HS_ERR_UNSUPPORTED, "%d results in 8 bits above %d", N, hs::kNormMaxC);
+  if (reinterpret_cast<uintptr_t>(bias) & 3u) return fail(HS_ERR_INVALID_ARGUMENT, "bias must be 4-byte aligned");
+  const Span out[2] = {rows_span(yr, M, N),
+                       {reinterpret_cast<uintptr_t>(yr.scales), yr.scales ? (uint64_t)M * 4 : 0, 0, 1}};
+  for (const Span &s : out) {
+    if (!s.at) continue;
+    bool bad = overlap(s, rows_span(xr, M, K)) ||
+               (xr.scales && overlap(s, {reinterpret_cast<uintptr_t>(xr.scales), (uint64_t)M * 4, 0, 1})) ||
+               (bias && overlap(s, {reinterpret_cast<uintptr_t>(bias), (uint64_t)N * 4, 0, 1}));
+    for (const hs_weights *w : {w0, w1})
+      if (w)
+        bad = bad || overlap(s, {reinterpret_cast<uintptr_t>(w->data), (uint64_t)N * (uint64_t)K, 0, 1}) ||
+              overlap(s, {reinterpret_cast<uintptr_t>(w->scales16), (uint64_t)N * 4, 0, 1});
+    if (bad) return fail(HS_ERR_INVALID_ARGUMENT, "y overlaps an input");
+  }
+  if (yr.scales && overlap(out[0], out[1])) return fail(HS_ERR_INVALID_ARGUMENT, "y overlaps its scales");
+  c.g.x = static_cast<const int8_t *>(xr.p);
+  c.g.ldx = xr.ld;
+  c.g.xs = xr.scales;
+  c.g.w[0] = static_cast<const int8_t *>(w0->data);
+  c.g.ws[0] = static_cast<const float *>(w0->scales16);
+  if (w1) {
+    c.g.w[1] = static_cast<const int8_t *>(w1->data);
+    c.g.ws[1] = static_cast<const float *>(w1->scales16);
+  }
+  c.g.bias = bias;
+  c.g.y = yr;
+  c.g.M = M;
+  c.g.N = N;
+  c.g.K = K;
+  c.g.pair = w1 != nullptr;
+  c.g.act = act;
+  if (xr.type != hs::kT_I8) {
+    c.pre.M = M;
+    c.pre.C = K;
+    c.pre.scale = 1.0f;
+    c.pre.x = xr;
+  }
+  if (yr.type == hs::kT_I8) {
+    c.post.M = M;
+    c.post.C = N;
+    c.post.scale = 1.0f;
+    c.post.out = yr;
+  }
+  return HS_OK;
+}
+
+// (the context's lock is held)
+int int8_run(hs_context *ctx, Int8Call &c, hipStream_t stream) {
+  DeviceGuard guard(ctx->device);
+  const bool cap = is_capturing(stream);
+  const int64_t M = c.g.M, K = c.g.K, ldh = (c.g.N + 7) / 8 * 8;
+  unsigned mask = 1u << hs::kInt8TimedSlot;
+  int rc = HS_OK;
+  if (c.pre.M) {
+    rc = kept_room(ctx->int8_x, (size_t)(M * K) + (size_t)M * sizeof(float), cap);
+    mask |= 1u << hs::kNormTimedSlot;
+  }
+  if (!rc && c.post.M) {
+    rc = kept_room(ctx->int8_y, (size_t)(M * ldh) * sizeof(float), cap);
+    mask |= 1u << hs::kRequantTimedSlot;
+  }
+  if (!rc && !cap) rc = enter_stream(ctx, stream);
+  hipEvent_t *ev = nullptr;
+  if (!rc && !cap) rc = timed_slots(ctx, mask, &ev);
+  if (rc) return rc;
+  auto of = [&](int slot) { return ev ? ev + 2 * slot : nullptr; };
+  const hipEvent_t done = cap ? nullptr : ctx->done_ev;
+  hipError_t e = hipSuccess;
+  if (c.pre.M) {
+    char *q = static_cast<char *>(ctx->int8_x.b.p);
+    c.pre.out.p = q;
+    c.pre.out.ld = K;
+    c.pre.out.scales = reinterpret_cast<float *>(q + M * K);
+    c.pre.out.type = hs::kT_I8;
+    c.pre.vec = wide_rows(c.pre);
+    e = inject_failure() ? hipErrorOutOfMemory : hs::launch_block_norm(c.pre, stream, of(hs::kNormTimedSlot), nullptr);
+    c.g.x = reinterpret_cast<const int8_t *>(q);
+    c.g.ldx = K;
+    c.g.xs = c.pre.out.scales;
+  }
+  if (c.post.M) {
+    c.g.y.p = ctx->int8_y.b.p;
+    c.g.y.ld = ldh;
+    c.g.y.type = hs::kT_F32;
+    c.post.x = c.g.y;
+    c.post.x.scales = nullptr;
+    c.post.vec = wide_rows(c.post);
+  }
+  if (e == hipSuccess)
+    e = inject_failure() ? hipErrorOutOfMemory
+                         : hs::launch_int8(c.g, stream, of(hs::kInt8TimedSlot), c.post.M ? nullptr : done);
+  if (e == hipSuccess && c.post.M)
+    e = inject_failure() ? hipErrorOutOfMemory
+                         : hs::launch_block_norm(c.post, stream, of(hs::kRequantTimedSlot), done);
+  if (e != hipSuccess) {
+    if (!cap) (void)leave_stream(ctx, stream, false);
+    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
+  }
+  return cap ? HS_OK : leave_stream(ctx, stream, ev == nullptr);
+}
+
+int int8_gemv(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *w, float *d_y,
+              int64_t ldy, hipStream_t stream) {
+  if (M > 65535) return fail(HS_ERR_UNSUPPORTED, "M %d above 65535", M);
+  const hs_rows x = {hs::kT_F32, ldx, const_cast<float *>(d_x), nullptr}, y = {hs::kT_F32, ldy, d_y, nullptr};
+  Int8Call c;
+  const int rc = int8_args(M, &x, w, nullptr, HS_ACT_NONE, nullptr, &y, c);
+  return rc || c.skip ? rc : int8_run(ctx, c, stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1607,6 +1947,8 @@ int hs_context_create(int device, hs_context **out) {
   if (e == hipSuccess) e = ctx->verify_ws.b.ensure(kVerifyWorkBytes);
   if (e == hipSuccess) e = ctx->verify_cnt.b.ensure(kVerifyCountBytes);
   if (e == hipSuccess) e = ctx->lora_t.b.ensure(kLoraWorkBytes);
+  if (e == hipSuccess) e = ctx->int8_x.b.ensure(kInt8WorkBytes);
+  if (e == hipSuccess) e = ctx->int8_y.b.ensure(kInt8WorkBytes);
   if (e == hipSuccess)
     e = hs::launch_fill_u32(static_cast<uint32_t *>(ctx->verify_cnt.b.p),
                             (int64_t)(ctx->verify_cnt.b.bytes / sizeof(uint32_t)), 0u, ctx->stream);
@@ -1673,6 +2015,8 @@ int hs_context_destroy(hs_context *ctx) {
     ctx->verify_ws.release();
     ctx->verify_cnt.release();
     ctx->lora_t.release();
+    ctx->int8_x.release();
+    ctx->int8_y.release();
     ctx->minp_cand.release();
     ctx->minp_meta.release();
     ctx->large_retry.release();
@@ -1783,7 +2127,7 @@ int lm_head_sample(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, co
   // 9 us (repetition penalty) slower than the GEMV and the argmax launch
   const bool sample_ok = tern || w->type == hs::kW_Q6_K || w->type == hs::kW_Q4_K;
   // (several rows whose GEMV reads the weights once for all of them: two launches)
-  bool fused = ctx->fuse && (sample_ok || ctx->fuse >= 2) && M > 0 && w->rows > 0 && configs &&
+  bool fused = ctx->fuse && (sample_ok || ctx->fuse >= 2) && w->type != hs::kT_I8 && M > 0 && w->rows > 0 && configs &&
                !hs::gemv_batched(w->type, M, w->rows, w->cols) &&
                d_uniforms && d_tokens && (d_hist_ids == nullptr) == (d_hist_offsets == nullptr);
   std::vector<hs::RowPlan> plans;
@@ -1942,6 +2286,80 @@ int hs_lm_head_lora_sample_device(hs_context *ctx, const float *d_x, int32_t M, 
   if (rc) return rc;
   return sample_device(ctx, d_logits, M, ldl, w->rows, d_hist_ids, d_hist_offsets, configs,
                        d_uniforms, d_tokens, 0, nullptr, nullptr, nullptr, nullptr, nullptr, st);
+}
+
+int hs_block_norm_device(hs_context *ctx, const hs_block_norm *norm, void *stream) {
+  hs::BlockNormArgs g;
+  bool skip = false;
+  const int rc = block_norm_args(norm, g, &skip);
+  if (rc) return rc;
+  HS_LOCK(ctx);
+  return skip ? HS_OK : block_norm_run(ctx, g, static_cast<hipStream_t>(stream));
+}
+
+int hs_matmul_int_device(hs_context *ctx, int32_t M, const hs_rows *x, const hs_weights *w,
+                        const float *bias, const hs_rows *y, void *stream) {
+  Int8Call c;
+  const int rc = int8_args(M, x, w, nullptr, HS_ACT_NONE, bias, y, c);
+  if (rc) return rc;
+  HS_LOCK(ctx);
+  return c.skip ? HS_OK : int8_run(ctx, c, static_cast<hipStream_t>(stream));
+}
+
+int hs_gated_int_device(hs_context *ctx, int32_t M, const hs_rows *x, const hs_weights *gate,
+                       const hs_weights *up, int32_t act, const hs_rows *y, void *stream) {
+  if (!up) return fail(HS_ERR_INVALID_ARGUMENT, "null up");
+  Int8Call c;
+  const int rc = int8_args(M, x, gate, up, act, nullptr, y, c);
+  if (rc) return rc;
+  HS_LOCK(ctx);
+  return c.skip ? HS_OK : int8_run(ctx, c, static_cast<hipStream_t>(stream));
+}
+
+int hs_lm_head_norm_sample_device(hs_context *ctx, const hs_block_norm *norm, const hs_weights *w,
+                                  float *d_logits, int64_t ldl, const int32_t *d_hist_ids,
+                                  const int64_t *d_hist_offsets, const hs_sample_config *configs,
+                                  const double *d_uniforms, int32_t *d_tokens, void *stream) {
+  hs::BlockNormArgs g;
+  bool skip = false;
+  int rc = block_norm_args(norm, g, &skip);
+  if (rc) return rc;
+  if (!w) return fail(HS_ERR_INVALID_ARGUMENT, "null weights");
+  const int32_t M = norm->rows;
+  if (w->cols != norm->cols)
+    return fail(HS_ERR_INVALID_ARGUMENT, "a norm over %d columns before weights of %d", norm->cols, w->cols);
+  if (M > 65535) return fail(HS_ERR_UNSUPPORTED, "M %d above 65535", M);
+  const bool i8 = norm->out.type == hs::kT_I8;
+  Int8Call c;
+  if (M > 0) {
+    if (!norm->out.data || (!i8 && norm->out.type != hs::kT_F32))
+      return fail(HS_ERR_INVALID_ARGUMENT, "the lm_head needs the norm's out in F32 or I8");
+    if (!configs || !d_uniforms || !d_tokens)
+      return fail(HS_ERR_INVALID_ARGUMENT, "configs, uniforms and tokens must not be null");
+    if ((d_hist_ids == nullptr) != (d_hist_offsets == nullptr))
+      return fail(HS_ERR_INVALID_ARGUMENT, "history ids and offsets must both be given or both null");
+    if (w->type == hs::kT_I8) {
+      const hs_rows y = {hs::kT_F32, ldl, d_logits, nullptr};
+      rc = int8_args(M, &norm->out, w, nullptr, HS_ACT_NONE, nullptr, &y, c);
+      if (rc) return rc;
+    } else if (i8) {
+      return fail(HS_ERR_INVALID_ARGUMENT, "I8 rows need weights of type I8 (type %d)", w->type);
+    }
+  }
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  HS_LOCK(ctx);
+  if (M == 0) return HS_OK;
+  // (a graph would read the sampler's plans, which later calls rewrite)
+  if (is_capturing(st)) return fail(HS_ERR_UNSUPPORTED, "sampling must not be captured into a graph");
+  rc = skip ? HS_OK : block_norm_run(ctx, g, st);
+  if (rc) return rc;
+  if (w->type != hs::kT_I8)
+    return lm_head_sample(ctx, static_cast<const float *>(norm->out.data), M, norm->out.stride, w, d_logits, ldl,
+                          d_hist_ids, d_hist_offsets, configs, d_uniforms, d_tokens, st);
+  rc = c.skip ? HS_OK : int8_run(ctx, c, st);
+  if (rc) return rc;
+  return sample_device(ctx, d_logits, M, ldl, w->rows, d_hist_ids, d_hist_offsets, configs, d_uniforms, d_tokens,
+                       0, nullptr, nullptr, nullptr, nullptr, nullptr, st);
 }
 
 // src/engine.ts:80-175 (createBlockSplitter): GGUF blocks of Q1_0 ([d][16 B

@@ -207,11 +207,11 @@ struct LaunchArgs {
 // (0 penalty pre-pass, 1 row kernel, 2 chunk kernel, 3 finalize, 4 large-k
 // kernel, 5 mid kernel, 6 GPU greedy-route argmax, 8 two-pass large-k kernel,
 // 9 the large-k slot replay, 10 the device-memory slot replay, 11 min-p kernel;
-// 7 is the lm_head GEMV, 12 to 16 the serving operators below, launched
+// 7 is the lm_head GEMV, 12 to 19 the serving operators, launched
 // apart), for the kernels that launch only:
 // launched_kernels() says which.  The large-k kernel launches whenever a row
 // has k > 1024: it also takes the rows the two-pass kernel hands back.
-constexpr int kTimedKernels = 17;
+constexpr int kTimedKernels = 20;
 inline unsigned launched_kernels(const LaunchArgs &a) {
   return (a.n_pf > 0 ? 1u : 0u) | (a.n_row > 0 ? 2u : 0u) | (a.n_chunk > 0 ? 12u : 0u) |
          (a.n_large + a.n_lfast > 0 ? 16u : 0u) | (a.n_mid > 0 ? 32u : 0u) |

@@ -39,7 +39,8 @@ EXPORTS = ("hs_abi_version", "hs_last_error", "hs_config_default", "hs_context_c
            "hs_argmax", "hs_gemv_device", "hs_gemv_device_ex", "hs_split_blocks",
            "hs_lm_head_sample_device", "hs_lm_head_sample_device_ex", "hs_decode_step_device",
            "hs_verify_drafts_device", "hs_verify_candidates_device", "hs_lora_device",
-           "hs_gemv_lora_device", "hs_lm_head_lora_sample_device",
+           "hs_gemv_lora_device", "hs_lm_head_lora_sample_device", "hs_block_norm_device",
+           "hs_matmul_int_device", "hs_gated_int_device", "hs_lm_head_norm_sample_device",
            "hs_context_set_timing", "hs_context_kernel_times")
 
 
@@ -78,6 +79,8 @@ def split_blocks(wtype: int, blocks) -> tuple[np.ndarray, np.ndarray]:
 
 def weights(wtype: int, N: int, K: int, d_data: int, d_scales16: int | None = None,
             hadamard: bool = False, d_signs: int | None = None) -> WeightsC:
+    """A weight tensor on the device.  I8 (24): N rows of K int8, d_scales16
+    their N float32 scales."""
     return WeightsC(int(wtype), int(N), int(K), 1 if hadamard else 0, d_data, d_scales16 or None,
                     d_signs or None)
 
@@ -157,6 +160,52 @@ def adapters(atype: int, count: int, rank: int, K: int, N: int, d_a: int, d_b: i
     or 30 (BF16), with a float32 scale and an int32 rank per adapter."""
     return AdaptersC(int(atype), int(count), int(rank), int(K), int(N), d_a or None, d_b or None,
                      d_scales or None, d_ranks or None)
+
+
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU, ACT_SIGMOID, ACT_TANH = range(7)
+
+
+class RowsC(ctypes.Structure):
+    """hs_rows: rows of elements, 8-bit ones with a scale each."""
+    _fields_ = [("type", ctypes.c_int32), ("stride", ctypes.c_int64), ("data", ctypes.c_void_p),
+                ("scales", ctypes.c_void_p)]
+
+
+def rows(rtype: int, d_data: int, stride: int, d_scales: int | None = None) -> RowsC:
+    """Rows of GGML type 0 (F32), 1 (F16), 30 (BF16) or 24 (I8, with a float32
+    scale per row), `stride` elements apart."""
+    return RowsC(int(rtype), int(stride), d_data or None, d_scales or None)
+
+
+class NormC(ctypes.Structure):
+    """hs_norm: a norm over a row's columns."""
+    _fields_ = [("kind", ctypes.c_int32), ("eps", ctypes.c_float), ("weight", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p)]
+
+
+def norm(kind: int = NORM_NONE, eps: float = 1e-6, d_weight: int | None = None,
+         d_bias: int | None = None) -> NormC:
+    """NORM_RMS or NORM_LAYER with float32 weight and bias (None: 1, 0), or NORM_NONE."""
+    return NormC(int(kind), float(eps), d_weight or None, d_bias or None)
+
+
+class BlockNormC(ctypes.Structure):
+    """hs_block_norm: the end of a block and the start of the next."""
+    _fields_ = [("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("x", RowsC), ("after", NormC),
+                ("gate", RowsC), ("gate_act", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("residual", RowsC), ("sum", RowsC), ("before", NormC), ("out", RowsC)]
+
+
+def block_norm(M: int, C: int, x: RowsC, residual: RowsC | None = None, scale: float = 1.0,
+               gate: RowsC | None = None, gate_act: int = ACT_NONE, after: NormC | None = None,
+               sum: RowsC | None = None, before: NormC | None = None,
+               out: RowsC | None = None) -> BlockNormC:
+    """For Sampler.block_norm_device: sum = residual + scale * act(gate) * after(x),
+    out = before(sum); a gate of stride 0 is one row for all."""
+    none = RowsC()
+    return BlockNormC(int(M), int(C), x, after or norm(), gate or none, int(gate_act), float(scale),
+                      residual or none, sum or none, before or norm(), out or none)
 
 
 class SampleConfigC(ctypes.Structure):
@@ -239,6 +288,11 @@ def _load() -> ctypes.CDLL:
     L.hs_gemv_lora_device.argtypes = [vp, vp, i32, i64, P(WeightsC), P(AdaptersC), vp, vp, i64, vp]
     L.hs_lm_head_lora_sample_device.argtypes = [vp, vp, i32, i64, P(WeightsC), P(AdaptersC), vp,
                                                 vp, i64, vp, vp, P(SampleConfigC), vp, vp, vp]
+    L.hs_block_norm_device.argtypes = [vp, P(BlockNormC), vp]
+    L.hs_matmul_int_device.argtypes = [vp, i32, P(RowsC), P(WeightsC), vp, P(RowsC), vp]
+    L.hs_gated_int_device.argtypes = [vp, i32, P(RowsC), P(WeightsC), P(WeightsC), i32, P(RowsC), vp]
+    L.hs_lm_head_norm_sample_device.argtypes = [vp, P(BlockNormC), P(WeightsC), vp, i64, vp, vp,
+                                                P(SampleConfigC), vp, vp, vp]
     L.hs_context_set_timing.argtypes = [vp, ctypes.c_int]
     L.hs_context_kernel_times.argtypes = [vp, P(dbl), i32, P(i64)]
     return L
@@ -330,7 +384,8 @@ class Sampler:
                "mid_kernel", "argmax_kernel", "gemv_kernel", "large_fast_kernel",
                "large_replay_kernel", "large_replay_dev_kernel", "minp_kernel",
                "verify_stats_kernel", "verify_final_kernel", "verify_lists_kernel",
-               "lora_shrink_kernel", "lora_expand_kernel")
+               "lora_shrink_kernel", "lora_expand_kernel", "block_norm_kernel",
+               "int8_kernel", "requant_kernel")
 
     def kernel_times(self):
         """({kernel: total device ms}, calls) since the last query."""
@@ -540,6 +595,37 @@ class Sampler:
         _check(lib().hs_lm_head_lora_sample_device(
             self._ctx, d_x, M, ldx, w, ad, d_slots, d_logits, ldl, d_hist_ids or None,
             d_hist_off or None, cfgs, d_uniforms, d_tokens, st))
+
+    # ---- norms between blocks, 8-bit products ---------------------------------------
+    def block_norm_device(self, block: BlockNormC, stream=None) -> None:
+        """Enqueue sum = residual + scale * act(gate) * after(x), out = before(sum)
+        (hs_block_norm_device); 8-bit rows out: quantised."""
+        st = stream.handle if isinstance(stream, hip.Stream) else stream
+        _check(lib().hs_block_norm_device(self._ctx, block, st))
+
+    def matmul_int_device(self, M: int, x: RowsC, w: WeightsC, d_bias: int | None, y: RowsC,
+                         stream=None) -> None:
+        """y = x W^T + bias with W of type I8 (24) and x in 8 bits, or quantised
+        first (hs_matmul_int_device)."""
+        st = stream.handle if isinstance(stream, hip.Stream) else stream
+        _check(lib().hs_matmul_int_device(self._ctx, M, x, w, d_bias or None, y, st))
+
+    def gated_int_device(self, M: int, x: RowsC, gate: WeightsC, up: WeightsC, act: int, y: RowsC,
+                        stream=None) -> None:
+        """y = act(x gate^T) * (x up^T) (hs_gated_int_device)."""
+        st = stream.handle if isinstance(stream, hip.Stream) else stream
+        _check(lib().hs_gated_int_device(self._ctx, M, x, gate, up, act, y, st))
+
+    def lm_head_norm_sample_device(self, block: BlockNormC, w: WeightsC, d_logits: int, ldl: int,
+                                   d_hist_ids, d_hist_off, configs, d_uniforms: int, d_tokens: int,
+                                   stream=None) -> None:
+        """block_norm_device, the lm_head on its `out`, then sampling
+        (hs_lm_head_norm_sample_device)."""
+        cfgs = configs if isinstance(configs, ctypes.Array) else _configs(configs, block.rows)
+        st = stream.handle if isinstance(stream, hip.Stream) else stream
+        _check(lib().hs_lm_head_norm_sample_device(
+            self._ctx, block, w, d_logits, ldl, d_hist_ids or None, d_hist_off or None, cfgs,
+            d_uniforms, d_tokens, st))
 
     # ---- device-resident batch ----------------------------------------------
     def sample_device(self, d_logits: int, rows: int, row_stride: int, vocab: int,

@@ -466,6 +466,108 @@ int hs_lm_head_lora_sample_device(hs_context *ctx, const float *d_x, int32_t M, 
                                   const hs_sample_config *configs, const double *d_uniforms,
                                   int32_t *d_tokens, void *stream);
 
+/* ---- The block of a model in 8-bit integers: norms between blocks, products
+ * with a scale for each token and each output channel, gated pairs of them.  No
+ * counterpart in the reference, whose forward pass is WGSL kernels over GGUF
+ * weights (rmsnorm, src/kernels.ts:324; swiglu_fused, src/kernels.ts:1208). */
+
+/* Rows of elements: F32 (0), F16 (1), BF16 (30) or I8 (24), GGML ids.  An I8
+ * row m stands for data[m][c] * scales[m].  Elements are aligned as such. */
+typedef struct hs_rows {
+  int32_t type;
+  int64_t stride;              /* elements from row to row, at least the columns */
+  void *data;                  /* device; NULL: absent, where that is allowed */
+  float *scales;               /* device [rows]: I8 only, NULL otherwise */
+} hs_rows;
+
+/* A norm over the columns of a row, or none (weight and bias are then unused):
+ *   HS_NORM_RMS:   v / sqrt(mean(v^2) + eps) * weight + bias
+ *   HS_NORM_LAYER: (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight + bias
+ * weight and bias: device [cols] binary32, or NULL for 1 and 0. */
+#define HS_NORM_NONE  0
+#define HS_NORM_RMS   1
+#define HS_NORM_LAYER 2
+typedef struct hs_norm {
+  int32_t kind;
+  float eps;                   /* >= 0 */
+  const float *weight;
+  const float *bias;
+} hs_norm;
+
+/* Activations: v, v / (1 + exp(-v)), v Phi(v), the same by
+ * tanh(sqrt(2 / pi) (v + 0.044715 v^3)), max(v, 0), 1 / (1 + exp(-v)), tanh(v). */
+#define HS_ACT_NONE      0
+#define HS_ACT_SILU      1
+#define HS_ACT_GELU      2
+#define HS_ACT_GELU_TANH 3
+#define HS_ACT_RELU      4
+#define HS_ACT_SIGMOID   5
+#define HS_ACT_TANH      6
+
+/* The end of a block and the start of the next, in one pass over the rows:
+ *   s   = residual + scale * act(gate) * after(x)
+ *   sum = s;   out = before(s)
+ * in binary32, each result rounded once to its type (out is formed from s as it
+ * is before it is rounded to sum's type).  x, gate, residual and sum are float rows;
+ * gate (absent: 1) has a row for each row, or one for all of them with stride 0;
+ * residual absent: 0; sum or out may be absent.  out may be I8: then its
+ * scale is max|out| / 127 of the row, rounded to binary32, and its integers
+ * out / scale to the nearest, ties to even; a row whose largest magnitude is
+ * below 2^-100 gets scale 0 and zeros, one with a NaN or an infinity scale NaN
+ * and zeros, so that its products are NaN.  With both norms HS_NORM_NONE
+ * the call quantises or converts rows.  sum and out may be x, residual or a gate of
+ * as many rows themselves (same data, type and stride); otherwise they overlap
+ * nothing.  cols up to 32768, rows up to 2^24.  Asynchronous on `stream`, no
+ * workspace; may be captured. */
+typedef struct hs_block_norm {
+  int32_t rows, cols;
+  hs_rows x;
+  hs_norm after;
+  hs_rows gate;
+  int32_t gate_act;
+  float scale;
+  hs_rows residual;
+  hs_rows sum;
+  hs_norm before;
+  hs_rows out;
+} hs_block_norm;
+
+int hs_block_norm_device(hs_context *ctx, const hs_block_norm *norm, void *stream);
+
+/* y[m][n] = (sum_k x[m][k] w[n][k]) * xs[m] * ws[n] + bias[n] for m < M: w is an
+ * hs_weights of type I8 (24): `data` N rows of K int8 back to back, 16-byte
+ * aligned, K a multiple of 16 up to 65536, `scales16` its N binary32 (not
+ * binary16) channel scales, no `hadamard`.  x is I8 (16-byte aligned, stride a
+ * multiple of 16), or float rows, which are quantised first as
+ * hs_block_norm_device does it, into the context's workspace.  The integer sums are
+ * exact, so that a row's result does not depend on M or on what is beside it.
+ * y: float rows, or I8 quantised as above (from binary32 results, in the
+ * workspace).  y overlaps none of the inputs.  bias: device [N] binary32 or NULL.
+ * M up to 2^20, N up to 2^24 (32768 where y is I8).  Captured calls and the
+ * workspace as in hs_verify_drafts_device; x in I8 and y in floats need none.
+ *
+ * hs_gemv_device_ex, hs_lm_head_sample_device_ex, hs_gemv_lora_device and
+ * hs_lm_head_lora_sample_device take such weights too (K then up to 65536), with
+ * binary32 x and y. */
+int hs_matmul_int_device(hs_context *ctx, int32_t M, const hs_rows *x, const hs_weights *w,
+                        const float *bias, const hs_rows *y, void *stream);
+
+/* A gated feed-forward's two projections, its activation and their product in
+ * one kernel: y = act(x gate^T) * (x up^T), both as hs_matmul_int_device forms them
+ * (without a bias), gate and up of the same rows and cols. */
+int hs_gated_int_device(hs_context *ctx, int32_t M, const hs_rows *x, const hs_weights *gate,
+                       const hs_weights *up, int32_t act, const hs_rows *y, void *stream);
+
+/* The model's last step from the stream on: hs_block_norm_device, then the
+ * lm_head on its `out` (F32, for any weights, or I8 for I8 weights) into
+ * d_logits, then sampling, as hs_lm_head_sample_device_ex.  Not to be captured, as
+ * hs_lm_head_lora_sample_device. */
+int hs_lm_head_norm_sample_device(hs_context *ctx, const hs_block_norm *norm,
+                                  const hs_weights *w, float *d_logits, int64_t ldl,
+                                  const int32_t *d_hist_ids, const int64_t *d_hist_offsets,
+                                  const hs_sample_config *configs, const double *d_uniforms,
+                                  int32_t *d_tokens, void *stream);
+
 /* Diagnostics (no counterpart in the reference, which has no GPU sampler):
  * while enabled, every sampling call records HIP events on its stream around
  * each of its kernel launches.  hs_context_kernel_times() waits for the
@@ -476,7 +578,9 @@ int hs_lm_head_lora_sample_device(hs_context *ctx, const float *d_x, int32_t M, 
  * slot replay in LDS, ms[10] large-k slot replay in device memory, ms[11]
  * min-p kernel, ms[12] the drafted rows' sums, ms[13] their outcome, ms[14]
  * verification against candidate lists, ms[15] and ms[16] the adapters' two
- * products; a kernel a call did not launch adds 0)
+ * products, ms[17] block norms and the quantising of rows, ms[18] 8-bit
+ * products, ms[19] the quantising of their results; a kernel a call did not
+ * launch adds 0)
  * and the number of
  * timed calls, and resets the totals. */
 int hs_context_set_timing(hs_context *ctx, int enable);
