@@ -48,6 +48,7 @@ hipError_t launch_block_norm(const BlockNormArgs &a, hipStream_t stream, hipEven
 // y[m][n] = xs[m] * ws[n] * sum_k x[m][k] w[n][k] + bias[n], and with a second
 // weight act(the first's) * the second's.
 constexpr int kInt8MaxM = 1 << 20, kInt8MaxN = 1 << 24, kNormMaxM = 1 << 24;
+constexpr int64_t kInt8MaxLd = 1 << 23;   // 255 rows of it below 2^31
 constexpr int kInt8MaxK = 65536;   // 2^16 * 2^14 below 2^31: the sums are exact
 struct Int8Args {
   const int8_t *x;           // [M][ldx], 16-byte aligned rows
@@ -58,6 +59,7 @@ struct Int8Args {
   const float *bias;         // [N] or null
   RowsArg y;
   int32_t M, N, K, pair, act;
+  int32_t wide;              // y's rows are 16-byte aligned
 };
 hipError_t launch_int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done);
 

@@ -1765,6 +1765,8 @@ int int8_args(int32_t M, const hs_rows *x, const hs_weights *w0, const hs_weight
   if (rc) return rc;
   if (xr.type == hs::kT_I8 && ((reinterpret_cast<uintptr_t>(xr.p) | (uintptr_t)xr.ld) & 15u))
     return fail(HS_ERR_INVALID_ARGUMENT, "x in 8 bits must be 16-byte aligned, its stride a multiple of 16");
+  if (xr.type == hs::kT_I8 && xr.ld > hs::kInt8MaxLd)
+    return fail(HS_ERR_UNSUPPORTED, "x in 8 bits: stride %lld above 2^23", (long long)xr.ld);
   if (xr.type != hs::kT_I8 && K > hs::kNormMaxC)
     return fail(HS_ERR_UNSUPPORTED, "K %d of float rows above %d", K, hs::kNormMaxC);
   if (yr.type == hs::kT_I8 && N > hs::kNormMaxC)
@@ -1836,6 +1838,15 @@ int int8_run(hs_context *ctx, Int8Call &c, hipStream_t stream) {
   if (rc) return rc;
   auto of = [&](int slot) { return ev ? ev + 2 * slot : nullptr; };
   const hipEvent_t done = cap ? nullptr : ctx->done_ev;
+  if (c.post.M) {
+    c.g.y.p = ctx->int8_y.b.p;
+    c.g.y.ld = ldh;
+    c.g.y.type = hs::kT_F32;
+    c.post.x = c.g.y;
+    c.post.x.scales = nullptr;
+    c.post.vec = wide_rows(c.post);
+  }
+  c.g.wide = ((reinterpret_cast<uintptr_t>(c.g.y.p) | (uintptr_t)(c.g.y.ld * hs::row_elem_bytes(c.g.y.type))) & 15u) == 0;
   hipError_t e = hipSuccess;
   if (c.pre.M) {
     char *q = static_cast<char *>(ctx->int8_x.b.p);
@@ -1848,14 +1859,6 @@ int int8_run(hs_context *ctx, Int8Call &c, hipStream_t stream) {
     c.g.x = reinterpret_cast<const int8_t *>(q);
     c.g.ldx = K;
     c.g.xs = c.pre.out.scales;
-  }
-  if (c.post.M) {
-    c.g.y.p = ctx->int8_y.b.p;
-    c.g.y.ld = ldh;
-    c.g.y.type = hs::kT_F32;
-    c.post.x = c.g.y;
-    c.post.x.scales = nullptr;
-    c.post.vec = wide_rows(c.post);
   }
   if (e == hipSuccess)
     e = inject_failure() ? hipErrorOutOfMemory
