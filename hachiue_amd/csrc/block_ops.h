@@ -60,7 +60,12 @@ struct Int8Args {
   RowsArg y;
   int32_t M, N, K, pair, act;
   int32_t wide;              // y's rows are 16-byte aligned
+  RowsArg rows;              // a float row that the kernel quantises itself (int8_row), or p null
 };
+// One row that a workgroup holds in its threads' registers has a kernel of its own,
+// which quantises it too.
+constexpr int kInt8RowK = 4096;
+inline bool int8_row(int32_t M, int32_t K) { return M == 1 && K <= kInt8RowK; }
 hipError_t launch_int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done);
 
 #ifdef __HIPCC__
@@ -77,11 +82,22 @@ hipError_t launch_timed(F kernel, dim3 grid, int threads, hipStream_t stream, hi
   return hipGetLastError();
 }
 
+// exp(x) for x <= 0, a step or two off: x log2(e) as an integer and the rest, the
+// logarithm in two parts, so that nothing is lost where x is far below 0.
+__device__ __forceinline__ float exp_below(float x) {
+  const float n = rintf(x * 1.44269502f);
+  const float f = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269502f, -n));
+  return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+}
 // v / (1 + exp(-z)): the exponential never overflows, so that the result goes to
-// 0 as slowly as it should where z is far below 0.
+// 0 as slowly as it should where z is far below 0.  The divisor lies in [1, 2]: its
+// reciprocal and one correction, a third of a division's instructions.  (4096 tokens'
+// gated pairs, where a lane has 128 results of a tile: see int8_tile_kernel.)
 __device__ __forceinline__ float logistic(float v, float z) {
-  const float e = expf(-fabsf(z));
-  return v * (z < 0.0f ? e : 1.0f) / (1.0f + e);
+  const float e = exp_below(fmaxf(-fabsf(z), -256.0f));
+  const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d), n = z < 0.0f ? e : 1.0f;
+  const float q = n * r;
+  return v * fmaf(fmaf(-d, q, n), r, q);
 }
 
 __device__ __forceinline__ float activation(int act, float v) {
@@ -91,10 +107,34 @@ __device__ __forceinline__ float activation(int act, float v) {
     case kActGeluTanh:   // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u))
       return logistic(v, 1.59576912f * fmaf(0.044715f * v * v, v, v));
     case kActRelu: return v > 0.0f ? v : v != v ? v : 0.0f;
-    case kActSigmoid: return logistic(1.0f, v);
+    case kActSigmoid: return v != v ? v : logistic(1.0f, v);
     case kActTanh: return tanhf(v);
     default: return v;
   }
+}
+
+// The scale of a row whose largest magnitude has the bits `most` (a NaN's are above
+// an infinity's, and those above every number's): NaN where it is not finite, 0
+// below 2^-100.  *inv: 1 / scale, or 0 where the row's integers are 0.
+__device__ __forceinline__ float scale_of(uint32_t most, float *inv) {
+  const bool finite = most < 0x7F800000u, some = finite && most >= 0x0D800000u;
+  const float scale = some ? __uint_as_float(most) / 127.0f : finite ? 0.0f : __uint_as_float(0x7FC00000u);
+  *inv = some ? 1.0f / scale : 0.0f;
+  return scale;
+}
+// v / scale to the nearest integer, ties to even, as if the quotient were exact:
+// v * inv is off by less than 2^-15, so that only next to a half does it not tell;
+// there v is compared with the half times the scale, which binary64 holds exactly.
+__device__ __forceinline__ int quantised(float v, float inv, float scale) {
+  const float a = fabsf(v), t = a * inv;
+  float q = rintf(t);
+  const float half = rintf(t - 0.5f) + 0.5f;
+  if (fabsf(t - half) < 0.000244140625f) {
+    const double edge = (double)half * (double)scale;
+    const float low = half - 0.5f;
+    q = (double)a > edge ? low + 1.0f : (double)a < edge ? low : rintf(half);
+  }
+  return (int)copysignf(q, v);
 }
 
 __device__ __forceinline__ uint16_t bits16(int type, float v) {

@@ -10,11 +10,18 @@
 
 #include <hip/hip_ext.h>
 
+#include <type_traits>
+
 namespace hs {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+typedef const __attribute__((address_space(1))) void *GlobalPtr;
+typedef __attribute__((address_space(3))) void *LdsPtr;
+// 16 zero bytes: what is loaded behind a row's end.
+__device__ const int4 zeros = {0, 0, 0, 0};
 
 // One result from its exact sums, `ws` and `bias` those of its channel.
 __device__ __forceinline__ float scaled(int sum, float xs, float ws) { return (float)sum * xs * ws; }
@@ -43,61 +50,298 @@ __device__ __forceinline__ void put8(const Int8Args &a, int64_t m, int n, const 
   }
 }
 
-// ---- few tokens: the weights go from memory to registers once, HBM-bound.  A
-// workgroup has TN tiles of 16 channels (of each weight) and TM tiles of 16
-// tokens; its waves take the steps of 64 k in turn and add their sums up in LDS.
-constexpr int kFewWaves = 4;
-template <int TM, int TN, int PAIR>
-__global__ void __launch_bounds__(kFewWaves * 64) int8_few_kernel(Int8Args a) {
-  constexpr int T = PAIR * TN * TM;
-  __shared__ i32x4 part[kFewWaves][T][64];
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const int n0 = blockIdx.x * 16 * TN, m0 = blockIdx.y * 16 * TM;
-  const int row = lane % 16, at = lane / 16 * 16;
-  const int8_t *w[PAIR][TN], *x[TM];
+// Waits of this wave alone, in the order of the code: at most `loads` of its loads
+// (and stores) are still on their way, and what it read from LDS is in registers.
+template <int loads>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (loads & 15) | (loads >> 4) << 14);   // vmcnt, lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+// A barrier behind which every wave's LDS accesses are done; loads stay on their way.
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---- one token: HBM-bound, the weights go through LDS once.  A workgroup takes tiles
+// of 16 channels (of each weight) in turn, its waves the steps of 128 k of a tile;
+// their sums are added up in LDS, by one wave while the others go on.  A wave's
+// weights pass through its own part of LDS, 8 KB on their way at a time, without a
+// barrier and on into the next tile, so that nothing runs dry at a tile's end.  A
+// float row is quantised by each workgroup while its first weights are on their
+// way, which saves a launch.  The product is the matrix cores' with the token in
+// all 16 columns: they have 30 times the rate that the weights come at.
+constexpr int kRowWaves = 4;
+
+// The row into LDS, zeros behind K (a multiple of 128 bytes), and its scale.
+__device__ __forceinline__ void keep_row(const Int8Args &a, int8_t *q, float *scale_at, uint32_t *most) {
+  constexpr int kThreads = kRowWaves * 64, kHeld = kInt8RowK / kThreads;
+  const int t = threadIdx.x, wide = (a.K + 127) / 128 * 128;
+  if (!a.rows.p) {
+    static_assert(kInt8RowK / 16 == kThreads, "a thread has 16 bytes");
+    if (t * 16 < wide) reinterpret_cast<int4 *>(q)[t] = t * 16 < a.K ? reinterpret_cast<const int4 *>(a.x)[t] : zeros;
+    if (t == 0) *scale_at = a.xs[0];
+    return;
+  }
+  float v[kHeld];
+  if (a.rows.type == kT_F32) {
 #pragma unroll
-  for (int p = 0; p < PAIR; ++p)
+    for (int e = 0; e < kHeld; ++e) {
+      const int k = t + e * kThreads;
+      v[e] = k < a.K ? static_cast<const float *>(a.rows.p)[k] : 0.0f;
+    }
+  } else {
+    uint16_t u[kHeld];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) w[p][j] = a.w[p] + (int64_t)min(n0 + 16 * j + row, a.N - 1) * a.K;
+    for (int e = 0; e < kHeld; ++e) {
+      const int k = t + e * kThreads;
+      u[e] = k < a.K ? static_cast<const uint16_t *>(a.rows.p)[k] : (uint16_t)0;
+    }
 #pragma unroll
-  for (int i = 0; i < TM; ++i) x[i] = a.x + (int64_t)min(m0 + 16 * i + row, a.M - 1) * a.ldx;
-  i32x4 acc[PAIR][TN][TM] = {};
-#pragma unroll 4
-  for (int k = wave * 64 + at; k - at < a.K; k += kFewWaves * 64) {
-    i32x4 wf[PAIR][TN] = {}, xf[TM] = {};
-    if (k < a.K) {
+    for (int e = 0; e < kHeld; ++e) v[e] = widen16(a.rows.type, u[e]);
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < kHeld; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+  if (t % 64 == 0) most[t / 64] = top;
+  meet();
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) top = max(top, most[w]);
+  float inv;
+  const float scale = scale_of(top, &inv);
+  if (t == 0) *scale_at = scale;
+#pragma unroll
+  for (int e = 0; e < kHeld; ++e) {
+    const int k = t + e * kThreads;
+    if (k < wide) q[k] = k < a.K && inv > 0.0f ? (int8_t)quantised(v[e], inv, scale) : (int8_t)0;
+  }
+}
+
+template <int PAIR>
+__global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
+  constexpr int W = kRowWaves, kSlot = PAIR * 2048, kLoads = 2 * PAIR, D = 4 / PAIR;
+  // (arrays of their own: the compiler sees that loads are on their way to others)
+  __shared__ __align__(1024) int8_t r0[W * kSlot], r1[W * kSlot];
+  __shared__ __align__(1024) int8_t r2[D == 4 ? W * kSlot : 16], r3[D == 4 ? W * kSlot : 16];
+  __shared__ __align__(16) int8_t q[kInt8RowK];
+  __shared__ int part[2][W][PAIR][16];
+  __shared__ float scale;
+  __shared__ uint32_t most[W];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int tiles = (a.N + 15) / 16;
+  const int steps = (a.K + 127) / 128, turns = (steps + W - 1) / W;   // of a tile, a wave's
+  // Where the next load is.  A step's rows of 128 bytes lie in 16-byte pieces, piece ^
+  // (row / 2 % 8), so that sixteen rows' same pieces fill the 64 banks once (loads
+  // to LDS are in lane order: the order is made by what a lane reads); a load is
+  // eight rows.
+  int to_tile = blockIdx.x, to_turn = 0;
+  const int8_t *base[PAIR];
+  uint32_t off[2];
+  auto seek = [&](int tile) {
+    const int n0 = tile * 16;
+#pragma unroll
+    for (int p = 0; p < PAIR; ++p) base[p] = a.w[p] + (int64_t)n0 * a.K;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      off[i] = (uint32_t)min(i * 8 + lane / 8, a.N - 1 - n0) * (uint32_t)a.K + (lane % 8 ^ (i * 4 + lane / 16)) * 16;
+  };
+  seek(to_tile);
+  auto load = [&](int8_t *slot) {
+    const int k = (to_turn * W + wave) * 128;
+    const bool whole = k + 128 <= a.K && to_tile < tiles;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int piece = (lane % 8 ^ (i % 2 * 4 + lane / 16)) * 16;
+      const void *p = base[i / 2] + k + off[i % 2];
+      if (!whole && (k + piece >= a.K || to_tile >= tiles)) p = &zeros;
+      __builtin_amdgcn_global_load_lds((GlobalPtr)p, (LdsPtr)(slot + wave * kSlot + i * 1024), 16, 0, 0);
+    }
+    if (++to_turn == turns) {
+      to_turn = 0;
+      to_tile += gridDim.x;
+      if (to_tile < tiles) seek(to_tile);
+    }
+  };
+  load(r0);
+  load(r1);
+  if constexpr (D == 4) {
+    load(r2);
+    load(r3);
+  }
+  keep_row(a, q, &scale, most);
+  meet();
+  int tile = blockIdx.x, at_turn = 0, done = 0;
+  i32x4 acc[PAIR] = {};
+  auto turn = [&](int8_t *slot) {
+    // A slot's loads are there when at most those of the D - 1 behind it are not.
+    wait_loads<(D - 1) * kLoads>();
+    const int s = at_turn * W + wave;
+    if (s < steps) {
+      const int8_t *at = slot + wave * kSlot + lane % 16 * 128;
+      i32x4 w[2][PAIR], x[2];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const int p = kk * 4 + lane / 16;
+#pragma unroll
+        for (int i = 0; i < PAIR; ++i)
+          w[kk][i] = *reinterpret_cast<const i32x4 *>(at + i * 2048 + (p ^ lane / 2 % 8) * 16);
+        x[kk] = *reinterpret_cast<const i32x4 *>(q + s * 128 + p * 16);
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int i = 0; i < PAIR; ++i)
+          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[kk][i], x[kk], acc[i], 0, 0, 0);
+    }
+    // what was read is in registers: its place may be loaded anew
+    wait_loads<(D - 1) * kLoads>();
+    load(slot);
+    if (++at_turn < turns) return;
+    at_turn = 0;
+    // lanes 0, 16, 32 and 48 have the first column: four channels each
+#pragma unroll
+    for (int p = 0; p < PAIR; ++p) {
+      if (lane % 16 == 0) *reinterpret_cast<i32x4 *>(&part[done % 2][wave][p][lane / 4]) = acc[p];
+      acc[p] = i32x4{};
+    }
+    // (a place is written again two tiles later, behind the next tile's barrier, at
+    // which the wave that reads it here arrives when it has read it)
+    meet();
+    const int n = tile * 16 + lane;
+    if (done % W == wave && lane < 16 && n < a.N) {
+      int s[PAIR] = {};
 #pragma unroll
       for (int p = 0; p < PAIR; ++p)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) wf[p][j] = *reinterpret_cast<const i32x4 *>(w[p][j] + k);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) xf[i] = *reinterpret_cast<const i32x4 *>(x[i] + k);
+        for (int v = 0; v < W; ++v) s[p] += part[done % 2][v][p][lane];
+      float v = scaled(s[0], scale, a.ws[0][n]);
+      if constexpr (PAIR == 2) v = activation(a.act, v) * scaled(s[PAIR - 1], scale, a.ws[PAIR - 1][n]);
+      else if (a.bias) v += a.bias[n];
+      put(a.y, 0, n, v);
     }
-#pragma unroll
-    for (int p = 0; p < PAIR; ++p)
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-          acc[p][j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[p][j], xf[i], acc[p][j][i], 0, 0, 0);
+    ++done;
+    tile += gridDim.x;
+  };
+  while (tile < tiles) {   // (turns behind the last tile's end read zeros and are not stored)
+    turn(r0);
+    if (tile < tiles) turn(r1);
+    if constexpr (D == 4) {
+      if (tile < tiles) turn(r2);
+      if (tile < tiles) turn(r3);
+    }
   }
+}
+
+// ---- few results: K is split among a workgroup's waves, so that as many compute
+// units as there are tiles of 16 channels (of each weight) and TM tiles of 16 tokens
+// read at once.  A wave's weights and tokens pass through its own part of LDS, four
+// steps of 128 k on their way at a time (two of more rows), without a barrier; the
+// waves' sums are added up at the end.  (Loaded straight to registers, a matrix
+// operand's neighbouring lanes are different rows, and each 16 bytes are a look-up of
+// their own in the cache: 16 tokens of 4096 x 4096 8.8 us, 6.5 so.)
+template <int TM, int PAIR, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
+  constexpr int T = PAIR * TM, kRows = PAIR + TM;   // tiles of 16 rows of a step
+  constexpr int D = kRows <= 2 ? 4 : 2, kSlot = kRows * 2048, kLoads = 2 * kRows;
+  // (arrays of their own: the compiler sees that loads are on their way to others)
+  __shared__ __align__(1024) int8_t r0[WAVES * kSlot], r1[WAVES * kSlot];
+  __shared__ __align__(1024) int8_t r2[D == 4 ? WAVES * kSlot : 16], r3[D == 4 ? WAVES * kSlot : 16];
+  static_assert(T * 1024 <= kSlot, "a wave's sums fit its first slot");
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * TM;
+  const int steps = (a.K + 127) / 128;
+  // A step's rows of 128 bytes lie in 16-byte pieces, piece ^ (row / 2 % 8); a load
+  // is eight rows.
+  const int8_t *base[kRows];
+  uint32_t off[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = i % 2 * 8 + lane / 8;
+    if (i < 2 * PAIR) {
+      base[i / 2] = a.w[i / 2] + (int64_t)n0 * a.K;
+      off[i] = (uint32_t)min(r, a.N - 1 - n0) * (uint32_t)a.K;
+    } else {
+      const int m = m0 + (i / 2 - PAIR) * 16;
+      base[i / 2] = a.x + (int64_t)min(m, a.M - 1) * a.ldx;
+      off[i] = (uint32_t)max(0, min(r, a.M - 1 - m)) * (uint32_t)a.ldx;
+    }
+    off[i] += (lane % 8 ^ (i % 2 * 4 + lane / 16)) * 16;
+  }
+  auto load = [&](int8_t *slot, int s) {
+    const int k = s * 128;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int piece = (lane % 8 ^ (i % 2 * 4 + lane / 16)) * 16;
+      const void *p = base[i / 2] + k + off[i];
+      if (k + 128 > a.K && k + piece >= a.K) p = &zeros;
+      __builtin_amdgcn_global_load_lds((GlobalPtr)p, (LdsPtr)(slot + wave * kSlot + i * 1024), 16, 0, 0);
+    }
+  };
+  i32x4 acc[PAIR][TM] = {};
+  auto products = [&](const int8_t *slot, int s) {
+    const int8_t *at = slot + wave * kSlot + lane % 16 * 128;
+    i32x4 w[2][PAIR], x[2][TM];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const int p = ((kk * 4 + lane / 16) ^ (lane / 2 % 8)) * 16;
+#pragma unroll
+      for (int i = 0; i < PAIR; ++i) w[kk][i] = *reinterpret_cast<const i32x4 *>(at + i * 2048 + p);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) x[kk][i] = *reinterpret_cast<const i32x4 *>(at + (PAIR + i) * 2048 + p);
+    }
+    // what is read is in registers: its place may be loaded anew
+    wait_loads<(D - 1) * kLoads>();
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < PAIR; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[kk][i], x[kk][j], acc[i][j], 0, 0, 0);
+  };
+  // A slot: its loads are there when at most those of the D - 1 behind it are not.
+  auto turn = [&](int8_t *slot, int s) {
+    wait_loads<(D - 1) * kLoads>();
+    products(slot, s);
+    load(slot, s + D * WAVES);
+  };
+  load(r0, wave);
+  load(r1, wave + WAVES);
+  if constexpr (D == 4) {
+    load(r2, wave + 2 * WAVES);
+    load(r3, wave + 3 * WAVES);
+  }
+  for (int s = wave; s < steps; s += D * WAVES) {
+    turn(r0, s);
+    if (s + WAVES < steps) turn(r1, s + WAVES);
+    if constexpr (D == 4) {
+      if (s + 2 * WAVES < steps) turn(r2, s + 2 * WAVES);
+      if (s + 3 * WAVES < steps) turn(r3, s + 3 * WAVES);
+    }
+  }
+  // (the loads behind the rows' end are there too before the sums take their place)
+  wait_loads<0>();
+  i32x4 *const part = reinterpret_cast<i32x4 *>(r0);
 #pragma unroll
   for (int p = 0; p < PAIR; ++p)
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int i = 0; i < TM; ++i) part[wave][(p * TN + j) * TM + i][lane] = acc[p][j][i];
+    for (int i = 0; i < TM; ++i) part[wave * (kSlot / 16) + (p * TM + i) * 64 + lane] = acc[p][i];
   __syncthreads();
-  for (int tile = wave; tile < TN * TM; tile += kFewWaves) {
+  for (int tile = wave; tile < TM; tile += WAVES) {
     i32x4 s[PAIR];
 #pragma unroll
     for (int p = 0; p < PAIR; ++p) {
-      s[p] = part[0][p * TN * TM + tile][lane];
+      s[p] = part[(p * TM + tile) * 64 + lane];
 #pragma unroll
-      for (int v = 1; v < kFewWaves; ++v) s[p] += part[v][p * TN * TM + tile][lane];
+      for (int v = 1; v < WAVES; ++v) s[p] += part[v * (kSlot / 16) + (p * TM + tile) * 64 + lane];
     }
     // a lane has one token's four channels
-    const int m = m0 + tile % TM * 16 + lane % 16, n = n0 + tile / TM * 16 + lane / 16 * 4;
+    const int m = m0 + tile * 16 + lane % 16, n = n0 + lane / 16 * 4;
     if (m >= a.M) continue;
     const float xs = a.xs[m];
 #pragma unroll
@@ -112,12 +356,6 @@ __global__ void __launch_bounds__(kFewWaves * 64) int8_few_kernel(Int8Args a) {
 }
 
 // ---- many tokens: tiles through LDS.
-// 16 zero bytes: what is loaded behind a row's end.
-__device__ const int4 zeros = {0, 0, 0, 0};
-
-typedef const __attribute__((address_space(1))) void *GlobalPtr;
-typedef __attribute__((address_space(3))) void *LdsPtr;
-
 // A workgroup of 2 x 2 waves has a tile of BM tokens and BN channels (PAIR 2: BN / 2
 // of each weight), a wave a quarter of it.  A stage is 128 k of all of its rows.
 template <int BM, int BN>
@@ -141,24 +379,38 @@ __device__ __forceinline__ void tile_of(int id, int total, int tm, int &im, int 
   in = (t - g * span) / in_group;
 }
 
-template <int BM, int BN, int PAIR>
-__global__ void __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) int8_tile_kernel(Int8Args a) {
+// The order of `products` matrix instructions, `reads` from LDS and `loads` to it:
+// evenly among each other.  (The waves of a CU are alone on their SIMDs: what stands
+// between two products is hidden behind the first, what stands together is not.)
+template <int products, int reads, int loads, int i = 0>
+__device__ __forceinline__ void interleave() {
+  constexpr int r = (i + 1) * reads / products - i * reads / products;
+  constexpr int l = (i + 1) * loads / products - i * loads / products;
+  __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+  if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
+  if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x010, l, 0);
+  if constexpr (i + 1 < products) interleave<products, reads, loads, i + 1>();
+}
+
+template <int BM, int BN, int PAIR, int D>
+__global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int8_tile_kernel(Int8Args a) {
   typedef Tile<BM, BN> C;
-  // (two arrays: the compiler sees that a stage that is read is not the one that
-  // loads are on their way to)
-  __shared__ __align__(1024) int8_t even[C::kStage];
-  __shared__ __align__(1024) int8_t odd[C::kStage];
+  constexpr int kEarly = D > 2 ? C::kLoads : C::kLoads - C::kLoads / 4;
+  // (arrays of their own: the compiler sees that a stage that is read is not one
+  // that loads are on their way to)
+  __shared__ __align__(1024) int8_t s0[C::kStage], s1[C::kStage];
+  __shared__ __align__(1024) int8_t s2[D == 4 ? C::kStage : 16], s3[D == 4 ? C::kStage : 16];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
   const int wm = wave / 2, wn = wave % 2;
   int im, in;
   tile_of(blockIdx.x, gridDim.x, (a.M + BM - 1) / BM, im, in);
   const int m0 = im * BM, n0 = in * (BN / PAIR);
   // A stage holds rows of 128 bytes, tokens then channels, a row's 16-byte pieces
-  // in the order piece ^ (row % 8): eight rows' same pieces lie in eight different
-  // sets of banks.  (Loads to LDS are in lane order: the order is made by what a
+  // in the order piece ^ (row / 2 % 8): sixteen rows' same pieces fill the 64
+  // banks once.  (Loads to LDS are in lane order: the order is made by what a
   // lane reads.)  A load of a wave is eight rows; pairs: each 32 channels of the
   // first weight are followed by the second's.
-  const int piece = ((lane % 8) ^ (lane / 8)) * 16;
+  const int piece = ((lane % 8) ^ (wave % 2 * 4 + lane / 16)) * 16;
   const int8_t *base[1 + PAIR] = {a.x + (int64_t)m0 * a.ldx, a.w[0] + (int64_t)n0 * a.K};
   if constexpr (PAIR == 2) base[PAIR] = a.w[1] + (int64_t)n0 * a.K;
   uint32_t off[C::kLoads];
@@ -172,20 +424,20 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) int8_tile_ke
       off[i] = (uint32_t)min(n, a.N - 1 - n0) * (uint32_t)a.K + piece;
     }
   }
-  auto load = [&](int8_t *stage, int k) {
-    if (k + 128 <= a.K) {
+  // Loads [from, to) of the stage at k; zeros behind the rows' end.
+  auto load = [&](int8_t *stage, int k, int from, int to) {
 #pragma unroll
-      for (int i = 0; i < C::kLoads; ++i) {
-        const int8_t *from = base[i < BM / 32 ? 0 : 1 + (i - BM / 32) % PAIR] + k;
-        __builtin_amdgcn_global_load_lds((GlobalPtr)(from + off[i]), (LdsPtr)(stage + (i * 4 + wave) * 1024), 16, 0, 0);
-      }
-    } else {
+    for (int i = from; i < to; ++i) {
+      const int8_t *p = base[i < BM / 32 ? 0 : 1 + (i - BM / 32) % PAIR] + k;
+      __builtin_amdgcn_global_load_lds((GlobalPtr)(p + off[i]), (LdsPtr)(stage + (i * 4 + wave) * 1024), 16, 0, 0);
+    }
+  };
+  auto load_end = [&](int8_t *stage, int k, int from, int to) {
 #pragma unroll
-      for (int i = 0; i < C::kLoads; ++i) {
-        const int8_t *from = base[i < BM / 32 ? 0 : 1 + (i - BM / 32) % PAIR] + k;
-        const void *p = k + piece < a.K ? (const void *)(from + off[i]) : (const void *)&zeros;
-        __builtin_amdgcn_global_load_lds((GlobalPtr)p, (LdsPtr)(stage + (i * 4 + wave) * 1024), 16, 0, 0);
-      }
+    for (int i = from; i < to; ++i) {
+      const int8_t *p = base[i < BM / 32 ? 0 : 1 + (i - BM / 32) % PAIR] + k;
+      const void *q = k + piece < a.K ? (const void *)(p + off[i]) : (const void *)&zeros;
+      __builtin_amdgcn_global_load_lds((GlobalPtr)q, (LdsPtr)(stage + (i * 4 + wave) * 1024), 16, 0, 0);
     }
   };
   i32x16 acc[C::kMi][C::kNi] = {};
@@ -195,7 +447,7 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) int8_tile_ke
   };
   // the operands of 32 k
   auto read = [&](const int8_t *stage, int kk, Pieces &f) {
-    const int p = ((kk * 2 + lane / 32) ^ (lane % 8)) * 16;
+    const int p = ((kk * 2 + lane / 32) ^ (lane / 2 % 8)) * 16;
 #pragma unroll
     for (int i = 0; i < C::kMi; ++i) f.a[i] = *reinterpret_cast<const i32x4 *>(stage + ar + i * 4096 + p);
 #pragma unroll
@@ -208,41 +460,91 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) int8_tile_ke
       for (int j = 0; j < C::kNi; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
   };
-  // All of this wave's loads are there and what it read is in registers; then the
-  // same of the other waves: the stage that was read may be loaded anew.
+  // This wave's loads of the next stage are there (at most those of the D - 2 stages
+  // behind it are not) and what it read is in registers; then the same of the other
+  // waves: the stage that was read may be loaded anew.
   auto arrive = [&] {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0)
+    wait_loads<(D - 2) * C::kLoads>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
   Pieces f, g;
   // A stage: each 32 k's operands are read while the 32 k before are multiplied,
-  // the next stage's first ones too; the stage after it is loaded into this one.
-  auto step = [&](int8_t *cur, int8_t *next, int k) {
+  // the next stage's first ones too.  When all waves have read a stage, the one
+  // that is D further on is loaded into it, kEarly loads at once, the others (of two
+  // stages) with the next stage's first products.  `whole`: these loads lie within
+  // the rows.
+  auto step = [&](int8_t *cur, int8_t *next, int k, auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;
+    constexpr int kP = C::kMi * C::kNi, kR = C::kMi + C::kNi;
+    if constexpr (kEarly < C::kLoads) {
+      if constexpr (kWhole) load(next, k + 128, kEarly, C::kLoads);
+      else load_end(next, k + 128, kEarly, C::kLoads);
+    }
     read(cur, 1, g);
     products(f);
+    if constexpr (kWhole) interleave<kP, kR, C::kLoads - kEarly>();
     read(cur, 2, f);
     products(g);
+    if constexpr (kWhole) interleave<kP, kR, 0>();
     read(cur, 3, g);
     products(f);
+    if constexpr (kWhole) interleave<kP, kR, 0>();
     arrive();
+    if constexpr (kWhole) load(cur, k + 128 * D, 0, kEarly);
+    else load_end(cur, k + 128 * D, 0, kEarly);
     read(next, 0, f);
-    load(cur, k + 256);
     products(g);
+    if constexpr (kWhole) interleave<kP, kR, kEarly>();
   };
-  load(even, 0);
-  arrive();
-  load(odd, 128);
-  read(even, 0, f);
-  for (int k = 0; k < a.K; k += 256) {
-    step(even, odd, k);
-    step(odd, even, k + 128);
+  int k = 0;
+  if constexpr (D == 4) {
+    load_end(s0, 0, 0, C::kLoads);
+    load_end(s1, 128, 0, C::kLoads);
+    load_end(s2, 256, 0, C::kLoads);
+    arrive();
+    load_end(s3, 384, 0, C::kLoads);
+    read(s0, 0, f);
+    for (; k + 1024 <= a.K; k += 512) {
+      step(s0, s1, k, std::true_type());
+      step(s1, s2, k + 128, std::true_type());
+      step(s2, s3, k + 256, std::true_type());
+      step(s3, s0, k + 384, std::true_type());
+    }
+    for (; k < a.K; k += 512) {
+      step(s0, s1, k, std::false_type());
+      if (k + 128 >= a.K) break;
+      step(s1, s2, k + 128, std::false_type());
+      if (k + 256 >= a.K) break;
+      step(s2, s3, k + 256, std::false_type());
+      if (k + 384 >= a.K) break;
+      step(s3, s0, k + 384, std::false_type());
+    }
+  } else {
+    // (stages behind the end are zeros: a loop with an exit in the middle would have
+    // the compiler move all sums between registers)
+    load_end(s0, 0, 0, C::kLoads);
+    arrive();
+    load_end(s1, 128, 0, kEarly);
+    read(s0, 0, f);
+    for (; k + 512 <= a.K; k += 256) {
+      step(s0, s1, k, std::true_type());
+      step(s1, s0, k + 128, std::true_type());
+    }
+    for (; k < a.K; k += 256) {
+      step(s0, s1, k, std::false_type());
+      step(s1, s0, k + 128, std::false_type());
+    }
   }
-  arrive();
+  wait_loads<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
   // The sums go through LDS, 32 tokens of a wave at a time, so that a thread has
   // eight channels of a token and stores are whole lines.
-  int *const out = reinterpret_cast<int *>(wm ? odd : even) + wn * 32 * C::kOutLd;
+  __shared__ float xs_of[BM];
+  for (int r = tid; r < BM; r += 256) xs_of[r] = a.xs[min(m0 + r, a.M - 1)];
+  __syncthreads();
+  int *const out = reinterpret_cast<int *>(wm ? s1 : s0) + wn * 32 * C::kOutLd;
   constexpr int kCols = BN / 2 / PAIR, kLanes = kCols / 8, kRows = 64 / kLanes;
   const int c = lane % kLanes * 8, n = n0 + wn * kCols + c;
   const int at = PAIR == 2 ? c / 32 * 64 + c % 32 : c;
@@ -267,7 +569,7 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) int8_tile_ke
     for (int r = lane / kLanes; r < 32; r += kRows) {
       const int m = m0 + wm * (BM / 2) + i * 32 + r;
       if (m >= a.M || n >= a.N) continue;
-      const float xs = a.xs[m];
+      const float xs = xs_of[wm * (BM / 2) + i * 32 + r];
       const int *s = out + r * C::kOutLd + at;
       float v[8];
 #pragma unroll
@@ -285,24 +587,45 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) int8_tile_ke
   }
 }
 
-template <int TM, int TN, int PAIR>
-hipError_t few(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
-  const dim3 grid((unsigned)((a.N + 16 * TN - 1) / (16 * TN)), (unsigned)((a.M + 16 * TM - 1) / (16 * TM)));
-  return launch_timed(int8_few_kernel<TM, TN, PAIR>, grid, kFewWaves * 64, stream, ev, done, a);
+template <int PAIR>
+hipError_t row(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
+  // as many workgroups as a compute unit's LDS holds (37 KB each), each with the same number of tiles
+  const int tiles = (a.N + 15) / 16, most = 4 * kSplitCUs, turns = (tiles + most - 1) / most;
+  return launch_timed(int8_row_kernel<PAIR>, dim3((unsigned)((tiles + turns - 1) / turns)), kRowWaves * 64, stream, ev,
+                      done, a);
+}
+template <int TM, int PAIR, int WAVES>
+hipError_t split(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
+  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * TM - 1) / (16 * TM)));
+  return launch_timed(int8_split_kernel<TM, PAIR, WAVES>, grid, WAVES * 64, stream, ev, done, a);
 }
 template <int BM, int BN, int PAIR>
+int64_t tile_count(const Int8Args &a) {
+  return (int64_t)((a.M + BM - 1) / BM) * ((a.N + BN / PAIR - 1) / (BN / PAIR));
+}
+template <int BM, int BN, int PAIR, int D>
 hipError_t tiles(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
-  const int64_t n = (int64_t)((a.M + BM - 1) / BM) * ((a.N + BN / PAIR - 1) / (BN / PAIR));
-  return launch_timed(int8_tile_kernel<BM, BN, PAIR>, dim3((unsigned)n), 256, stream, ev, done, a);
+  return launch_timed(int8_tile_kernel<BM, BN, PAIR, D>, dim3((unsigned)tile_count<BM, BN, PAIR>(a)), 256, stream, ev,
+                      done, a);
 }
 
 template <int PAIR>
 hipError_t int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
-  if (a.M <= 16) return few<1, 1, PAIR>(a, stream, ev, done);
-  if (a.M <= 32) return few<2, 1, PAIR>(a, stream, ev, done);
-  if (a.M <= 64) return few<4, 1, PAIR>(a, stream, ev, done);
-  if (a.M <= 512) return tiles<128, 128, PAIR>(a, stream, ev, done);
-  return tiles<256, 256, PAIR>(a, stream, ev, done);
+  if (int8_row(a.M, a.K)) return row<PAIR>(a, stream, ev, done);
+  const int64_t strips = (a.N + 15) / 16, groups = (a.M + 63) / 64;
+  if (a.M <= 16 && strips <= 768)
+    return strips <= 256 ? split<1, PAIR, 8>(a, stream, ev, done) : split<1, PAIR, 4>(a, stream, ev, done);
+  if (a.M <= 32 && strips <= 512)
+    return strips <= 256 ? split<2, PAIR, 8>(a, stream, ev, done) : split<2, PAIR, 4>(a, stream, ev, done);
+  if (strips * groups * PAIR <= 512) return split<4, PAIR, 4>(a, stream, ev, done);
+  if (tile_count<64, 128, PAIR>(a) <= kSplitCUs) return tiles<64, 128, PAIR, 4>(a, stream, ev, done);
+  if (a.M <= 64) return tiles<64, 128, PAIR, 2>(a, stream, ev, done);
+  const int64_t mid = tile_count<128, 128, PAIR>(a), large = tile_count<256, 256, PAIR>(a);
+  if (mid <= kSplitCUs) return tiles<128, 128, PAIR, 4>(a, stream, ev, done);
+  // rounds of a workgroup per compute unit, and of two that take 0.575 of its time
+  const double mid_time = 0.575 * (double)((mid + 2 * kSplitCUs - 1) / (2 * kSplitCUs));
+  return mid_time < (double)((large + kSplitCUs - 1) / kSplitCUs) ? tiles<128, 128, PAIR, 2>(a, stream, ev, done)
+                                                                : tiles<256, 256, PAIR, 2>(a, stream, ev, done);
 }
 
 }  // namespace

@@ -191,21 +191,6 @@ __device__ __forceinline__ void norm_row(const NormArg &n, int C, int t, float (
   }
 }
 
-// v / scale to the nearest integer, ties to even, as if the quotient were exact:
-// v * inv is off by less than 2^-15, so that only next to a half does it not tell;
-// there v is compared with the half times the scale, which binary64 holds exactly.
-__device__ __forceinline__ int quantised(float v, float inv, float scale) {
-  const float a = fabsf(v), t = a * inv;
-  float q = rintf(t);
-  const float half = rintf(t - 0.5f) + 0.5f;
-  if (fabsf(t - half) < 0.000244140625f) {
-    const double edge = (double)half * (double)scale;
-    const float low = half - 0.5f;
-    q = (double)a > edge ? low + 1.0f : (double)a < edge ? low : rintf(half);
-  }
-  return (int)copysignf(q, v);
-}
-
 // Threads of a workgroup: several rows where a row has one wave.
 template <int G>
 constexpr int kNormThreads = G > 256 ? G : 256;
@@ -259,17 +244,14 @@ __global__ void __launch_bounds__(kNormThreads<G>) block_norm_kernel(BlockNormAr
     write_row<V, P, G>(a.out, row, a.C, t, v);
     return;
   }
-  // The largest magnitude by its bits: a NaN's are above an infinity's, and those
-  // above every number's.
   uint32_t most = 0;
 #pragma unroll
   for (int j = 0; j < P; ++j)
 #pragma unroll
     for (int e = 0; e < V; ++e) most = max(most, __float_as_uint(v[j][e]) & 0x7FFFFFFFu);
   most = row_max<G>(most, reinterpret_cast<uint32_t *>(slots[4]), t);
-  const bool finite = most < 0x7F800000u, some = finite && most >= 0x0D800000u;   // 2^-100
-  const float scale = some ? __uint_as_float(most) / 127.0f : finite ? 0.0f : __uint_as_float(0x7FC00000u);
-  const float inv = some ? 1.0f / scale : 0.0f;
+  float inv;
+  const float scale = scale_of(most, &inv);
   if (t == 0) a.out.scales[row] = scale;
   int8_t *p = static_cast<int8_t *>(a.out.p) + row * a.out.ld;
 #pragma unroll
@@ -279,7 +261,7 @@ __global__ void __launch_bounds__(kNormThreads<G>) block_norm_kernel(BlockNormAr
     uint32_t u[(V + 3) / 4] = {};
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      u[e / 4] |= (uint32_t)(some ? quantised(v[j][e], inv, scale) & 255 : 0) << (8 * (e % 4));
+      u[e / 4] |= (uint32_t)(inv > 0.0f ? quantised(v[j][e], inv, scale) & 255 : 0) << (8 * (e % 4));
     if constexpr (V == 8) *reinterpret_cast<uint2 *>(p + c) = make_uint2(u[0], u[1]);
     else p[c] = (int8_t)u[0];
   }

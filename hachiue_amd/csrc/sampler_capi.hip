@@ -1802,7 +1802,9 @@ int int8_args(int32_t M, const hs_rows *x, const hs_weights *w0, const hs_weight
   c.g.K = K;
   c.g.pair = w1 != nullptr;
   c.g.act = act;
-  if (xr.type != hs::kT_I8) {
+  if (xr.type != hs::kT_I8 && hs::int8_row(M, K)) {
+    c.g.rows = xr;
+  } else if (xr.type != hs::kT_I8) {
     c.pre.M = M;
     c.pre.C = K;
     c.pre.scale = 1.0f;
