@@ -41,7 +41,6 @@ struct BlockNormArgs {
   NormArg after, before;
   int32_t M, C, act;
   float scale;
-  int32_t vec;               // everything is aligned for 8 elements at a time
 };
 hipError_t launch_block_norm(const BlockNormArgs &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done);
 
@@ -69,6 +68,27 @@ inline bool int8_row(int32_t M, int32_t K) { return M == 1 && K <= kInt8RowK; }
 hipError_t launch_int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done);
 
 #ifdef __HIPCC__
+// A wave's sum or maximum, in every lane: within rows of 16 lanes by DPP, then the
+// four rows' by scalars (no LDS: 30 clocks where six shuffles take 400).
+template <typename F>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t v, F both) {
+  v = both(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));    // lane ^ 1
+  v = both(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));    // lane ^ 2
+  v = both(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));   // 7 - lane of 8
+  v = both(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));   // 15 - lane of 16
+  const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)v, 0), b = (uint32_t)__builtin_amdgcn_readlane((int)v, 16);
+  const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)v, 32), d = (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
+  return both(both(a, b), both(c, d));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return __uint_as_float(wave_reduce(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  return wave_reduce(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+
 // One launch; with events its start and end, else the end of it in `done`.
 template <typename F, typename A>
 hipError_t launch_timed(F kernel, dim3 grid, int threads, hipStream_t stream, hipEvent_t *ev, hipEvent_t done,
@@ -114,11 +134,12 @@ __device__ __forceinline__ float activation(int act, float v) {
 }
 
 // The scale of a row whose largest magnitude has the bits `most` (a NaN's are above
-// an infinity's, and those above every number's): NaN where it is not finite, 0
-// below 2^-100.  *inv: 1 / scale, or 0 where the row's integers are 0.
+// an infinity's, and those above every number's): that magnitude times 1 / 127, both
+// in binary32; NaN where it is not finite, 0 below 2^-100.  *inv: 1 / scale, or 0
+// where the row's integers are 0.
 __device__ __forceinline__ float scale_of(uint32_t most, float *inv) {
   const bool finite = most < 0x7F800000u, some = finite && most >= 0x0D800000u;
-  const float scale = some ? __uint_as_float(most) / 127.0f : finite ? 0.0f : __uint_as_float(0x7FC00000u);
+  const float scale = some ? __uint_as_float(most) * (1.0f / 127.0f) : finite ? 0.0f : __uint_as_float(0x7FC00000u);
   *inv = some ? 1.0f / scale : 0.0f;
   return scale;
 }
@@ -129,12 +150,34 @@ __device__ __forceinline__ int quantised(float v, float inv, float scale) {
   const float a = fabsf(v), t = a * inv;
   float q = rintf(t);
   const float half = rintf(t - 0.5f) + 0.5f;
-  if (fabsf(t - half) < 0.000244140625f) {
+  if (fabsf(t - half) < 0.000030517578f) {
     const double edge = (double)half * (double)scale;
     const float low = half - 0.5f;
     q = (double)a > edge ? low + 1.0f : (double)a < edge ? low : rintf(half);
   }
   return (int)copysignf(q, v);
+}
+// The same of n values, four to a word: six instructions each where none of a
+// wave's lies next to a half.  1.5 * 2^23 + t is rounded to an integer, which its low
+// bits are.
+template <int n>
+__device__ __forceinline__ void quantised_bytes(const float (&v)[n], float inv, float scale, uint32_t (&u)[n / 4]) {
+  uint32_t r[n];
+  float most = 0.0f;
+#pragma unroll
+  for (int e = 0; e < n; ++e) {
+    const float t = v[e] * inv, up = t + 12582912.0f;
+    r[e] = __float_as_uint(up);
+    most = fmaxf(most, fabsf(t - (up - 12582912.0f)));
+  }
+  if (most > 0.5f - 0.000030517578f) {
+#pragma unroll
+    for (int e = 0; e < n; ++e) r[e] = (uint32_t)quantised(v[e], inv, scale);
+  }
+#pragma unroll
+  for (int e = 0; e < n; e += 4)
+    u[e / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(r[e + 3], r[e + 2], 0x0C0C0400u),
+                                     __builtin_amdgcn_perm(r[e + 1], r[e], 0x0C0C0400u), 0x05040100u);
 }
 
 __device__ __forceinline__ uint16_t bits16(int type, float v) {

@@ -106,8 +106,7 @@ __device__ __forceinline__ void keep_row(const Int8Args &a, int8_t *q, float *sc
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < kHeld; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+  top = wave_max(top);
   if (t % 64 == 0) most[t / 64] = top;
   meet();
 #pragma unroll

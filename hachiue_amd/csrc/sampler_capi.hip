@@ -1632,21 +1632,6 @@ int norm_arg(const hs_norm &n, const char *what, hs::NormArg &a) {
 
 bool act_known(int32_t act) { return act >= HS_ACT_NONE && act <= HS_ACT_TANH; }
 
-// Whether a row kernel may take 8 elements at a time of each tensor.
-bool wide_rows(const hs::BlockNormArgs &g) {
-  if (g.C % 8) return false;
-  uintptr_t bits = 0;
-  for (const hs::RowsArg *r : {&g.x, &g.gate, &g.res, &g.sum, &g.out}) {
-    if (!r->p) continue;
-    // (8 8-bit elements are 8 bytes)
-    const uintptr_t b = reinterpret_cast<uintptr_t>(r->p) | (uintptr_t)(r->ld * hs::row_elem_bytes(r->type));
-    bits |= r->type == hs::kT_I8 ? b * 2 : b;
-  }
-  for (const hs::NormArg *n : {&g.after, &g.before})
-    bits |= reinterpret_cast<uintptr_t>(n->w) | reinterpret_cast<uintptr_t>(n->b);
-  return (bits & 15u) == 0;
-}
-
 // The checks of a block norm; *skip: nothing to do.
 int block_norm_args(const hs_block_norm *n, hs::BlockNormArgs &g, bool *skip) {
   if (!n) return fail(HS_ERR_INVALID_ARGUMENT, "null norm");
@@ -1698,7 +1683,6 @@ int block_norm_args(const hs_block_norm *n, hs::BlockNormArgs &g, bool *skip) {
   g.C = (int32_t)C;
   g.act = n->gate_act;
   g.scale = n->scale;
-  g.vec = wide_rows(g);
   return HS_OK;
 }
 
@@ -1846,7 +1830,6 @@ int int8_run(hs_context *ctx, Int8Call &c, hipStream_t stream) {
     c.g.y.type = hs::kT_F32;
     c.post.x = c.g.y;
     c.post.x.scales = nullptr;
-    c.post.vec = wide_rows(c.post);
   }
   c.g.wide = ((reinterpret_cast<uintptr_t>(c.g.y.p) | (uintptr_t)(c.g.y.ld * hs::row_elem_bytes(c.g.y.type))) & 15u) == 0;
   hipError_t e = hipSuccess;
@@ -1856,7 +1839,6 @@ int int8_run(hs_context *ctx, Int8Call &c, hipStream_t stream) {
     c.pre.out.ld = K;
     c.pre.out.scales = reinterpret_cast<float *>(q + M * K);
     c.pre.out.type = hs::kT_I8;
-    c.pre.vec = wide_rows(c.pre);
     e = inject_failure() ? hipErrorOutOfMemory : hs::launch_block_norm(c.pre, stream, of(hs::kNormTimedSlot), nullptr);
     c.g.x = reinterpret_cast<const int8_t *>(q);
     c.g.ldx = K;

@@ -511,7 +511,7 @@ typedef struct hs_norm {
  * is before it is rounded to sum's type).  x, gate, residual and sum are float rows;
  * gate (absent: 1) has a row for each row, or one for all of them with stride 0;
  * residual absent: 0; sum or out may be absent.  out may be I8: then its
- * scale is max|out| / 127 of the row, rounded to binary32, and its integers
+ * scale is max|out| of the row times 1 / 127, both in binary32, and its integers
  * out / scale to the nearest, ties to even; a row whose largest magnitude is
  * below 2^-100 gets scale 0 and zeros, one with a NaN or an infinity scale NaN
  * and zeros, so that its products are NaN.  With both norms HS_NORM_NONE

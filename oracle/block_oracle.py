@@ -117,12 +117,12 @@ def rounded(bound, want, kind):
 
 def quantise(v):
     """Integers and scales of binary32 rows, exactly as promised: scale =
-    binary32(max / 127), integers by the exact quotient, ties to even."""
+    max * binary32(1 / 127) in binary32, integers by the exact quotient, ties to even."""
     v = np.asarray(v, np.float32)
     most = np.abs(v).max(1)
     bad = ~np.isfinite(v).all(1)
     zero = ~bad & (most < np.float32(2.0 ** -100))
-    scale = np.where(bad, np.float32(np.nan), np.where(zero, np.float32(0), most / np.float32(127)))
+    scale = np.where(bad, np.float32(np.nan), np.where(zero, np.float32(0), most * (np.float32(1) / np.float32(127))))
     live = ~bad & ~zero
     q = np.zeros(v.shape, np.int8)
     # a quotient of two binary32 values is a half of an odd integer below 256 or
