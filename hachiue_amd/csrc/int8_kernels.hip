@@ -608,6 +608,26 @@ hipError_t tiles(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent
                       done, a);
 }
 
+// How long `count` tiles of `stages` 128 k take, `slots` of them at a time: in us, a
+// stage's and an epilogue's share, and of a round that is not full its idle part
+// costs the less, the more of it there is (fewer units run faster).  Measured over
+// 300 to 4096 tokens by 2048 to 20000 channels and K of 1024 to 8192, 36 cases: the
+// faster of 128 x 128 and 256 x 256 was chosen in 33, and the others' loss was
+// below 8 %.
+inline double rounds_time(int64_t count, int slots, double idle, double stage, double rest, int64_t stages) {
+  const int64_t full = count / slots, left = count % slots;
+  const double rounds = (double)full + (left ? idle + (1.0 - idle) * (double)left / slots : 0.0);
+  return rounds * (stage * (double)stages + rest);
+}
+
+// Which kernel.  us at K = 4096 unless said (2048 for 151936 channels and 40000):
+//   one token: 52 over 151936 channels, 7.3 over 4096 (the split kernel 84, 6.5)
+//   K split among 8 waves up to 256 strips of 16 channels, among 4 above: 16 tokens
+//   over 4096 6.7 and 7.5, over 8192 11.7 and 10.3 (tiles of four stages 12.6, 12.6)
+//   tiles of 64 x 128: 16 tokens over 16384 16 (split 19), over 151936 57 (95); 64
+//   over 4096 13 (split 10), over 16384 19 (27); of two stages, three workgroups a
+//   unit, above a workgroup a unit: 64 over 40000 23 (four stages 27), over 4096 20 (13)
+//   tiles of 128 x 128 of four stages: 1024 over 4096 22 (two stages 26, 64 x 128 25)
 template <int PAIR>
 hipError_t int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
   if (int8_row(a.M, a.K)) return row<PAIR>(a, stream, ev, done);
@@ -619,12 +639,12 @@ hipError_t int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_
   if (strips * groups * PAIR <= 512) return split<4, PAIR, 4>(a, stream, ev, done);
   if (tile_count<64, 128, PAIR>(a) <= kSplitCUs) return tiles<64, 128, PAIR, 4>(a, stream, ev, done);
   if (a.M <= 64) return tiles<64, 128, PAIR, 2>(a, stream, ev, done);
-  const int64_t mid = tile_count<128, 128, PAIR>(a), large = tile_count<256, 256, PAIR>(a);
+  const int64_t mid = tile_count<128, 128, PAIR>(a), large = tile_count<256, 256, PAIR>(a), stages = (a.K + 127) / 128;
   if (mid <= kSplitCUs) return tiles<128, 128, PAIR, 4>(a, stream, ev, done);
-  // rounds of a workgroup per compute unit, and of two that take 0.575 of its time
-  const double mid_time = 0.575 * (double)((mid + 2 * kSplitCUs - 1) / (2 * kSplitCUs));
-  return mid_time < (double)((large + kSplitCUs - 1) / kSplitCUs) ? tiles<128, 128, PAIR, 2>(a, stream, ev, done)
-                                                                : tiles<256, 256, PAIR, 2>(a, stream, ev, done);
+  const double mid_us = rounds_time(mid, 2 * kSplitCUs, 0.5, 1.12, PAIR == 2 ? 5.5 : 4.2, stages);
+  const double large_us = rounds_time(large, kSplitCUs, 0.6, 1.7, PAIR == 2 ? 20.0 : 11.5, stages);
+  return mid_us < large_us ? tiles<128, 128, PAIR, 2>(a, stream, ev, done)
+                           : tiles<256, 256, PAIR, 2>(a, stream, ev, done);
 }
 
 }  // namespace
