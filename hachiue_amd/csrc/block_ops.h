@@ -120,16 +120,23 @@ __device__ __forceinline__ float logistic(float v, float z) {
   return v * fmaf(fmaf(-d, q, n), r, q);
 }
 
-__device__ __forceinline__ float activation(int act, float v) {
+// (the choice outside of the loops: n independent chains of instructions, not n
+// branches.  4096 tokens' gated pairs, 128 results a lane of each tile: 451 us with
+// the branches.)
+template <int n>
+__device__ __forceinline__ void activate(int act, float (&v)[n]) {
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int e = 0; e < n; ++e) v[e] = f(v[e]);
+  };
   switch (act) {
-    case kActSilu: return logistic(v, v);
-    case kActGelu: return 0.5f * v * erfcf(v * -0.70710678f);   // (no cancellation for v << 0)
+    case kActSilu: return each([](float x) { return logistic(x, x); });
+    case kActGelu: return each([](float x) { return 0.5f * x * erfcf(x * -0.70710678f); });   // (no cancellation for x << 0)
     case kActGeluTanh:   // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u))
-      return logistic(v, 1.59576912f * fmaf(0.044715f * v * v, v, v));
-    case kActRelu: return v > 0.0f ? v : v != v ? v : 0.0f;
-    case kActSigmoid: return v != v ? v : logistic(1.0f, v);
-    case kActTanh: return tanhf(v);
-    default: return v;
+      return each([](float x) { return logistic(x, 1.59576912f * fmaf(0.044715f * x * x, x, x)); });
+    case kActRelu: return each([](float x) { return x > 0.0f ? x : x != x ? x : 0.0f; });
+    case kActSigmoid: return each([](float x) { return x != x ? x : logistic(1.0f, x); });
+    case kActTanh: return each([](float x) { return tanhf(x); });
   }
 }
 

@@ -218,10 +218,14 @@ __global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
       for (int p = 0; p < PAIR; ++p)
 #pragma unroll
         for (int v = 0; v < W; ++v) s[p] += part[done % 2][v][p][lane];
-      float v = scaled(s[0], scale, a.ws[0][n]);
-      if constexpr (PAIR == 2) v = activation(a.act, v) * scaled(s[PAIR - 1], scale, a.ws[PAIR - 1][n]);
-      else if (a.bias) v += a.bias[n];
-      put(a.y, 0, n, v);
+      float v[1] = {scaled(s[0], scale, a.ws[0][n])};
+      if constexpr (PAIR == 2) {
+        activate<1>(a.act, v);
+        v[0] *= scaled(s[PAIR - 1], scale, a.ws[PAIR - 1][n]);
+      } else if (a.bias) {
+        v[0] += a.bias[n];
+      }
+      put(a.y, 0, n, v[0]);
     }
     ++done;
     tile += gridDim.x;
@@ -343,14 +347,20 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
     const int m = m0 + tile * 16 + lane % 16, n = n0 + lane / 16 * 4;
     if (m >= a.M) continue;
     const float xs = a.xs[m];
+    float v[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (n + r >= a.N) break;
-      float v = scaled(s[0][r], xs, a.ws[0][n + r]);
-      if constexpr (PAIR == 2) v = activation(a.act, v) * scaled(s[PAIR - 1][r], xs, a.ws[PAIR - 1][n + r]);
-      else if (a.bias) v += a.bias[n + r];
-      put(a.y, m, n + r, v);
+    for (int r = 0; r < 4; ++r) v[r] = scaled(s[0][r], xs, a.ws[0][min(n + r, a.N - 1)]);
+    if constexpr (PAIR == 2) {
+      activate<4>(a.act, v);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] *= scaled(s[PAIR - 1][r], xs, a.ws[PAIR - 1][min(n + r, a.N - 1)]);
+    } else if (a.bias) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += a.bias[min(n + r, a.N - 1)];
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < a.N) put(a.y, m, n + r, v[r]);
   }
 }
 
@@ -565,7 +575,8 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int
     // (a wave's own part of LDS, its accesses are in order)
     asm volatile("" ::: "memory");
 #pragma unroll 1
-    for (int r = lane / kLanes; r < 32; r += kRows) {
+    for (int r0 = 0; r0 < 32; r0 += kRows) {
+      const int r = r0 + lane / kLanes;
       const int m = m0 + wm * (BM / 2) + i * 32 + r;
       if (m >= a.M || n >= a.N) continue;
       const float xs = xs_of[wm * (BM / 2) + i * 32 + r];
@@ -574,8 +585,9 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = scaled(s[e], xs, w0[e]);
       if constexpr (PAIR == 2) {
+        activate<8>(a.act, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = activation(a.act, v[e]) * scaled(s[32 + e], xs, w1[e]);
+        for (int e = 0; e < 8; ++e) v[e] *= scaled(s[32 + e], xs, w1[e]);
       } else if (a.bias) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += bias[e];

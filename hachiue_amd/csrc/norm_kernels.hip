@@ -223,8 +223,9 @@ __global__ void __launch_bounds__(kNormThreads<G>) block_norm_kernel(BlockNormAr
     for (int j = 0; j < P; ++j) {
       float g[8];
       widen_raw(a.gate.type, raw[j], g);
+      activate<8>(a.act, g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] *= activation(a.act, g[e]);
+      for (int e = 0; e < 8; ++e) v[j][e] *= g[e];
     }
   }
 #pragma unroll
@@ -298,7 +299,7 @@ hipError_t launch(const BlockNormArgs &a, hipStream_t stream, hipEvent_t *ev, hi
 hipError_t launch_block_norm(const BlockNormArgs &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
   const int C = a.C;
   if (C <= 512) return launch<1, 64>(a, stream, ev, done);
-  if (C <= 1024) return launch<2, 64>(a, stream, ev, done);
+  if (C <= 1024 && a.M > 2 * kSplitCUs) return launch<2, 64>(a, stream, ev, done);
   if (C <= 2048) return launch<1, 256>(a, stream, ev, done);
   if (C <= 4096) return a.M <= kSplitCUs ? launch<1, 512>(a, stream, ev, done) : launch<2, 256>(a, stream, ev, done);
   if (C <= 8192) return a.M <= kSplitCUs ? launch<1, 1024>(a, stream, ev, done) : launch<2, 512>(a, stream, ev, done);
