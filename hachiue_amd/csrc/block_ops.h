@@ -46,6 +46,7 @@ hipError_t launch_block_norm(const BlockNormArgs &a, hipStream_t stream, hipEven
 
 // y[m][n] = xs[m] * ws[n] * sum_k x[m][k] w[n][k] + bias[n], and with a second
 // weight act(the first's) * the second's.
+constexpr int64_t kInt8MaxResults = (int64_t)1 << 36;   // (grids below 2^32 threads)
 constexpr int kInt8MaxM = 1 << 20, kInt8MaxN = 1 << 24, kNormMaxM = 1 << 24;
 constexpr int64_t kInt8MaxLd = 1 << 23;   // 255 rows of it below 2^31
 constexpr int kInt8MaxK = 65536;   // 2^16 * 2^14 below 2^31: the sums are exact

@@ -203,12 +203,15 @@ __device__ __forceinline__ void norm_row(const NormArg &n, int C, int t, float (
 // Threads of a workgroup: several rows where a row has one wave.
 template <int G>
 constexpr int kNormThreads = G > 256 ? G : 256;
+// Workgroups of a grid's first dimension (2^32 threads of one are too many).
+constexpr unsigned kGridX = 1u << 16;
 
 template <int P, int G, bool WHOLE>
 __global__ void __launch_bounds__(kNormThreads<G>) block_norm_kernel(BlockNormArgs a) {
   __shared__ float slots[5][16];
   const int t = threadIdx.x % G;
-  const int64_t row = (int64_t)blockIdx.x * (kNormThreads<G> / G) + threadIdx.x / G;
+  const int64_t group = (int64_t)blockIdx.y * kGridX + blockIdx.x;
+  const int64_t row = group * (kNormThreads<G> / G) + threadIdx.x / G;
   if (row >= a.M) return;   // (whole waves; with barriers, G is the workgroup)
   Raw raw[P], res[P];
   float v[P][8];
@@ -284,7 +287,8 @@ __global__ void __launch_bounds__(kNormThreads<G>) block_norm_kernel(BlockNormAr
 template <int P, int G>
 hipError_t launch(const BlockNormArgs &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
   constexpr int per = kNormThreads<G> / G;
-  const dim3 grid((unsigned)((a.M + per - 1) / per));
+  const unsigned groups = (unsigned)((a.M + per - 1) / per), x = std::min(groups, kGridX);
+  const dim3 grid(x, (groups + x - 1) / x);
   return a.C % 8 ? launch_timed(block_norm_kernel<P, G, false>, grid, kNormThreads<G>, stream, ev, done, a)
                  : launch_timed(block_norm_kernel<P, G, true>, grid, kNormThreads<G>, stream, ev, done, a);
 }

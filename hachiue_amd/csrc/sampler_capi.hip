@@ -806,15 +806,11 @@ int argmax_device(hs_context *ctx, const float *d_logits, int32_t rows, int64_t 
   return leave_stream(ctx, stream, ev == nullptr);
 }
 
-// src/engine.ts:1493-1515 (the lm_head GEMV; see lmhead_kernels.hip).
-// The checks and arguments of an lm_head GEMV call, on the call's stream
-// (entered: enter_stream ran).  A Hadamard-folded weight's input is rotated
-// here, into the workspace, except where the GEMV does it (planar formats, a
-// row at a time).  *skip: nothing to compute (M or N is 0).
-int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *wt,
-               float *d_y, int64_t ldy, hipStream_t stream, bool cap, hs::GemvArgs &g, bool *skip) {
+// The checks of an lm_head GEMV call, apart from what its workspace needs: *bw
+// weights are *bb bytes.
+int gemv_checks(const float *d_x, int32_t M, int64_t ldx, const hs_weights *wt, const float *d_y, int64_t ldy,
+                int *bw_out, int *bb_out, bool *skip) {
   *skip = false;
-  if (!ctx) return fail(HS_ERR_INVALID_ARGUMENT, "null context");
   if (!wt) return fail(HS_ERR_INVALID_ARGUMENT, "null weights");
   const int32_t K = wt->cols, N = wt->rows, w_type = wt->type;
   const void *d_w = wt->data;
@@ -857,6 +853,28 @@ int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const 
   // (Q6_K's slabs read up to 3 KiB past a row's start)
   if ((int64_t)N * row_bytes > (w_type == hs::kW_Q6_K ? 0xFFFF0000LL : 0xFFFFFF00LL))
     return fail(HS_ERR_UNSUPPORTED, "weights of %lld bytes above 4 GiB", (long long)(N * row_bytes));
+  if (M > 65535) return fail(HS_ERR_UNSUPPORTED, "M %d above 65535", M);
+  *bw_out = bw;
+  *bb_out = bb;
+  return HS_OK;
+}
+
+// src/engine.ts:1493-1515 (the lm_head GEMV; see lmhead_kernels.hip).
+// The checks and arguments of an lm_head GEMV call, on the call's stream
+// (entered: enter_stream ran).  A Hadamard-folded weight's input is rotated
+// here, into the workspace, except where the GEMV does it (planar formats, a
+// row at a time).  *skip: nothing to compute (M or N is 0).
+int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *wt,
+               float *d_y, int64_t ldy, hipStream_t stream, bool cap, hs::GemvArgs &g, bool *skip) {
+  *skip = false;
+  if (!ctx) return fail(HS_ERR_INVALID_ARGUMENT, "null context");
+  int bw = 0, bb = 0;
+  const int bad = gemv_checks(d_x, M, ldx, wt, d_y, ldy, &bw, &bb, skip);
+  if (bad || *skip) return bad;
+  const int32_t K = wt->cols, N = wt->rows, w_type = wt->type;
+  const void *d_w = wt->data;
+  const bool planar = hs::tern_quant_bytes(w_type) > 0;
+  const int64_t row_bytes = (int64_t)(K / bw) * bb;
   memset(&g, 0, sizeof g);
   g.x = d_x;
   g.ldx = ldx;
@@ -880,7 +898,6 @@ int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const 
   // at most one wave per row step (the launch caps it at the resident workgroups)
   const int64_t wpb = hs::kGemvThreads / 64;
   g.blocks = (int32_t)std::min<int64_t>((steps + wpb - 1) / wpb, 1 << 20);
-  if (M > 65535) return fail(HS_ERR_UNSUPPORTED, "M %d above 65535", M);
   if (hs::gemv_batched(w_type, M, N, K)) g.tab = ctx->gemv_tab.p;   // several rows: their limb tables
   const bool rotate = wt->hadamard && !(planar && !g.tab);   // (planar rows: by the GEMV itself)
   if (rotate) {
@@ -1678,6 +1695,10 @@ int block_norm_args(const hs_block_norm *n, hs::BlockNormArgs &g, bool *skip) {
     const Span s = {reinterpret_cast<uintptr_t>(g.out.scales), (uint64_t)M * 4, 0, 1};
     for (const hs::RowsArg *r : {&g.x, &g.gate, &g.res, &g.sum, &g.out})
       if (r->p && overlap(s, rows_span(*r, M, C))) return fail(HS_ERR_INVALID_ARGUMENT, "scales overlap rows");
+    for (const hs::NormArg *p : {&g.after, &g.before})
+      for (const float *v : {p->w, p->b})
+        if (v && overlap(s, {reinterpret_cast<uintptr_t>(v), (uint64_t)C * 4, 0, 1}))
+          return fail(HS_ERR_INVALID_ARGUMENT, "scales overlap a norm's parameters");
   }
   g.M = (int32_t)M;
   g.C = (int32_t)C;
@@ -1740,6 +1761,8 @@ int int8_args(int32_t M, const hs_rows *x, const hs_weights *w0, const hs_weight
   if (w1 && !act_known(act)) return fail(HS_ERR_UNSUPPORTED, "activation %d is not supported", act);
   if (M < 0) return fail(HS_ERR_INVALID_ARGUMENT, "M must be >= 0 (got %d)", M);
   if (M > hs::kInt8MaxM) return fail(HS_ERR_UNSUPPORTED, "M %d above 2^20", M);
+  if ((int64_t)M * N > hs::kInt8MaxResults)
+    return fail(HS_ERR_UNSUPPORTED, "%d x %d results above 2^36", M, N);
   if (!x || !y) return fail(HS_ERR_INVALID_ARGUMENT, "x and y must not be null");
   c.skip = M == 0 || N == 0;
   if (c.skip) return HS_OK;
@@ -2303,6 +2326,8 @@ int hs_gated_int_device(hs_context *ctx, int32_t M, const hs_rows *x, const hs_w
   return c.skip ? HS_OK : int8_run(ctx, c, static_cast<hipStream_t>(stream));
 }
 
+// (all that would be refused is, before the norm is enqueued: its sum may be the
+// stream itself)
 int hs_lm_head_norm_sample_device(hs_context *ctx, const hs_block_norm *norm, const hs_weights *w,
                                   float *d_logits, int64_t ldl, const int32_t *d_hist_ids,
                                   const int64_t *d_hist_offsets, const hs_sample_config *configs,
@@ -2331,7 +2356,16 @@ int hs_lm_head_norm_sample_device(hs_context *ctx, const hs_block_norm *norm, co
       if (rc) return rc;
     } else if (i8) {
       return fail(HS_ERR_INVALID_ARGUMENT, "I8 rows need weights of type I8 (type %d)", w->type);
+    } else {
+      int bw = 0, bb = 0;
+      bool none = false;
+      rc = gemv_checks(static_cast<const float *>(norm->out.data), M, norm->out.stride, w, d_logits, ldl, &bw, &bb,
+                       &none);
+      if (rc) return rc;
     }
+    const int64_t chunks = ((int64_t)w->rows + hs::kChunk - 1) / hs::kChunk;   // (as sample_device)
+    if (chunks * hs::kChunkCap > 0x7FFFFFFF / 2 || M * chunks > 0x7FFFFFFF)
+      return fail(HS_ERR_UNSUPPORTED, "vocab %d x rows %d too large", w->rows, M);
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   HS_LOCK(ctx);

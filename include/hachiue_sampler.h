@@ -219,6 +219,8 @@ int hs_gemv_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx,
  *     of K / 128 blocks back to back; 16-byte aligned, PTQ1_0 4-byte),
  *     `scales16` the blocks' binary16 scales in the same order (4-byte
  *     aligned).  hs_split_blocks makes both from GGUF blocks.
+ *   - I8 (24): N rows of K int8, `scales16` their binary32 scales: see
+ *     hs_matmul_int_device below.
  * With `hadamard` set, the GEMV's input is rotated first, as
  * src/engine.ts:1121-1145 does: each 512-block of x is multiplied by
  * `signs` (K floats of +-1, or NULL for none; arch.hadamard's sign vector of
@@ -543,7 +545,8 @@ int hs_block_norm_device(hs_context *ctx, const hs_block_norm *norm, void *strea
  * exact, so that a row's result does not depend on M or on what is beside it.
  * y: float rows, or I8 quantised as above (from binary32 results, in the
  * workspace).  y overlaps none of the inputs.  bias: device [N] binary32 or NULL.
- * M up to 2^20, N up to 2^24 (32768 where y is I8).  Captured calls and the
+ * M up to 2^20, N up to 2^24 (32768 where y is I8), M N up to 2^36, strides of 8-bit
+ * rows x up to 2^23; K of float rows up to 32768.  Captured calls and the
  * workspace as in hs_verify_drafts_device; x in I8 and y in floats need none.
  *
  * hs_gemv_device_ex, hs_lm_head_sample_device_ex, hs_gemv_lora_device and
@@ -560,8 +563,9 @@ int hs_gated_int_device(hs_context *ctx, int32_t M, const hs_rows *x, const hs_w
 
 /* The model's last step from the stream on: hs_block_norm_device, then the
  * lm_head on its `out` (F32, for any weights, or I8 for I8 weights) into
- * d_logits, then sampling, as hs_lm_head_sample_device_ex.  Not to be captured, as
- * hs_lm_head_lora_sample_device. */
+ * d_logits, then sampling, as hs_lm_head_sample_device_ex.  A call that is refused
+ * has enqueued nothing; one that ends with HS_ERR_HIP may have written the norm's
+ * outputs.  Not to be captured, as hs_lm_head_lora_sample_device. */
 int hs_lm_head_norm_sample_device(hs_context *ctx, const hs_block_norm *norm,
                                   const hs_weights *w, float *d_logits, int64_t ldl,
                                   const int32_t *d_hist_ids, const int64_t *d_hist_offsets,

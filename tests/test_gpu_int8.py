@@ -14,7 +14,12 @@ FLOATS = ["f32", "f16", "bf16"]
 # of a step and of a stage
 SIZES = [(1, 1, 16), (1, 100, 64), (2, 17, 48), (5, 300, 1040), (16, 129, 4096), (17, 64, 112), (31, 65, 528),
          (33, 1001, 272), (64, 250, 2064), (65, 127, 144), (77, 1001, 1040), (128, 130, 128), (129, 256, 256),
-         (200, 513, 384), (500, 300, 400), (513, 257, 1296), (700, 1000, 112), (1030, 384, 640)]
+         (200, 513, 384), (500, 300, 400), (513, 257, 1296), (700, 1000, 112), (1030, 384, 640),
+         # one token over tiles enough that a workgroup has several, and longer than
+         # its kernel takes; K split among four waves; tiles of every form
+         (1, 40001, 272), (1, 17000, 2064), (1, 300, 4096), (1, 300, 4112), (9, 8200, 80), (16, 12290, 48),
+         (25, 8190, 1040), (16, 20000, 160), (50, 20001, 64), (64, 33000, 144), (64, 40000, 528),
+         (300, 10000, 656), (70, 33000, 272), (260, 9000, 1200), (1001, 8190, 2576), (1901, 8190, 4112)]
 
 
 def same(got, want, kind):
