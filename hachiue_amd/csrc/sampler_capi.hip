@@ -1619,8 +1619,8 @@ int rows_arg(const hs_rows &r, const char *what, int64_t cols, bool i8, hs::Rows
   if (!r.data) return fail(HS_ERR_INVALID_ARGUMENT, "%s must not be null", what);
   if (r.stride < cols)
     return fail(HS_ERR_INVALID_ARGUMENT, "%s: stride %lld below %lld", what, (long long)r.stride, (long long)cols);
-  if (r.stride > (int64_t)1 << 40)
-    return fail(HS_ERR_UNSUPPORTED, "%s: stride %lld above 2^40", what, (long long)r.stride);
+  if (r.stride > (int64_t)1 << 36)
+    return fail(HS_ERR_UNSUPPORTED, "%s: stride %lld above 2^36", what, (long long)r.stride);
   if (reinterpret_cast<uintptr_t>(r.data) % (uintptr_t)bytes || reinterpret_cast<uintptr_t>(r.scales) % 4)
     return fail(HS_ERR_INVALID_ARGUMENT, "%s must be aligned to their elements", what);
   if ((r.type == hs::kT_I8) != (r.scales != nullptr))

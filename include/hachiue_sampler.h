@@ -477,7 +477,7 @@ int hs_lm_head_lora_sample_device(hs_context *ctx, const float *d_x, int32_t M, 
  * row m stands for data[m][c] * scales[m].  Elements are aligned as such. */
 typedef struct hs_rows {
   int32_t type;
-  int64_t stride;              /* elements from row to row, at least the columns */
+  int64_t stride;              /* elements from row to row: the columns .. 2^36 */
   void *data;                  /* device; NULL: absent, where that is allowed */
   float *scales;               /* device [rows]: I8 only, NULL otherwise */
 } hs_rows;
