@@ -76,49 +76,52 @@ __device__ __forceinline__ void meet() {
 // all 16 columns: they have 30 times the rate that the weights come at.
 constexpr int kRowWaves = 4;
 
-// The row into LDS, zeros behind K (a multiple of 128 bytes), and its scale.
+// The row into LDS, zeros behind K (a multiple of 128 bytes), and its scale.  A thread
+// has 16 elements, all of them or (K is a multiple of 16) none within K.
 __device__ __forceinline__ void keep_row(const Int8Args &a, int8_t *q, float *scale_at, uint32_t *most) {
-  constexpr int kThreads = kRowWaves * 64, kHeld = kInt8RowK / kThreads;
+  static_assert(kInt8RowK == 16 * kRowWaves * 64, "a thread has 16 elements");
   const int t = threadIdx.x, wide = (a.K + 127) / 128 * 128;
+  const bool has = t * 16 < a.K;
+  i32x4 bytes = {};
   if (!a.rows.p) {
-    static_assert(kInt8RowK / 16 == kThreads, "a thread has 16 bytes");
-    if (t * 16 < wide) reinterpret_cast<int4 *>(q)[t] = t * 16 < a.K ? reinterpret_cast<const int4 *>(a.x)[t] : zeros;
+    if (has) bytes = reinterpret_cast<const i32x4 *>(a.x)[t];
     if (t == 0) *scale_at = a.xs[0];
-    return;
-  }
-  float v[kHeld];
-  if (a.rows.type == kT_F32) {
-#pragma unroll
-    for (int e = 0; e < kHeld; ++e) {
-      const int k = t + e * kThreads;
-      v[e] = k < a.K ? static_cast<const float *>(a.rows.p)[k] : 0.0f;
-    }
   } else {
-    uint16_t u[kHeld];
+    typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
+    float v[16] = {};
+    if (has && a.rows.type == kT_F32) {
+      const Any *p = reinterpret_cast<const Any *>(static_cast<const float *>(a.rows.p) + t * 16);
 #pragma unroll
-    for (int e = 0; e < kHeld; ++e) {
-      const int k = t + e * kThreads;
-      u[e] = k < a.K ? static_cast<const uint16_t *>(a.rows.p)[k] : (uint16_t)0;
+      for (int i = 0; i < 4; ++i) {
+        const Any u = p[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * i + e] = __uint_as_float(u[e]);
+      }
+    } else if (has) {
+      const Any *p = reinterpret_cast<const Any *>(static_cast<const uint16_t *>(a.rows.p) + t * 16);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Any u = p[i];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * i + e] = widen16(a.rows.type, (uint16_t)(u[e / 2] >> (16 * (e % 2))));
+      }
     }
+    uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < kHeld; ++e) v[e] = widen16(a.rows.type, u[e]);
+    for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    top = wave_max(top);
+    if (t % 64 == 0) most[t / 64] = top;
+    meet();
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) top = max(top, most[w]);
+    float inv;
+    const float scale = scale_of(top, &inv);
+    if (t == 0) *scale_at = scale;
+    uint32_t u[4] = {};
+    if (inv > 0.0f) quantised_bytes<16>(v, inv, scale, u);
+    bytes = i32x4{(int)u[0], (int)u[1], (int)u[2], (int)u[3]};
   }
-  uint32_t top = 0;
-#pragma unroll
-  for (int e = 0; e < kHeld; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-  top = wave_max(top);
-  if (t % 64 == 0) most[t / 64] = top;
-  meet();
-#pragma unroll
-  for (int w = 0; w < kRowWaves; ++w) top = max(top, most[w]);
-  float inv;
-  const float scale = scale_of(top, &inv);
-  if (t == 0) *scale_at = scale;
-#pragma unroll
-  for (int e = 0; e < kHeld; ++e) {
-    const int k = t + e * kThreads;
-    if (k < wide) q[k] = k < a.K && inv > 0.0f ? (int8_t)quantised(v[e], inv, scale) : (int8_t)0;
-  }
+  if (t * 16 < wide) reinterpret_cast<i32x4 *>(q)[t] = bytes;
 }
 
 template <int PAIR>
