@@ -20,6 +20,17 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 typedef const __attribute__((address_space(1))) void *GlobalPtr;
 typedef __attribute__((address_space(3))) void *LdsPtr;
+// 16 bytes a lane to LDS.  ONCE: nobody reads them again (non-temporal), which weights
+// of more than kOnceBytes are told where one tile of tokens reads them: 49.1 us for
+// the lm_head of one token (53.5), 65 of 64 (69), 19.3 for 12288 gated channels of
+// 16 (21.3).  Smaller ones may be in the last-level cache (256 MB) when the next
+// call comes, and are not when they were read so: 16 tokens over 16384 x 4096, four
+// weights in turn, 18.4 us (16.2).
+constexpr int64_t kOnceBytes = 80 << 20;
+template <bool ONCE>
+__device__ __forceinline__ void load_to_lds(const void *from, int8_t *to) {
+  __builtin_amdgcn_global_load_lds((GlobalPtr)from, (LdsPtr)to, 16, 0, ONCE ? 2 : 0);
+}
 // 16 zero bytes: what is loaded behind a row's end.
 __device__ const int4 zeros = {0, 0, 0, 0};
 
@@ -124,7 +135,7 @@ __device__ __forceinline__ void keep_row(const Int8Args &a, int8_t *q, float *sc
   if (t * 16 < wide) reinterpret_cast<i32x4 *>(q)[t] = bytes;
 }
 
-template <int PAIR>
+template <int PAIR, bool ONCE>
 __global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
   constexpr int W = kRowWaves, kSlot = PAIR * 2048, kLoads = 2 * PAIR, D = 4 / PAIR;
   // (arrays of their own: the compiler sees that loads are on their way to others)
@@ -161,7 +172,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
       const int piece = (lane % 8 ^ (i % 2 * 4 + lane / 16)) * 16;
       const void *p = base[i / 2] + k + off[i % 2];
       if (!whole && (k + piece >= a.K || to_tile >= tiles)) p = &zeros;
-      __builtin_amdgcn_global_load_lds((GlobalPtr)p, (LdsPtr)(slot + wave * kSlot + i * 1024), 16, 0, 0);
+      load_to_lds<ONCE>(p, slot + wave * kSlot + i * 1024);
     }
     if (++to_turn == turns) {
       to_turn = 0;
@@ -250,7 +261,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
 // waves' sums are added up at the end.  (Loaded straight to registers, a matrix
 // operand's neighbouring lanes are different rows, and each 16 bytes are a look-up of
 // their own in the cache: 16 tokens of 4096 x 4096 8.8 us, 6.5 so.)
-template <int TM, int PAIR, int WAVES>
+template <int TM, int PAIR, int WAVES, bool ONCE>
 __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
   constexpr int T = PAIR * TM, kRows = PAIR + TM;   // tiles of 16 rows of a step
   constexpr int D = kRows <= 2 ? 4 : 2, kSlot = kRows * 2048, kLoads = 2 * kRows;
@@ -285,7 +296,9 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
       const int piece = (lane % 8 ^ (i % 2 * 4 + lane / 16)) * 16;
       const void *p = base[i / 2] + k + off[i];
       if (k + 128 > a.K && k + piece >= a.K) p = &zeros;
-      __builtin_amdgcn_global_load_lds((GlobalPtr)p, (LdsPtr)(slot + wave * kSlot + i * 1024), 16, 0, 0);
+      int8_t *const to = slot + wave * kSlot + i * 1024;
+      if (i < 2 * PAIR) load_to_lds<ONCE>(p, to);
+      else load_to_lds<false>(p, to);
     }
   };
   i32x4 acc[PAIR][TM] = {};
@@ -404,7 +417,7 @@ __device__ __forceinline__ void interleave() {
   if constexpr (i + 1 < products) interleave<products, reads, loads, i + 1>();
 }
 
-template <int BM, int BN, int PAIR, int D>
+template <int BM, int BN, int PAIR, int D, bool ONCE>
 __global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int8_tile_kernel(Int8Args a) {
   typedef Tile<BM, BN> C;
   constexpr int kEarly = D > 2 ? C::kLoads : C::kLoads - C::kLoads / 4;
@@ -441,7 +454,9 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int
 #pragma unroll
     for (int i = from; i < to; ++i) {
       const int8_t *p = base[i < BM / 32 ? 0 : 1 + (i - BM / 32) % PAIR] + k;
-      __builtin_amdgcn_global_load_lds((GlobalPtr)(p + off[i]), (LdsPtr)(stage + (i * 4 + wave) * 1024), 16, 0, 0);
+      int8_t *const to = stage + (i * 4 + wave) * 1024;
+      if (i < BM / 32) load_to_lds<false>(p + off[i], to);
+      else load_to_lds<ONCE>(p + off[i], to);
     }
   };
   auto load_end = [&](int8_t *stage, int k, int from, int to) {
@@ -449,7 +464,7 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int
     for (int i = from; i < to; ++i) {
       const int8_t *p = base[i < BM / 32 ? 0 : 1 + (i - BM / 32) % PAIR] + k;
       const void *q = k + piece < a.K ? (const void *)(p + off[i]) : (const void *)&zeros;
-      __builtin_amdgcn_global_load_lds((GlobalPtr)q, (LdsPtr)(stage + (i * 4 + wave) * 1024), 16, 0, 0);
+      load_to_lds<false>(q, stage + (i * 4 + wave) * 1024);
     }
   };
   i32x16 acc[C::kMi][C::kNi] = {};
@@ -601,17 +616,22 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int
   }
 }
 
+inline bool read_once(const Int8Args &a) { return (int64_t)a.N * a.K * (a.pair ? 2 : 1) > kOnceBytes; }
+
 template <int PAIR>
 hipError_t row(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
   // as many workgroups as a compute unit's LDS holds (37 KB each), each with the same number of tiles
   const int tiles = (a.N + 15) / 16, most = 4 * kSplitCUs, turns = (tiles + most - 1) / most;
-  return launch_timed(int8_row_kernel<PAIR>, dim3((unsigned)((tiles + turns - 1) / turns)), kRowWaves * 64, stream, ev,
-                      done, a);
+  const dim3 grid((unsigned)((tiles + turns - 1) / turns));
+  return read_once(a) ? launch_timed(int8_row_kernel<PAIR, true>, grid, kRowWaves * 64, stream, ev, done, a)
+                      : launch_timed(int8_row_kernel<PAIR, false>, grid, kRowWaves * 64, stream, ev, done, a);
 }
 template <int TM, int PAIR, int WAVES>
 hipError_t split(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
   const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * TM - 1) / (16 * TM)));
-  return launch_timed(int8_split_kernel<TM, PAIR, WAVES>, grid, WAVES * 64, stream, ev, done, a);
+  if constexpr (TM <= 2)   // (one tile of tokens)
+    if (read_once(a)) return launch_timed(int8_split_kernel<TM, PAIR, WAVES, true>, grid, WAVES * 64, stream, ev, done, a);
+  return launch_timed(int8_split_kernel<TM, PAIR, WAVES, false>, grid, WAVES * 64, stream, ev, done, a);
 }
 template <int BM, int BN, int PAIR>
 int64_t tile_count(const Int8Args &a) {
@@ -619,8 +639,11 @@ int64_t tile_count(const Int8Args &a) {
 }
 template <int BM, int BN, int PAIR, int D>
 hipError_t tiles(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
-  return launch_timed(int8_tile_kernel<BM, BN, PAIR, D>, dim3((unsigned)tile_count<BM, BN, PAIR>(a)), 256, stream, ev,
-                      done, a);
+  const dim3 grid((unsigned)tile_count<BM, BN, PAIR>(a));
+  if constexpr (BM == 64)
+    if (a.M <= BM && read_once(a))
+      return launch_timed(int8_tile_kernel<BM, BN, PAIR, D, true>, grid, 256, stream, ev, done, a);
+  return launch_timed(int8_tile_kernel<BM, BN, PAIR, D, false>, grid, 256, stream, ev, done, a);
 }
 
 // How long `count` tiles of `stages` 128 k take, `slots` of them at a time: in us, a
