@@ -112,8 +112,7 @@ __device__ __forceinline__ float exp_below(float x) {
 }
 // v / (1 + exp(-z)): the exponential never overflows, so that the result goes to
 // 0 as slowly as it should where z is far below 0.  The divisor lies in [1, 2]: its
-// reciprocal and one correction, a third of a division's instructions.  (4096 tokens'
-// gated pairs, where a lane has 128 results of a tile: see int8_tile_kernel.)
+// reciprocal and one correction, a third of a division's instructions.
 __device__ __forceinline__ float logistic(float v, float z) {
   const float e = exp_below(fmaxf(-fabsf(z), -256.0f));
   const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d), n = z < 0.0f ? e : 1.0f;
@@ -123,7 +122,7 @@ __device__ __forceinline__ float logistic(float v, float z) {
 
 // (the choice outside of the loops: n independent chains of instructions, not n
 // branches.  4096 tokens' gated pairs, 128 results a lane of each tile: 451 us with
-// the branches.)
+// the branches, 413 so.)
 template <int n>
 __device__ __forceinline__ void activate(int act, float (&v)[n]) {
   auto each = [&](auto f) {

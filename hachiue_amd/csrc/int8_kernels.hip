@@ -84,7 +84,8 @@ __device__ __forceinline__ void meet() {
 // barrier and on into the next tile, so that nothing runs dry at a tile's end.  A
 // float row is quantised by each workgroup while its first weights are on their
 // way, which saves a launch.  The product is the matrix cores' with the token in
-// all 16 columns: they have 30 times the rate that the weights come at.
+// all 16 columns: they have 30 times the rate that the weights come at.  151936 x 2048:
+// 48.9 us, 6.4 TB/s (plain reads of as many bytes: 6.1).
 constexpr int kRowWaves = 4;
 
 // The row into LDS, zeros behind K (a multiple of 128 bytes), and its scale.  A thread
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
   __shared__ __align__(1024) int8_t r0[W * kSlot], r1[W * kSlot];
   __shared__ __align__(1024) int8_t r2[D == 4 ? W * kSlot : 16], r3[D == 4 ? W * kSlot : 16];
   __shared__ __align__(16) int8_t q[kInt8RowK];
-  __shared__ int part[2][W][PAIR][16];
+  __shared__ __align__(16) int part[2][W][PAIR][16];
   __shared__ float scale;
   __shared__ uint32_t most[W];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
 // steps of 128 k on their way at a time (two of more rows), without a barrier; the
 // waves' sums are added up at the end.  (Loaded straight to registers, a matrix
 // operand's neighbouring lanes are different rows, and each 16 bytes are a look-up of
-// their own in the cache: 16 tokens of 4096 x 4096 8.8 us, 6.5 so.)
+// their own in the cache: 16 tokens of 4096 x 4096 8.8 us, 6.4 so, 33 MB read in all.)
 template <int TM, int PAIR, int WAVES, bool ONCE>
 __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
   constexpr int T = PAIR * TM, kRows = PAIR + TM;   // tiles of 16 rows of a step
@@ -380,9 +381,18 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
   }
 }
 
-// ---- many tokens: tiles through LDS.
-// A workgroup of 2 x 2 waves has a tile of BM tokens and BN channels (PAIR 2: BN / 2
-// of each weight), a wave a quarter of it.  A stage is 128 k of all of its rows.
+// ---- many tokens: tiles through LDS, bound by the matrix cores and the power that
+// they draw.  A workgroup of 2 x 2 waves has a tile of BM tokens and BN channels (PAIR
+// 2: BN / 2 of each weight), a wave a quarter of it.  A stage is 128 k of all of its
+// rows.  256 x 256 reads each byte from L2 for 256 results and from LDS for 128, which
+// leaves either path half idle beside the products (128 x 128 takes all that a unit
+// gets from L2); its sums are all 256 accumulation registers of a lane, so that a
+// unit has one workgroup, and nothing runs beside a tile's epilogue.  8192 x 8192 x
+// 8192: 450 us, 2450 TOPS, the matrix cores busy for 62 % of the clocks, which fall to
+// 1.8 GHz; 4096 tokens of 4096 by 12288 gated channels 410 us, of which the epilogues
+// take 70.  (8 waves with 128 x 64 each: the compiler moves sums to memory.  128 x
+// 256 tiles of 64 k, two workgroups a unit: 6 to 10 % faster for K <= 2048, 10 to 25 %
+// slower above.)
 template <int BM, int BN>
 struct Tile {
   static constexpr int kThreads = 256;
@@ -647,11 +657,11 @@ hipError_t tiles(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent
 }
 
 // How long `count` tiles of `stages` 128 k take, `slots` of them at a time: in us, a
-// stage's and an epilogue's share, and of a round that is not full its idle part
-// costs the less, the more of it there is (fewer units run faster).  Measured over
-// 300 to 4096 tokens by 2048 to 20000 channels and K of 1024 to 8192, 36 cases: the
-// faster of 128 x 128 and 256 x 256 was chosen in 33, and the others' loss was
-// below 8 %.
+// stage's and an epilogue's share; a round that is not full costs from `idle` of a full
+// one's time on (fewer units run faster).  Fitted to 300 to 4096 tokens by 2048 to
+// 20000 channels and K of 1024 to 8192, 66 cases with and without a second weight,
+// where either of 128 x 128 and 256 x 256 is the faster by up to 70 %: the faster one
+// is chosen in 60, and the others lose 8 % at most.
 inline double rounds_time(int64_t count, int slots, double idle, double stage, double rest, int64_t stages) {
   const int64_t full = count / slots, left = count % slots;
   const double rounds = (double)full + (left ? idle + (1.0 - idle) * (double)left / slots : 0.0);
@@ -659,11 +669,12 @@ inline double rounds_time(int64_t count, int slots, double idle, double stage, d
 }
 
 // Which kernel.  us at K = 4096 unless said (2048 for 151936 channels and 40000):
-//   one token: 52 over 151936 channels, 7.3 over 4096 (the split kernel 84, 6.5)
+//   one token: 49 over 151936 channels, 7.1 over 4096 with a float row (the split kernel
+//   84, and 6.5 behind the quantising of the row, 3.5)
 //   K split among 8 waves up to 256 strips of 16 channels, among 4 above: 16 tokens
 //   over 4096 6.7 and 7.5, over 8192 11.7 and 10.3 (tiles of four stages 12.6, 12.6)
-//   tiles of 64 x 128: 16 tokens over 16384 16 (split 19), over 151936 57 (95); 64
-//   over 4096 13 (split 10), over 16384 19 (27); of two stages, three workgroups a
+//   tiles of 64 x 128: 16 tokens over 16384 16 (split 19), over 151936 56 (95); 64
+//   over 4096 13 (split 9.4), over 16384 18 (27); of two stages, three workgroups a
 //   unit, above a workgroup a unit: 64 over 40000 23 (four stages 27), over 4096 20 (13)
 //   tiles of 128 x 128 of four stages: 1024 over 4096 22 (two stages 26, 64 x 128 25)
 template <int PAIR>
@@ -679,8 +690,8 @@ hipError_t int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_
   if (a.M <= 64) return tiles<64, 128, PAIR, 2>(a, stream, ev, done);
   const int64_t mid = tile_count<128, 128, PAIR>(a), large = tile_count<256, 256, PAIR>(a), stages = (a.K + 127) / 128;
   if (mid <= kSplitCUs) return tiles<128, 128, PAIR, 4>(a, stream, ev, done);
-  const double mid_us = rounds_time(mid, 2 * kSplitCUs, 0.5, 1.12, PAIR == 2 ? 5.5 : 4.2, stages);
-  const double large_us = rounds_time(large, kSplitCUs, 0.6, 1.7, PAIR == 2 ? 20.0 : 11.5, stages);
+  const double mid_us = rounds_time(mid, 2 * kSplitCUs, 0.5, 1.12, PAIR == 2 ? 2.5 : 4.2, stages);
+  const double large_us = rounds_time(large, kSplitCUs, 0.6, 1.7, PAIR == 2 ? 12.0 : 11.5, stages);
   return mid_us < large_us ? tiles<128, 128, PAIR, 2>(a, stream, ev, done)
                            : tiles<256, 256, PAIR, 2>(a, stream, ev, done);
 }

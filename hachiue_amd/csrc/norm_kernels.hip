@@ -8,7 +8,9 @@
 // element.  A row is held in the registers of its threads (64 to 1024 of them, 8
 // elements of a tensor in one load, wherever rows start), so
 // that the norms' sums, up to five one after the other, read nothing again.  All
-// sums are binary32: each thread's own elements, then a tree.
+// sums are binary32: each thread's own elements, then a tree.  8192 rows of 4096, x
+// and out bfloat16, residual and s binary32: 78 us, 5.2 TB/s (a copy of 1 GB: 5.05);
+// 4096 rows of 12288 bfloat16 in 8 bits: 35 us, 4.3 TB/s.
 #include "block_ops.h"
 
 #include <hip/hip_ext.h>

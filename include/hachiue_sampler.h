@@ -550,7 +550,7 @@ int hs_block_norm_device(hs_context *ctx, const hs_block_norm *norm, void *strea
  * workspace as in hs_verify_drafts_device; x in I8 and y in floats need none.
  *
  * hs_gemv_device_ex, hs_lm_head_sample_device_ex, hs_gemv_lora_device and
- * hs_lm_head_lora_sample_device take such weights too (K then up to 65536), with
+ * hs_lm_head_lora_sample_device take such weights too (K then up to 32768), with
  * binary32 x and y. */
 int hs_matmul_int_device(hs_context *ctx, int32_t M, const hs_rows *x, const hs_weights *w,
                         const float *bias, const hs_rows *y, void *stream);
