@@ -330,6 +330,20 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
     products(slot, s);
     load(slot, s + D * WAVES);
   };
+  // What the end needs is asked for first: wave j finishes tile j, a lane one token's
+  // four channels.
+  static_assert(TM <= WAVES, "a wave a tile");
+  const int m = m0 + wave * 16 + lane % 16, n = n0 + lane / 16 * 4;
+  float xs = 0.0f, ws[PAIR][4] = {}, bias[4] = {};
+  if (wave < TM) {
+    xs = a.xs[min(m, a.M - 1)];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int p = 0; p < PAIR; ++p) ws[p][r] = a.ws[p][min(n + r, a.N - 1)];
+      if (PAIR == 1 && a.bias) bias[r] = a.bias[min(n + r, a.N - 1)];
+    }
+  }
   load(r0, wave);
   load(r1, wave + WAVES);
   if constexpr (D == 4) {
@@ -352,33 +366,28 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
 #pragma unroll
     for (int i = 0; i < TM; ++i) part[wave * (kSlot / 16) + (p * TM + i) * 64 + lane] = acc[p][i];
   __syncthreads();
-  for (int tile = wave; tile < TM; tile += WAVES) {
-    i32x4 s[PAIR];
+  if (wave >= TM || m >= a.M) return;
+  i32x4 sum[PAIR];
 #pragma unroll
-    for (int p = 0; p < PAIR; ++p) {
-      s[p] = part[(p * TM + tile) * 64 + lane];
+  for (int p = 0; p < PAIR; ++p) {
+    sum[p] = part[(p * TM + wave) * 64 + lane];
 #pragma unroll
-      for (int v = 1; v < WAVES; ++v) s[p] += part[v * (kSlot / 16) + (p * TM + tile) * 64 + lane];
-    }
-    // a lane has one token's four channels
-    const int m = m0 + tile * 16 + lane % 16, n = n0 + lane / 16 * 4;
-    if (m >= a.M) continue;
-    const float xs = a.xs[m];
-    float v[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = scaled(s[0][r], xs, a.ws[0][min(n + r, a.N - 1)]);
-    if constexpr (PAIR == 2) {
-      activate<4>(a.act, v);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] *= scaled(s[PAIR - 1][r], xs, a.ws[PAIR - 1][min(n + r, a.N - 1)]);
-    } else if (a.bias) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] += a.bias[min(n + r, a.N - 1)];
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (n + r < a.N) put(a.y, m, n + r, v[r]);
+    for (int v = 1; v < WAVES; ++v) sum[p] += part[v * (kSlot / 16) + (p * TM + wave) * 64 + lane];
   }
+  float v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = scaled(sum[0][r], xs, ws[0][r]);
+  if constexpr (PAIR == 2) {
+    activate<4>(a.act, v);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] *= scaled(sum[PAIR - 1][r], xs, ws[PAIR - 1][r]);
+  } else if (a.bias) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] += bias[r];
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (n + r < a.N) put(a.y, m, n + r, v[r]);
 }
 
 // ---- many tokens: tiles through LDS, bound by the matrix cores and the power that
@@ -477,6 +486,24 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int
       load_to_lds<false>(q, stage + (i * 4 + wave) * 1024);
     }
   };
+  // What the end needs is asked for first, where there are registers to hold it (24
+  // more in 256 x 256 have the compiler move others to memory: 134 us for 4096 tokens
+  // over 20000 x 1024, 142 so).
+  constexpr bool kAskFirst = BM * BN <= 128 * 128;
+  __shared__ float xs_of[BM];
+  constexpr int kCols = BN / 2 / PAIR, kLanes = kCols / 8, kRows = 64 / kLanes;
+  float w0[8], w1[8], bias[8];
+  auto ask = [&] {
+    for (int r = tid; r < BM; r += 256) xs_of[r] = a.xs[min(m0 + r, a.M - 1)];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int ne = min(n0 + wn * kCols + lane % kLanes * 8 + e, a.N - 1);
+      w0[e] = a.ws[0][ne];
+      w1[e] = PAIR == 2 ? a.ws[PAIR - 1][ne] : 0.0f;
+      bias[e] = PAIR == 1 && a.bias ? a.bias[ne] : 0.0f;
+    }
+  };
+  if constexpr (kAskFirst) ask();
   i32x16 acc[C::kMi][C::kNi] = {};
   const int ar = (wm * (BM / 2) + lane % 32) * 128, br = (BM + wn * (BN / 2) + lane % 32) * 128;
   struct Pieces {
@@ -578,21 +605,13 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int
   asm volatile("" ::: "memory");
   // The sums go through LDS, 32 tokens of a wave at a time, so that a thread has
   // eight channels of a token and stores are whole lines.
-  __shared__ float xs_of[BM];
-  for (int r = tid; r < BM; r += 256) xs_of[r] = a.xs[min(m0 + r, a.M - 1)];
-  __syncthreads();
-  int *const out = reinterpret_cast<int *>(wm ? s1 : s0) + wn * 32 * C::kOutLd;
-  constexpr int kCols = BN / 2 / PAIR, kLanes = kCols / 8, kRows = 64 / kLanes;
-  const int c = lane % kLanes * 8, n = n0 + wn * kCols + c;
-  const int at = PAIR == 2 ? c / 32 * 64 + c % 32 : c;
-  float w0[8], w1[8], bias[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int ne = min(n + e, a.N - 1);
-    w0[e] = a.ws[0][ne];
-    w1[e] = PAIR == 2 ? a.ws[PAIR - 1][ne] : 0.0f;
-    bias[e] = PAIR == 1 && a.bias ? a.bias[ne] : 0.0f;
+  if constexpr (!kAskFirst) {
+    ask();
+    __syncthreads();
   }
+  const int c = lane % kLanes * 8, n = n0 + wn * kCols + c;
+  int *const out = reinterpret_cast<int *>(wm ? s1 : s0) + wn * 32 * C::kOutLd;
+  const int at = PAIR == 2 ? c / 32 * 64 + c % 32 : c;
 #pragma unroll
   for (int i = 0; i < C::kMi; ++i) {
 #pragma unroll
