@@ -255,6 +255,65 @@ __global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
   }
 }
 
+// Rows that stay in LDS: 128 bytes of them in pieces of 16, piece ^ (row / 2 % 8), the
+// rows an odd multiple of 128 bytes apart, so that sixteen rows' same pieces fill
+// the 64 banks once.
+constexpr int kKeptBytes = kInt8KeptElems + kInt8KeptRows * 256;   // (a row's width: K + 255 at most)
+__device__ __forceinline__ int kept_width(int K) { return ((K + 127) / 128 | 1) * 128; }
+__device__ __forceinline__ int kept_piece(int row, int piece, int wide) {
+  return row * wide + (piece / 8 * 8 + (piece % 8 ^ row / 2 % 8)) * 16;
+}
+
+// All float rows, quantised into `q` by a workgroup, zeros behind K, and their scales:
+// a thread has 16 elements (K is a multiple of 16), the rows' largest magnitudes meet
+// in LDS.  `next` is called when the rows are asked for and not yet waited for.
+constexpr int kKeepThreads = kInt8KeptElems / 16;
+template <typename F>
+__device__ __forceinline__ void keep_rows(const Int8Args &a, int8_t *q, float *scales, uint32_t *most, F next) {
+  const int t = threadIdx.x, per = a.K / 16, wide = kept_width(a.K);
+  const int row = t / per, piece = t % per;
+  const bool has = row < a.M;
+  typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
+  Any raw[4] = {};
+  if (has) {
+    const int64_t at = (int64_t)row * a.rows.ld + piece * 16;
+    if (a.rows.type == kT_F32) {
+      const Any *p = reinterpret_cast<const Any *>(static_cast<const float *>(a.rows.p) + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw[e] = p[e];
+    } else {
+      const Any *p = reinterpret_cast<const Any *>(static_cast<const uint16_t *>(a.rows.p) + at);
+      raw[0] = p[0];
+      raw[1] = p[1];
+    }
+  }
+  next();
+  if (t < a.M) most[t] = 0;
+  for (int i = t; i < a.M * 16; i += kKeepThreads)   // at most 15 pieces behind K
+    if (const int z = per + i % 16; z * 16 < wide)
+      *reinterpret_cast<i32x4 *>(q + kept_piece(i / 16, z, wide)) = i32x4{};
+  meet();
+  float v[16];
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    v[e] = a.rows.type == kT_F32 ? __uint_as_float(raw[e / 4][e % 4])
+                                 : widen16(a.rows.type, (uint16_t)(raw[e / 8][e / 2 % 4] >> (16 * (e % 2))));
+    top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+  }
+  if (has) atomicMax(most + row, top);
+  meet();
+  if (has) {
+    float inv;
+    uint32_t u[4] = {};
+    const float scale = scale_of(most[row], &inv);
+    if (inv > 0.0f) quantised_bytes<16>(v, inv, scale, u);
+    *reinterpret_cast<i32x4 *>(q + kept_piece(row, piece, wide)) = i32x4{(int)u[0], (int)u[1], (int)u[2], (int)u[3]};
+    if (piece == 0) scales[row] = scale;
+  }
+  meet();
+}
+
 // ---- few results: K is split among a workgroup's waves, so that as many compute
 // units as there are tiles of 16 channels (of each weight) and TM tiles of 16 tokens
 // read at once.  A wave's weights and tokens pass through its own part of LDS, four
@@ -262,14 +321,20 @@ __global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
 // waves' sums are added up at the end.  (Loaded straight to registers, a matrix
 // operand's neighbouring lanes are different rows, and each 16 bytes are a look-up of
 // their own in the cache: 16 tokens of 4096 x 4096 8.8 us, 6.4 so, 33 MB read in all.)
-template <int TM, int PAIR, int WAVES, bool ONCE>
+// KEPT: float rows are quantised by each workgroup while its first weights are on
+// their way, and stay in LDS.
+template <int TM, int PAIR, int WAVES, bool ONCE, bool KEPT>
 __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
-  constexpr int T = PAIR * TM, kRows = PAIR + TM;   // tiles of 16 rows of a step
+  constexpr int T = PAIR * TM, kRows = PAIR + (KEPT ? 0 : TM);   // tiles of 16 rows of a step
   constexpr int D = kRows <= 2 ? 4 : 2, kSlot = kRows * 2048, kLoads = 2 * kRows;
   // (arrays of their own: the compiler sees that loads are on their way to others)
   __shared__ __align__(1024) int8_t r0[WAVES * kSlot], r1[WAVES * kSlot];
   __shared__ __align__(1024) int8_t r2[D == 4 ? WAVES * kSlot : 16], r3[D == 4 ? WAVES * kSlot : 16];
   static_assert(T * 1024 <= kSlot, "a wave's sums fit its first slot");
+  static_assert(!KEPT || (TM * 16 == kInt8KeptRows && WAVES * 64 == kKeepThreads), "one tile of tokens");
+  __shared__ __align__(1024) int8_t kept[KEPT ? kKeptBytes : 16];
+  __shared__ float kept_scales[KEPT ? kInt8KeptRows : 1];
+  __shared__ uint32_t most[KEPT ? kInt8KeptRows : 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * TM;
   const int steps = (a.K + 127) / 128;
@@ -312,7 +377,12 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
 #pragma unroll
       for (int i = 0; i < PAIR; ++i) w[kk][i] = *reinterpret_cast<const i32x4 *>(at + i * 2048 + p);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) x[kk][i] = *reinterpret_cast<const i32x4 *>(at + (PAIR + i) * 2048 + p);
+      for (int i = 0; i < TM; ++i) {
+        if constexpr (KEPT)   // (rows behind the last: its own again, not stored)
+          x[kk][i] = *reinterpret_cast<const i32x4 *>(
+              kept + kept_piece(min(lane % 16, a.M - 1), s * 8 + kk * 4 + lane / 16, kept_width(a.K)));
+        else x[kk][i] = *reinterpret_cast<const i32x4 *>(at + (PAIR + i) * 2048 + p);
+      }
     }
     // what is read is in registers: its place may be loaded anew
     wait_loads<(D - 1) * kLoads>();
@@ -336,7 +406,7 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
   const int m = m0 + wave * 16 + lane % 16, n = n0 + lane / 16 * 4;
   float xs = 0.0f, ws[PAIR][4] = {}, bias[4] = {};
   if (wave < TM) {
-    xs = a.xs[min(m, a.M - 1)];
+    if constexpr (!KEPT) xs = a.xs[min(m, a.M - 1)];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
 #pragma unroll
@@ -344,12 +414,16 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
       if (PAIR == 1 && a.bias) bias[r] = a.bias[min(n + r, a.N - 1)];
     }
   }
-  load(r0, wave);
-  load(r1, wave + WAVES);
-  if constexpr (D == 4) {
-    load(r2, wave + 2 * WAVES);
-    load(r3, wave + 3 * WAVES);
-  }
+  auto first = [&] {
+    load(r0, wave);
+    load(r1, wave + WAVES);
+    if constexpr (D == 4) {
+      load(r2, wave + 2 * WAVES);
+      load(r3, wave + 3 * WAVES);
+    }
+  };
+  if constexpr (KEPT) keep_rows(a, kept, kept_scales, most, first);
+  else first();
   for (int s = wave; s < steps; s += D * WAVES) {
     turn(r0, s);
     if (s + WAVES < steps) turn(r1, s + WAVES);
@@ -367,6 +441,7 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
     for (int i = 0; i < TM; ++i) part[wave * (kSlot / 16) + (p * TM + i) * 64 + lane] = acc[p][i];
   __syncthreads();
   if (wave >= TM || m >= a.M) return;
+  if constexpr (KEPT) xs = kept_scales[m];
   i32x4 sum[PAIR];
 #pragma unroll
   for (int p = 0; p < PAIR; ++p) {
@@ -659,8 +734,9 @@ template <int TM, int PAIR, int WAVES>
 hipError_t split(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
   const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * TM - 1) / (16 * TM)));
   if constexpr (TM <= 2)   // (one tile of tokens)
-    if (read_once(a)) return launch_timed(int8_split_kernel<TM, PAIR, WAVES, true>, grid, WAVES * 64, stream, ev, done, a);
-  return launch_timed(int8_split_kernel<TM, PAIR, WAVES, false>, grid, WAVES * 64, stream, ev, done, a);
+    if (read_once(a))
+      return launch_timed(int8_split_kernel<TM, PAIR, WAVES, true, false>, grid, WAVES * 64, stream, ev, done, a);
+  return launch_timed(int8_split_kernel<TM, PAIR, WAVES, false, false>, grid, WAVES * 64, stream, ev, done, a);
 }
 template <int BM, int BN, int PAIR>
 int64_t tile_count(const Int8Args &a) {
@@ -699,6 +775,9 @@ inline double rounds_time(int64_t count, int slots, double idle, double stage, d
 template <int PAIR>
 hipError_t int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
   if (int8_row(a.M, a.K)) return row<PAIR>(a, stream, ev, done);
+  if (a.rows.p)   // (int8_kept)
+    return launch_timed(int8_split_kernel<1, PAIR, 8, false, true>, dim3((a.N + 15) / 16), kKeepThreads, stream, ev,
+                        done, a);
   const int64_t strips = (a.N + 15) / 16, groups = (a.M + 63) / 64;
   if (a.M <= 16 && strips <= 768)
     return strips <= 256 ? split<1, PAIR, 8>(a, stream, ev, done) : split<1, PAIR, 4>(a, stream, ev, done);

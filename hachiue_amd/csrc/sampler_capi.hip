@@ -1809,7 +1809,7 @@ int int8_args(int32_t M, const hs_rows *x, const hs_weights *w0, const hs_weight
   c.g.K = K;
   c.g.pair = w1 != nullptr;
   c.g.act = act;
-  if (xr.type != hs::kT_I8 && hs::int8_row(M, K)) {
+  if (xr.type != hs::kT_I8 && hs::int8_quantises(M, N, K)) {
     c.g.rows = xr;
   } else if (xr.type != hs::kT_I8) {
     c.pre.M = M;

@@ -60,6 +60,34 @@ def test_float_rows_are_quantised_first(sampler, x, out, M):
     same(project(sampler, X, w, M, N, out), bo.product(q, s, w.w, w.s), out)
 
 
+# Rows that the product's workgroups quantise themselves (16 rows, 8192 elements, 4096
+# channels at most) and their neighbours beyond each limit; tails of 16 elements.
+FEW = [(1, 70, 4112), (1, 4096, 8192), (1, 70, 8208), (2, 4096, 4096), (2, 33, 4112), (3, 4097, 1040), (4, 300, 2048),
+       (5, 777, 1040), (7, 800, 1104), (8, 16, 1024), (13, 50, 624), (15, 4096, 528), (16, 33, 16), (16, 100, 512),
+       (16, 100, 528), (17, 40, 48)]
+
+
+@pytest.mark.parametrize("x", FLOATS)
+@pytest.mark.parametrize("M,N,K", FEW)
+def test_few_float_rows(sampler, M, N, K, x):
+    """Rows anywhere, of zeros, with an infinity and a NaN among them."""
+    rng = np.random.default_rng(M * K + N)
+    w, up = Weight(rng, N, K), Weight(rng, N, K)
+    v = rng.standard_normal((M, K)) * rng.uniform(0.1, 30, (M, 1))
+    if M > 3:
+        v[1], v[2, K - 1], v[M - 1, 0] = 0.0, np.inf, np.nan
+    X, v = Rows.of(v, x, 3, 1)
+    q, s = bo.quantise(v.astype(np.float32))
+    bias = rng.standard_normal(N).astype(np.float32)
+    same(project(sampler, X, w, M, N), bo.product(q, s, w.w, w.s), "f32")
+    same(project(sampler, X, w, M, N, "f16", bias, 3), bo.product(q, s, w.w, w.s, bias), "f16")
+    own, (q8, s8) = project(sampler, X, w, M, N, "i8"), bo.quantise(bo.product(q, s, w.w, w.s))
+    assert np.array_equal(own[0], q8) and np.array_equal(own[1], s8, equal_nan=True)
+    # a pair: the bits that the rows give when they come quantised
+    pair = [gated(sampler, rows, w, up, "gelu", M, N) for rows in (X, quantised(q, s))]
+    same(pair[0], pair[1], "f32")
+
+
 @pytest.mark.parametrize("M,K", [(1, 65536), (40, 65536), (130, 32768), (600, 16384)])
 def test_the_largest_sums(sampler, M, K):
     """Every product 2^14 or its negative: sums up to 2^30."""
