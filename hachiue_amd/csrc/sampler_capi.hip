@@ -1882,6 +1882,8 @@ int int8_run(hs_context *ctx, Int8Call &c, hipStream_t stream) {
 
 int int8_gemv(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *w, float *d_y,
               int64_t ldy, hipStream_t stream) {
+  // (as with every type of weights: without rows or channels nothing else is looked at)
+  if (M >= 0 && w->rows >= 0 && w->cols > 0 && (M == 0 || w->rows == 0)) return HS_OK;
   if (M > 65535) return fail(HS_ERR_UNSUPPORTED, "M %d above 65535", M);
   const hs_rows x = {hs::kT_F32, ldx, const_cast<float *>(d_x), nullptr}, y = {hs::kT_F32, ldy, d_y, nullptr};
   Int8Call c;
