@@ -2106,6 +2106,8 @@ int hs_gemv_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, in
   HS_LOCK(ctx);
   if (hs::tern_quant_bytes(w_type) > 0)
     return fail(HS_ERR_INVALID_ARGUMENT, "weight type %d is planar: use hs_gemv_device_ex", w_type);
+  if (w_type == hs::kT_I8 && M > 0 && N > 0 && K > 0)
+    return fail(HS_ERR_UNSUPPORTED, "weight type %d has scales: use hs_gemv_device_ex", w_type);
   const hs_weights w = raw_weights(K, d_w, w_type, N);
   return gemv_device(ctx, d_x, M, ldx, &w, d_y, ldy, static_cast<hipStream_t>(stream));
 }
@@ -2228,6 +2230,8 @@ int hs_lm_head_sample_device(hs_context *ctx, const float *d_x, int32_t M, int64
   if (hs::tern_quant_bytes(w_type) > 0)
     return fail(HS_ERR_INVALID_ARGUMENT, "weight type %d is planar: use hs_lm_head_sample_device_ex",
                 w_type);
+  if (w_type == hs::kT_I8 && M > 0 && N > 0 && K > 0)
+    return fail(HS_ERR_UNSUPPORTED, "weight type %d has scales: use hs_lm_head_sample_device_ex", w_type);
   const hs_weights w = raw_weights(K, d_w, w_type, N);
   return lm_head_sample(ctx, d_x, M, ldx, &w, d_logits, ldl, d_hist_ids, d_hist_offsets, configs,
                         d_uniforms, d_tokens, static_cast<hipStream_t>(stream));

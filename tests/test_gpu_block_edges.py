@@ -1,4 +1,4 @@
-"""Calls on I8 weights that have nothing to compute."""
+"""Calls on I8 weights that have nothing to compute, or no room for their scales."""
 import numpy as np
 import pytest
 
@@ -34,3 +34,21 @@ def test_sizes_that_are_none(sampler, M, N, K):
         with pytest.raises(SamplerError) as e:
             sampler.gemv_device_ex(0, M, 64, hs.weights(wtype, N, K, 0), 0, 64)
         assert e.value.status == 1
+
+
+def test_calls_that_take_blocks_do_not_know_the_type(sampler):
+    """They have no argument for the channels' scales: unsupported, as every type
+    that is not in blocks of its own."""
+    x, y, w = (hip.DeviceArray.from_numpy(np.zeros(64 * 64, np.float32)) for _ in range(3))
+    tok, u = hip.DeviceArray.from_numpy(np.full(2, -7, np.int32)), hip.DeviceArray.from_numpy(np.zeros(2))
+    for wtype in (7, 24):
+        with pytest.raises(SamplerError) as e:
+            sampler.gemv_device(x.addr, 2, 64, 64, w.addr, wtype, 5, y.addr, 64)
+        assert e.value.status == 4 and str(wtype) in str(e.value)
+        with pytest.raises(SamplerError) as e:
+            sampler.lm_head_sample_device(x.addr, 2, 64, 64, w.addr, wtype, 5, y.addr, 64, None, None,
+                                          dict(temperature=0.0), u.addr, tok.addr)
+        assert e.value.status == 4 and str(wtype) in str(e.value)
+        sampler.gemv_device(0, 0, 64, 64, 0, wtype, 5, 0, 64)
+    hip.synchronize()
+    assert (tok.download() == -7).all() and (y.download() == 0).all()
