@@ -562,25 +562,67 @@ hs::Workspace split_workspace(const hs_context *ctx) {
   return ws;
 }
 
-// With timing on, takes start/end events for every kernel the call launches.
-int begin_timed(hs_context *ctx, const hs::LaunchArgs &a, hipEvent_t **ev) {
-  *ev = nullptr;
-  if (!ctx->timing) return HS_OK;
-  hs_context::TimedCall tc{};
-  tc.mask = hs::launched_kernels(a);
+// The events of a timed call are free again.
+void free_events(hs_context *ctx, const hs_context::TimedCall &tc) {
   for (int i = 0; i < 2 * hs::kTimedKernels; ++i) {
     if (!(tc.mask >> (i / 2) & 1u)) continue;
-    if (ctx->ev_free.empty()) {
+    try {
+      ctx->ev_free.push_back(tc.ev[i]);
+    } catch (const std::bad_alloc &) {
+      (void)hipEventDestroy(tc.ev[i]);
+    }
+  }
+}
+
+// With timing on, start/end events of the slots of `mask` (one timed call): slot
+// k's are *ev + 2 k.  *ev is null otherwise, and where the events cannot be had,
+// which takes none.
+int timed_slots(hs_context *ctx, unsigned mask, hipEvent_t **ev) {
+  *ev = nullptr;
+  if (!ctx->timing) return HS_OK;
+  const size_t need = 2 * (size_t)__builtin_popcount(mask);
+  try {
+    ctx->ev_free.reserve(need);
+    while (ctx->ev_free.size() < need) {
       hipEvent_t x;
       HS_HIP(hipEventCreate(&x));
       ctx->ev_free.push_back(x);
     }
+    ctx->timed.push_back(hs_context::TimedCall{});
+  } catch (const std::bad_alloc &) {
+    return fail(HS_ERR_OUT_OF_MEMORY, "host allocation failed");
+  }
+  hs_context::TimedCall &tc = ctx->timed.back();
+  tc.mask = mask;
+  for (int i = 0; i < 2 * hs::kTimedKernels; ++i) {
+    if (!(mask >> (i / 2) & 1u)) continue;
     tc.ev[i] = ctx->ev_free.back();
     ctx->ev_free.pop_back();
   }
-  ctx->timed.push_back(tc);
-  *ev = ctx->timed.back().ev;
+  *ev = tc.ev;
   return HS_OK;
+}
+
+// The call that took events last has failed (ev null: it took none): some of
+// them may not have been recorded, and it counts as none.
+void drop_timed(hs_context *ctx, const hipEvent_t *ev) {
+  if (!ev) return;
+  free_events(ctx, ctx->timed.back());
+  ctx->timed.pop_back();
+}
+
+// The end of a call whose launches were made (with events: done_ev is not
+// attached to the last of them), and of one whose launches failed, if it is not
+// captured.
+int leave_timed(hs_context *ctx, hipStream_t s, const hipEvent_t *ev) {
+  const int rc = leave_stream(ctx, s, ev == nullptr);
+  if (rc) drop_timed(ctx, ev);
+  return rc;
+}
+int launch_failed(hs_context *ctx, hipStream_t s, bool cap, const hipEvent_t *ev, hipError_t e) {
+  drop_timed(ctx, ev);
+  if (!cap) (void)leave_stream(ctx, s, false);
+  return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
 }
 
 // A failed launch may have left counters of earlier kernels of the call
@@ -747,15 +789,14 @@ int sample_device(hs_context *ctx, float *d_logits, int32_t rows, int64_t row_st
   a.cutoff_out = d_cutoff;
   a.row_flags = d_row_flags;
   hipEvent_t *ev = nullptr;
-  rc = begin_timed(ctx, a, &ev);
+  rc = timed_slots(ctx, hs::launched_kernels(a), &ev);
   if (rc) return rc;
   hipError_t e = hs::launch_sample(a, ws, stream, ev, ctx->done_ev);
   if (e != hipSuccess) {
     reset_counters(ctx, stream);
-    (void)leave_stream(ctx, stream, false);
-    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
+    return launch_failed(ctx, stream, false, ev, e);
   }
-  return leave_stream(ctx, stream, ev == nullptr);
+  return leave_timed(ctx, stream, ev);
 }
 
 // src/kernels.ts:1613-1654 (the argmax pipeline of the engine's greedy route).
@@ -795,15 +836,14 @@ int argmax_device(hs_context *ctx, const float *d_logits, int32_t rows, int64_t 
   a.rows_direct = 1;
   a.tokens = d_tokens;
   hipEvent_t *ev = nullptr;
-  rc = begin_timed(ctx, a, &ev);
+  rc = timed_slots(ctx, hs::launched_kernels(a), &ev);
   if (rc) return rc;
   hipError_t e = hs::launch_sample(a, ws, stream, ev, ctx->done_ev);
   if (e != hipSuccess) {
     reset_counters(ctx, stream);
-    (void)leave_stream(ctx, stream, false);
-    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
+    return launch_failed(ctx, stream, false, ev, e);
   }
-  return leave_stream(ctx, stream, ev == nullptr);
+  return leave_timed(ctx, stream, ev);
 }
 
 // The checks of an lm_head GEMV call, apart from what its workspace needs: *bw
@@ -930,69 +970,20 @@ int gemv_setup(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const 
   return HS_OK;
 }
 
-// Start/end events of the slots of `mask` (one timed call), when timing is on:
-// slot k's are *ev + 2 k, and *ev is null otherwise.
-int timed_slots(hs_context *ctx, unsigned mask, hipEvent_t **ev) {
-  *ev = nullptr;
-  if (!ctx->timing) return HS_OK;
-  hs_context::TimedCall tc{};
-  tc.mask = mask;
-  for (int i = 0; i < 2 * hs::kTimedKernels; ++i) {
-    if (!(mask >> (i / 2) & 1u)) continue;
-    if (ctx->ev_free.empty()) {
-      hipEvent_t x;
-      HS_HIP(hipEventCreate(&x));
-      ctx->ev_free.push_back(x);
-    }
-    tc.ev[i] = ctx->ev_free.back();
-    ctx->ev_free.pop_back();
-  }
-  ctx->timed.push_back(tc);
-  *ev = ctx->timed.back().ev;
-  return HS_OK;
-}
-
-// Start/end events of timing slot `slot` for the call's one kernel, when
-// timing is on (null otherwise).
+// The same of a call's one kernel: *ev are its events.
 int timed_slot(hs_context *ctx, int slot, hipEvent_t **ev) {
-  *ev = nullptr;
-  if (!ctx->timing) return HS_OK;
-  hs_context::TimedCall tc{};
-  tc.mask = 1u << slot;
-  for (int i = 0; i < 2; ++i) {
-    if (ctx->ev_free.empty()) {
-      hipEvent_t x;
-      HS_HIP(hipEventCreate(&x));
-      ctx->ev_free.push_back(x);
-    }
-    tc.ev[2 * slot + i] = ctx->ev_free.back();
-    ctx->ev_free.pop_back();
-  }
-  ctx->timed.push_back(tc);
-  *ev = ctx->timed.back().ev + 2 * slot;
-  return HS_OK;
+  const int rc = timed_slots(ctx, 1u << slot, ev);
+  if (*ev) *ev += 2 * slot;
+  return rc;
 }
 
-// The same for a call's two kernels (one timed call).
+// And of its two kernels.
 int timed_pair(hs_context *ctx, int first, int second, hipEvent_t **ev1, hipEvent_t **ev2) {
-  *ev1 = *ev2 = nullptr;
-  if (!ctx->timing) return HS_OK;
-  hs_context::TimedCall tc{};
-  tc.mask = 1u << first | 1u << second;
-  for (int slot : {first, second})
-    for (int i = 0; i < 2; ++i) {
-      if (ctx->ev_free.empty()) {
-        hipEvent_t x;
-        HS_HIP(hipEventCreate(&x));
-        ctx->ev_free.push_back(x);
-      }
-      tc.ev[2 * slot + i] = ctx->ev_free.back();
-      ctx->ev_free.pop_back();
-    }
-  ctx->timed.push_back(tc);
-  *ev1 = ctx->timed.back().ev + 2 * first;
-  *ev2 = ctx->timed.back().ev + 2 * second;
-  return HS_OK;
+  hipEvent_t *ev;
+  const int rc = timed_slots(ctx, 1u << first | 1u << second, &ev);
+  *ev1 = ev ? ev + 2 * first : nullptr;
+  *ev2 = ev ? ev + 2 * second : nullptr;
+  return rc;
 }
 
 // (the 8-bit products' section)
@@ -1018,11 +1009,8 @@ int gemv_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const
     return rc;
   }
   const hipError_t e = hs::launch_gemv(g, stream, ev, cap ? nullptr : ctx->done_ev);
-  if (e != hipSuccess) {
-    if (!cap) (void)leave_stream(ctx, stream, false);
-    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
-  }
-  return cap ? HS_OK : leave_stream(ctx, stream, ev == nullptr);
+  if (e != hipSuccess) return launch_failed(ctx, stream, cap, ev, e);
+  return cap ? HS_OK : leave_timed(ctx, stream, ev);
 }
 
 // Plans and routing lists written into fixed arrays (no allocation): the
@@ -1408,13 +1396,10 @@ int verify_drafts(hs_context *ctx, const hs_distribution *target, const hs_distr
   const hipError_t e = hs::launch_verify(a, stream, ev1, ev2, cap ? nullptr : ctx->done_ev);
   if (e != hipSuccess) {
     // the first launch may have left its counts behind
-    if (!cap) {
-      (void)hs::launch_fill_u32(a.arrived, (int64_t)counts, 0u, stream);
-      (void)leave_stream(ctx, stream, false);
-    }
-    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
+    if (!cap) (void)hs::launch_fill_u32(a.arrived, (int64_t)counts, 0u, stream);
+    return launch_failed(ctx, stream, cap, ev1 ? ev1 : ev2, e);
   }
-  return cap ? HS_OK : leave_stream(ctx, stream, !ev1 && !ev2);
+  return cap ? HS_OK : leave_timed(ctx, stream, ev1 ? ev1 : ev2);
 }
 
 int list_side(const hs_candidates *x, const char *what, hs::ListArgs &a, int side) {
@@ -1457,11 +1442,8 @@ int verify_candidates(hs_context *ctx, const hs_candidates *target, const hs_can
   if (!cap) rc = timed_slot(ctx, hs::kListsTimedSlot, &ev);
   if (rc) return rc;
   const hipError_t e = hs::launch_verify_lists(a, stream, ev, cap ? nullptr : ctx->done_ev);
-  if (e != hipSuccess) {
-    if (!cap) (void)leave_stream(ctx, stream, false);
-    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
-  }
-  return cap ? HS_OK : leave_stream(ctx, stream, ev == nullptr);
+  if (e != hipSuccess) return launch_failed(ctx, stream, cap, ev, e);
+  return cap ? HS_OK : leave_timed(ctx, stream, ev);
 }
 
 // The checks of an adapter call; *skip: nothing to do.
@@ -1543,11 +1525,8 @@ int lora_run(hs_context *ctx, hs::LoraArgs &g, hipStream_t stream) {
   hipError_t e = hipSuccess;
   if (g.count > 0) e = hs::launch_lora_shrink(g, stream, ev1);
   if (e == hipSuccess) e = hs::launch_lora_expand(g, stream, ev2, cap ? nullptr : ctx->done_ev);
-  if (e != hipSuccess) {
-    if (!cap) (void)leave_stream(ctx, stream, false);
-    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
-  }
-  return cap ? HS_OK : leave_stream(ctx, stream, ev2 == nullptr);
+  if (e != hipSuccess) return launch_failed(ctx, stream, cap, ev2, e);
+  return cap ? HS_OK : leave_timed(ctx, stream, ev2);
 }
 
 int lora_device(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_adapters *ad,
@@ -1717,11 +1696,8 @@ int block_norm_run(hs_context *ctx, const hs::BlockNormArgs &g, hipStream_t stre
   if (rc) return rc;
   const hipError_t e = inject_failure() ? hipErrorOutOfMemory
                                         : hs::launch_block_norm(g, stream, ev, cap ? nullptr : ctx->done_ev);
-  if (e != hipSuccess) {
-    if (!cap) (void)leave_stream(ctx, stream, false);
-    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
-  }
-  return cap ? HS_OK : leave_stream(ctx, stream, ev == nullptr);
+  if (e != hipSuccess) return launch_failed(ctx, stream, cap, ev, e);
+  return cap ? HS_OK : leave_timed(ctx, stream, ev);
 }
 
 // A weight of an 8-bit product.
@@ -1873,11 +1849,8 @@ int int8_run(hs_context *ctx, Int8Call &c, hipStream_t stream) {
   if (e == hipSuccess && c.post.M)
     e = inject_failure() ? hipErrorOutOfMemory
                          : hs::launch_block_norm(c.post, stream, of(hs::kRequantTimedSlot), done);
-  if (e != hipSuccess) {
-    if (!cap) (void)leave_stream(ctx, stream, false);
-    return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
-  }
-  return cap ? HS_OK : leave_stream(ctx, stream, ev == nullptr);
+  if (e != hipSuccess) return launch_failed(ctx, stream, cap, ev, e);
+  return cap ? HS_OK : leave_timed(ctx, stream, ev);
 }
 
 int int8_gemv(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, const hs_weights *w, float *d_y,
@@ -1993,9 +1966,7 @@ int hs_context_kernel_times(hs_context *ctx, double *ms, int32_t count, int64_t 
     }
     ++ctx->timed_calls;
   }
-  for (const hs_context::TimedCall &tc : ctx->timed)
-    for (int i = 0; i < 2 * hs::kTimedKernels; ++i)
-      if (tc.mask >> (i / 2) & 1u) ctx->ev_free.push_back(tc.ev[i]);
+  for (const hs_context::TimedCall &tc : ctx->timed) free_events(ctx, tc);
   ctx->timed.clear();
   for (int k = 0; k < count; ++k) ms[k] = k < hs::kTimedKernels ? ctx->kernel_ms[k] : 0.0;
   if (calls) *calls = ctx->timed_calls;
@@ -2205,11 +2176,8 @@ int lm_head_sample(hs_context *ctx, const float *d_x, int32_t M, int64_t ldx, co
       const hipError_t e = greedy ? hs::launch_argmax_fused(g, f, st, ev, ctx->done_ev)
                            : tern ? hs::launch_tern_sample(g, f, st, ev, ctx->done_ev)
                                   : hs::launch_kq_sample(g, f, st, ev, ctx->done_ev);
-      if (e != hipSuccess) {
-        (void)leave_stream(ctx, st, false);
-        return fail(HS_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
-      }
-      return leave_stream(ctx, st, ev == nullptr);
+      if (e != hipSuccess) return launch_failed(ctx, st, false, ev, e);
+      return leave_timed(ctx, st, ev);
     }
     if (g.x != d_x) (void)leave_stream(ctx, st, false);   // the rotation was enqueued
   }
