@@ -276,12 +276,10 @@ struct hs_context {
   };
   std::vector<hipEvent_t> ev_free;
   std::vector<TimedCall> timed;
-  double kernel_ms[hs::kTimedKernels] = {};
   // rows routed to the row kernel only when a call has at least this many
   int row_min_rows = 1;
   // workgroups per row of the row kernel: 0 chooses by batch size
   int row_split = 0;
-  int64_t timed_calls = 0;
   // hs_sample_batch_device_noalloc: pinned staging of plans and lists, the
   // configs of this context's last upload into the device's scratch, and the
   // device's upload count after it (all set up at creation)
@@ -1956,22 +1954,20 @@ int hs_context_kernel_times(hs_context *ctx, double *ms, int32_t count, int64_t 
   HS_LOCK(ctx);
   if (count < 0 || (count > 0 && !ms)) return fail(HS_ERR_INVALID_ARGUMENT, "bad output array");
   DeviceGuard guard(ctx->device);
-  for (const hs_context::TimedCall &tc : ctx->timed) {
+  double total[hs::kTimedKernels] = {};
+  for (const hs_context::TimedCall &tc : ctx->timed)
     for (int k = 0; k < hs::kTimedKernels; ++k) {
       if (!(tc.mask >> k & 1u)) continue;
       float t = 0;
       HS_HIP(hipEventSynchronize(tc.ev[2 * k + 1]));
       HS_HIP(hipEventElapsedTime(&t, tc.ev[2 * k], tc.ev[2 * k + 1]));
-      ctx->kernel_ms[k] += t;
+      total[k] += t;
     }
-    ++ctx->timed_calls;
-  }
+  // (a query that failed above has changed nothing: the next one has every call)
+  for (int k = 0; k < count; ++k) ms[k] = k < hs::kTimedKernels ? total[k] : 0.0;
+  if (calls) *calls = (int64_t)ctx->timed.size();
   for (const hs_context::TimedCall &tc : ctx->timed) free_events(ctx, tc);
   ctx->timed.clear();
-  for (int k = 0; k < count; ++k) ms[k] = k < hs::kTimedKernels ? ctx->kernel_ms[k] : 0.0;
-  if (calls) *calls = ctx->timed_calls;
-  for (int k = 0; k < hs::kTimedKernels; ++k) ctx->kernel_ms[k] = 0;
-  ctx->timed_calls = 0;
   return HS_OK;
 }
 

@@ -55,3 +55,31 @@ def test_a_timed_call_that_fails_has_no_times(nothing_left_to_fail):
         if not failed:
             break
     assert seen >= 20     # (12 launches of the 8 calls, their events and those of the contexts)
+
+
+def test_reading_the_times_anew_after_a_failure(sampler, nothing_left_to_fail):
+    """Each of the query's HIP calls fails once: the next query has every call once."""
+    b = Block(40, x="f32")
+    failed = 0
+    for n in range(60):
+        with _context({"HS_INJECT_HIP_FAILURE": "-1"}) as ctx:
+            ctx.set_timing(True)
+            for call in calls_of(b, ctx):
+                call()
+            hip.synchronize()
+            _context({"HS_INJECT_HIP_FAILURE": str(n)}).close()
+            print(f"[gpu] query's failure {n}", flush=True)
+            try:
+                ms, calls = ctx.kernel_times()
+            except SamplerError as e:
+                assert e.status == 2
+                failed += 1
+                ms, calls = ctx.kernel_times()
+            else:
+                n = None
+            assert calls == 4 and all(0 < ms[k] < 1000 for k in KERNELS)
+        if n is None:
+            break
+    # a wait and a difference for each launch: 1 of a norm, 3 of the pair (its rows and
+    # its results quantised), 1 of the product, 1 of a norm
+    assert failed == 12
