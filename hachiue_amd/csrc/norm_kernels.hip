@@ -205,6 +205,13 @@ __device__ __forceinline__ void norm_row(const NormArg &n, int C, int t, float (
 // Threads of a workgroup: several rows where a row has one wave.
 template <int G>
 constexpr int kNormThreads = G > 256 ? G : 256;
+// Whether eight gates are activated together (eight chains of instructions and their
+// registers).  One by one, two runs of 1024 threads take 60 registers and not 74, so
+// that a compute unit has two workgroups: 34 us for 4096 rows of 12288 quantised (49),
+// 118 for 4096 of 10240 with a gate and two norms (147).  Fewer threads a row have
+// other workgroups beside them either way: 81 us for 8192 rows of 4096 (84 one by one).
+template <int P, int G>
+constexpr bool kTogether = !(P == 2 && G == 1024);
 // Workgroups of a grid's first dimension (2^32 threads of one are too many).
 constexpr unsigned kGridX = 1u << 16;
 
@@ -228,7 +235,16 @@ __global__ void __launch_bounds__(kNormThreads<G>) block_norm_kernel(BlockNormAr
     for (int j = 0; j < P; ++j) {
       float g[8];
       widen_raw(a.gate.type, raw[j], g);
-      activate<8>(a.act, g);
+      if constexpr (kTogether<P, G>) {
+        activate<8>(a.act, g);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float one[1] = {g[e]};
+          activate<1>(a.act, one);
+          g[e] = one[0];
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[j][e] *= g[e];
     }
