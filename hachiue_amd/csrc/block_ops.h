@@ -67,11 +67,12 @@ struct Int8Args {
 constexpr int kInt8RowK = 4096;
 inline bool int8_row(int32_t M, int32_t K) { return M == 1 && K <= kInt8RowK; }
 // A few float rows, 16 elements a thread of each workgroup, are quantised by the split
-// kernel in less time than a launch before it takes: 4.2 us for 2 rows of 1024 by
-// 1024 channels (5.7), 5.6 for 8 x 1024 by 2048 (6.4), 7.5 for 2 x 4096 by 4096 (9.1),
-// 10.2 for 1 x 8192 by 4096 (11.9), 6.5 for a pair of 8 x 1024 by 2816 (6.6).  More
-// elements a thread, or more workgroups that repeat it: 14.2 for 8 x 4096 by 4096 (9.5),
-// 11.7 for 2 x 2048 by 12288 (11.2).
+// kernel in less time than a launch before it takes: 4.3 us for 2 rows of 1024 by
+// 1024 channels (5.7), 5.6 for 8 x 1024 by 2048 (6.4), 7.7 for 2 x 4096 by 4096 (9.1),
+// 9.9 for 1 x 8192 by 4096 (11.9), 6.6 for a pair of 8 x 1024 by 2816 (6.6).  More
+// elements a thread, or more workgroups that repeat it: 14.2 for 8 x 4096 by 4096 (9.6),
+// 11.7 for 2 x 2048 by 12288 (11.7).  (The rows are waited for together with the
+// first weights: where they were not, the limits would lie elsewhere.)
 constexpr int kInt8KeptRows = 16, kInt8KeptElems = 8192, kInt8KeptN = 4096;
 inline bool int8_kept(int32_t M, int32_t N, int32_t K) {
   return M <= kInt8KeptRows && (int64_t)M * K <= kInt8KeptElems && N <= kInt8KeptN;

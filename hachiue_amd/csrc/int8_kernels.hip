@@ -82,10 +82,10 @@ __device__ __forceinline__ void meet() {
 // their sums are added up in LDS, by one wave while the others go on.  A wave's
 // weights pass through its own part of LDS, 8 KB on their way at a time, without a
 // barrier and on into the next tile, so that nothing runs dry at a tile's end.  A
-// float row is quantised by each workgroup while its first weights are on their
-// way, which saves a launch.  The product is the matrix cores' with the token in
-// all 16 columns: they have 30 times the rate that the weights come at.  151936 x 2048:
-// 48.9 us, 6.4 TB/s (plain reads of as many bytes: 6.1).
+// float row is quantised by each workgroup, which saves a launch: its elements are
+// asked for behind the first weights, and come behind them.  The product is the
+// matrix cores' with the token in all 16 columns: they have 30 times the rate that the
+// weights come at.  151936 x 2048: 48.9 us, 6.4 TB/s (plain reads of as many bytes: 6.1).
 constexpr int kRowWaves = 4;
 
 // The row into LDS, zeros behind K (a multiple of 128 bytes), and its scale.  A thread
@@ -139,7 +139,9 @@ __device__ __forceinline__ void keep_row(const Int8Args &a, int8_t *q, float *sc
 template <int PAIR, bool ONCE>
 __global__ void __launch_bounds__(kRowWaves * 64) int8_row_kernel(Int8Args a) {
   constexpr int W = kRowWaves, kSlot = PAIR * 2048, kLoads = 2 * PAIR, D = 4 / PAIR;
-  // (arrays of their own: the compiler sees that loads are on their way to others)
+  // (Arrays of their own, for the compiler to see that loads are on their way to others.
+  // It does with a pair, but for r0; with one weight it waits for all of a wave's
+  // loads in front of the reads of every slot.)
   __shared__ __align__(1024) int8_t r0[W * kSlot], r1[W * kSlot];
   __shared__ __align__(1024) int8_t r2[D == 4 ? W * kSlot : 16], r3[D == 4 ? W * kSlot : 16];
   __shared__ __align__(16) int8_t q[kInt8RowK];
@@ -266,7 +268,7 @@ __device__ __forceinline__ int kept_piece(int row, int piece, int wide) {
 
 // All float rows, quantised into `q` by a workgroup, zeros behind K, and their scales:
 // a thread has 16 elements (K is a multiple of 16), the rows' largest magnitudes meet
-// in LDS.  `next` is called when the rows are asked for and not yet waited for.
+// in LDS.  `next` is called when the rows are asked for.
 constexpr int kKeepThreads = kInt8KeptElems / 16;
 template <typename F>
 __device__ __forceinline__ void keep_rows(const Int8Args &a, int8_t *q, float *scales, uint32_t *most, F next) {
@@ -317,17 +319,20 @@ __device__ __forceinline__ void keep_rows(const Int8Args &a, int8_t *q, float *s
 // ---- few results: K is split among a workgroup's waves, so that as many compute
 // units as there are tiles of 16 channels (of each weight) and TM tiles of 16 tokens
 // read at once.  A wave's weights and tokens pass through its own part of LDS, four
-// steps of 128 k on their way at a time (two of more rows), without a barrier; the
-// waves' sums are added up at the end.  (Loaded straight to registers, a matrix
-// operand's neighbouring lanes are different rows, and each 16 bytes are a look-up of
-// their own in the cache: 16 tokens of 4096 x 4096 8.8 us, 6.4 so, 33 MB read in all.)
-// KEPT: float rows are quantised by each workgroup while its first weights are on
-// their way, and stay in LDS.
+// steps of 128 k asked for at a time (two of more rows), without a barrier; the
+// waves' sums are added up at the end.  Loads go on behind K's end, as zeros.  (Loaded
+// straight to registers, a matrix operand's neighbouring lanes are different rows, and
+// each 16 bytes are a look-up of their own in the cache: 16 tokens of 4096 x 4096 8.8 us,
+// 6.4 so, 33 MB read in all.)
+// KEPT: float rows are quantised by each workgroup and stay in LDS; its first weights
+// are asked for behind them (and, as built, are there too before rows are widened).
 template <int TM, int PAIR, int WAVES, bool ONCE, bool KEPT>
 __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
   constexpr int T = PAIR * TM, kRows = PAIR + (KEPT ? 0 : TM);   // tiles of 16 rows of a step
   constexpr int D = kRows <= 2 ? 4 : 2, kSlot = kRows * 2048, kLoads = 2 * kRows;
-  // (arrays of their own: the compiler sees that loads are on their way to others)
+  // (Arrays of their own, for the compiler to see that loads are on their way to others.
+  // It does in some turns; as built, all of a wave's loads are waited for in front of
+  // the reads of r0, and with four slots of one weight and a tile of tokens of r2 and r3.)
   __shared__ __align__(1024) int8_t r0[WAVES * kSlot], r1[WAVES * kSlot];
   __shared__ __align__(1024) int8_t r2[D == 4 ? WAVES * kSlot : 16], r3[D == 4 ? WAVES * kSlot : 16];
   static_assert(T * 1024 <= kSlot, "a wave's sums fit its first slot");
@@ -401,7 +406,8 @@ __global__ void __launch_bounds__(WAVES * 64) int8_split_kernel(Int8Args a) {
     load(slot, s + D * WAVES);
   };
   // What the end needs is asked for first: wave j finishes tile j, a lane one token's
-  // four channels.
+  // four channels.  (With one weight the wave has some of it before it asks for
+  // weights, as built.)
   static_assert(TM <= WAVES, "a wave a tile");
   const int m = m0 + wave * 16 + lane % 16, n = n0 + lane / 16 * 4;
   float xs = 0.0f, ws[PAIR][4] = {}, bias[4] = {};
@@ -561,9 +567,9 @@ __global__ void __launch_bounds__(256, BM * BN > 128 * 128 || D > 2 ? 1 : 2) int
       load_to_lds<false>(q, stage + (i * 4 + wave) * 1024);
     }
   };
-  // What the end needs is asked for first, where there are registers to hold it (24
-  // more in 256 x 256 have the compiler move others to memory: 134 us for 4096 tokens
-  // over 20000 x 1024, 142 so).
+  // What the end needs is asked for first (and, as built, there before the first
+  // stage is asked for), where there are registers to hold it (24 more in 256 x 256 have
+  // the compiler move others to memory: 134 us for 4096 tokens over 20000 x 1024, 142 so).
   constexpr bool kAskFirst = BM * BN <= 128 * 128;
   __shared__ float xs_of[BM];
   constexpr int kCols = BN / 2 / PAIR, kLanes = kCols / 8, kRows = 64 / kLanes;
@@ -763,15 +769,17 @@ inline double rounds_time(int64_t count, int slots, double idle, double stage, d
   return rounds * (stage * (double)stages + rest);
 }
 
-// Which kernel.  us at K = 4096 unless said (2048 for 151936 channels and 40000):
-//   one token: 49 over 151936 channels, 7.1 over 4096 with a float row (the split kernel
-//   84, and 6.5 behind the quantising of the row, 3.5)
+// Which kernel.  us in replayed graphs, four weights in turn, binary32 results, at K =
+// 4096 unless said (2048 for 40000 channels and more):
+//   one token: 49 over 151936 channels (the split kernel 84); over 4096 7.4, where the
+//   split kernel takes 6.5, and with a float row 7.5 and 6.3, but 4.2 and 4.4 for K =
+//   2048, 7.4 and 7.9 for a pair of it, 10.9 and 11.2 for a pair of 4096
 //   K split among 8 waves up to 256 strips of 16 channels, among 4 above: 16 tokens
-//   over 4096 6.7 and 7.5, over 8192 11.7 and 10.3 (tiles of four stages 12.6, 12.6)
-//   tiles of 64 x 128: 16 tokens over 16384 16 (split 19), over 151936 56 (95); 64
-//   over 4096 13 (split 9.4), over 16384 18 (27); of two stages, three workgroups a
+//   over 4096 6.4 and 6.9, over 8192 11.3 and 10.2 (tiles of four stages 12.8, 13.0)
+//   tiles of 64 x 128: 16 tokens over 16384 16.5 (split 18.6), over 151936 59 (90); 64
+//   over 4096 13.3 (split 9.5), over 16384 19.3 (27); of two stages, three workgroups a
 //   unit, above a workgroup a unit: 64 over 40000 23 (four stages 27), over 4096 20 (13)
-//   tiles of 128 x 128 of four stages: 1024 over 4096 22 (two stages 26, 64 x 128 25)
+//   tiles of 128 x 128 of four stages: 1024 over 4096 25 (two stages 28, 64 x 128 30)
 template <int PAIR>
 hipError_t int8(const Int8Args &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
   if (int8_row(a.M, a.K)) return row<PAIR>(a, stream, ev, done);

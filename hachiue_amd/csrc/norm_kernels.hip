@@ -8,9 +8,18 @@
 // element.  A row is held in the registers of its threads (64 to 1024 of them, 8
 // elements of a tensor in one load, wherever rows start), so
 // that the norms' sums, up to five one after the other, read nothing again.  All
-// sums are binary32: each thread's own elements, then a tree.  8192 rows of 4096, x
-// and out bfloat16, residual and s binary32: 78 us, 5.2 TB/s (a copy of 1 GB: 5.05);
-// 4096 rows of 12288 bfloat16 in 8 bits: 35 us, 4.3 TB/s.
+// sums are binary32: each thread's own elements one after the other, a tree over the
+// lanes of a wave, the waves' one after the other; the number of threads depends on
+// the number of rows too.  The kernel's time over three inputs in turn: 8192 rows of
+// 4096, x and out bfloat16, residual and s binary32, both norms, 78 us, 5.2 TB/s, and
+// 81 with a gate for each channel (a copy of 1 GB: 5.05 to 5.1); 4096 rows of 12288
+// bfloat16 in 8 bits 34 us, 4.4 TB/s.
+//
+// Few rows wait: the types are known at run time, and as built a tensor's elements
+// are there before the next tensor's are asked for, and both before the gate's and
+// the norms' parameters are (their own below).  Widths that 8 does not divide have a
+// second chain of such loads, element by element: 300 rows of 1001 with a gate and two
+// norms 6 us, 4096 in one row 4.2.
 #include "block_ops.h"
 
 #include <hip/hip_ext.h>
@@ -156,7 +165,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *slot, int t) {
 }
 
 // `early`: the weights are asked for before the sums are formed, not behind them (a
-// lone row's time is its chain of waits: 4.9 us, 5.2 so).
+// lone row's time is its chain of waits: 4.9 us, 5.2 so), if behind the row itself.
 template <int P, int G, bool WHOLE>
 __device__ __forceinline__ void norm_row(const NormArg &n, int C, int t, float (&v)[P][8], float (*slots)[16]) {
   if (n.kind == kNormNone) return;
@@ -314,10 +323,12 @@ hipError_t launch(const BlockNormArgs &a, hipStream_t stream, hipEvent_t *ev, hi
 }  // namespace
 
 // Threads of a row: two runs of eight elements each, so that many rows are on their
-// way at a time; one where there are few rows, which end sooner.  us, with 256 x 2,
-// 512 x 1, 512 x 2 and 1024 x 2 runs: 8192 rows of 4096, bfloat16 and binary32 in and
-// out, 76, 76, 78, 90; 1 row 4.7, 4.3, 5.0, 4.2; 4096 rows of 12288 quantised -, -, -,
-// 38 (512 x 3: 40, 256 x 6: 40); 20000 rows of 512 with 64 x 1 16, 256 x 1 26.
+// way at a time; one where there are few rows, which end sooner.  Kernel times in us
+// over three inputs in turn, with 256 x 2, 512 x 1, 512 x 2 and 1024 x 2 runs: 8192 rows
+// of 4096, bfloat16 and binary32 in and out, 78, 76, 76, 86; 300 rows 4.9, 5.1, 4.9, 5.6;
+// 1 row 4.0 to 4.5 with any.  4000 rows of 8192 with 512 x 2 77, 1024 x 1 83.  4096 rows of
+// 12288 quantised with 1024 x 2 34 (512 x 3: 36, 256 x 6: 46); 20000 rows of 512 with 64 x 1
+// 14.5, 256 x 1 22.6, of 1024 with 64 x 2 32.5, 256 x 1 34.7, where 300 of 1001 take 7.5 and 6.
 hipError_t launch_block_norm(const BlockNormArgs &a, hipStream_t stream, hipEvent_t *ev, hipEvent_t done) {
   const int C = a.C;
   if (C <= 512) return launch<1, 64>(a, stream, ev, done);

@@ -1,10 +1,12 @@
 """Binary64 forms of the norms between blocks and of the 8-bit products, with
 bounds on what binary32 arithmetic can be off from them.
 
-u = 2^-24 is half a step of binary32.  A sum of C terms is formed by threads of
-at most 32 terms each and a tree of at most 12 levels: each term passes at most
-44 additions, so that a sum is off by at most 44 u times the sum of its terms'
-magnitudes (to first order; SUM leaves room for the products and the division).
+u = 2^-24 is half a step of binary32.  A sum of C terms is formed by up to 1024 threads
+of at most 32 terms each, one after the other, then over the 64 lanes of a wave in
+six levels, then over up to 16 waves one after the other: each term passes at most 32
++ 6 + 16 = 54 additions, so that a sum is off by at most 54 u times the sum of its
+terms' magnitudes (to first order; squares are added unrounded).  SUM leaves ten
+more, for the division and the second order.
 """
 from __future__ import annotations
 
