@@ -519,8 +519,9 @@ typedef struct hs_norm {
  * and zeros, so that its products are NaN.  With both norms HS_NORM_NONE
  * the call quantises or converts rows.  sum and out may be x, residual or a gate of
  * as many rows themselves (same data, type and stride); otherwise they overlap
- * nothing.  cols up to 32768, rows up to 2^24.  Asynchronous on `stream`, no
- * workspace; may be captured. */
+ * nothing.  cols up to 32768, rows up to 2^24.  The order of a norm's sums depends on
+ * rows and cols: a row may differ by rounding in calls of other sizes.  Asynchronous
+ * on `stream`, no workspace; may be captured. */
 typedef struct hs_block_norm {
   int32_t rows, cols;
   hs_rows x;
@@ -586,7 +587,8 @@ int hs_lm_head_norm_sample_device(hs_context *ctx, const hs_block_norm *norm,
  * products, ms[19] the quantising of their results; a kernel a call did not
  * launch adds 0)
  * and the number of
- * timed calls, and resets the totals. */
+ * timed calls, and resets the totals.  A call that failed counts as none; a query
+ * that fails resets nothing. */
 int hs_context_set_timing(hs_context *ctx, int enable);
 int hs_context_kernel_times(hs_context *ctx, double *ms, int32_t count, int64_t *calls);
 
